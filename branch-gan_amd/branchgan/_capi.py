@@ -15,6 +15,7 @@ BG_F32, BG_BF16 = 0, 1
 MAX_TOPN, MAX_BLOCKED, MAX_SLOTS, MAX_GATHER = 64, 8, 64, 80
 MAX_RANKS = 8
 RL_DIAG_COUNT = 20
+POLICY_STATS = 8
 
 c_i64, c_i32, c_f32, c_vp, c_sz = ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
 c_f64 = ctypes.c_double
@@ -45,6 +46,16 @@ class DiscLossShape(ctypes.Structure):
 class RlLossShape(ctypes.Structure):
     _fields_ = [("B", c_i32), ("S", c_i32), ("N", c_i32), ("K", c_i32), ("wA", c_f32), ("wB", c_f32), ("wC", c_f32),
                 ("ignore_input", c_i32), ("ignore_alt", c_i32), ("use_depth_mask", c_i32), ("probs_input", c_i32)]
+
+
+class KvCache(ctypes.Structure):
+    _fields_ = [("bits", c_i32), ("B", c_i32), ("H", c_i32), ("Dh", c_i32), ("capacity", c_i32), ("reserved", c_i32),
+                ("c_sb", c_i64), ("c_sh", c_i64)]
+
+
+class PolicyShape(ctypes.Structure):
+    _fields_ = [("dtype", c_i32), ("reserved", c_i32), ("rows", c_i64), ("V", c_i64), ("x_stride", c_i64), ("ref_stride", c_i64),
+                ("temperature", c_f64), ("clip_low", c_f64), ("clip_high", c_f64), ("kl_coef", c_f64)]
 
 
 class ReduceDesc(ctypes.Structure):
@@ -110,6 +121,14 @@ SIGNATURES = {
     "bg_dual_head_advantages": (c_i32, [c_vp] * 4 + [c_i32] * 3 + [c_f32] * 3 + [c_i32] * 2 + [c_f32] * 2 + [c_vp] * 6 + [c_vp]),
     "bg_reinforce_terms_fwd": (c_i32, [c_vp, c_vp, c_vp, c_i64, c_i32, c_f32, c_f32, c_vp, c_vp]),
     "bg_reinforce_terms_bwd": (c_i32, [c_vp, c_vp, c_vp, c_i64, c_i32, c_f32, c_f32, c_vp, c_vp, c_vp]),
+    "bg_kv_cache_tile_bytes": (c_sz, [c_i32, c_i32]),
+    "bg_kv_cache_append": (c_i32, [ctypes.POINTER(KvCache), c_vp, c_vp, c_vp, c_i32, c_i32] + [c_i64] * 6 + [c_vp] * 3),
+    "bg_kv_cache_read": (c_i32, [ctypes.POINTER(KvCache), c_vp, c_vp, c_vp, c_i32, c_i32] + [c_i64] * 3 + [c_vp] * 3),
+    "bg_kv_cache_attn_workspace_bytes": (c_sz, [ctypes.POINTER(KvCache), c_i32, c_i32, c_i32]),
+    "bg_kv_cache_attn_fwd": (c_i32, [ctypes.POINTER(KvCache), c_vp, c_vp, c_i32, c_i32, c_i32, c_i64, c_i64, c_i64, c_vp, c_vp, c_i32, c_f32,
+                                     c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_sz, c_vp]),
+    "bg_policy_loss_fwd": (c_i32, [ctypes.POINTER(PolicyShape)] + [c_vp] * 13),
+    "bg_policy_loss_bwd": (c_i32, [ctypes.POINTER(PolicyShape)] + [c_vp] * 7),
     "bg_graph_node_census": (c_i32, [c_vp] + [ctypes.POINTER(c_i32)] * 4),
     "bg_graph_replace_memset_nodes": (c_i32, [c_vp, ctypes.POINTER(c_i32)]),
     "bg_rl_loss_bwd": (c_i32, [ctypes.POINTER(RlLossShape)] + [c_vp] * 7 + [c_vp, c_vp, c_vp, c_vp]),

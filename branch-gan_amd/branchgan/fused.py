@@ -1196,6 +1196,10 @@ def packed_attention(qkv, lp, scale, out_for=None, qkv_from=None, p_drop=0.0, dr
     add_layer_norm).  drop_site / drop_row0: the dropout masks as functions of (site, logical row) - text rows 0.., tree rows
     from drop_row0 - instead of the call order (ops.drop_site)."""
     B, T, _, H, Dh = qkv.shape
+    if getattr(lp, "cache", None) is not None:          # decoding over a quantised cache (models.CachePast): no gradient
+        from .models import cached_attention_core
+        q, k, v = [qkv[:, :, i].permute(0, 2, 1, 3) for i in range(3)]
+        return cached_attention_core(q, k, v, lp, scale, p_drop=p_drop).permute(0, 2, 1, 3).reshape(B, T, H * Dh), (k, v)
     extra = {"att_buf": _x_slab_for(out_for, B * T, H * Dh, qkv.dtype, qkv.device), "qkv_from": _pass_of(qkv_from, qkv.device),
              "p_drop": p_drop, "drop_site": drop_site, "drop_row0": drop_row0}
     if lp is None:

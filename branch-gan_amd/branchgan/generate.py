@@ -13,12 +13,17 @@ branch node at the single branch point `S - 1` whose ancestors are the tokens ge
 call as a training branch step with K = 1, no concatenation per token.  Every `FOLD` tokens the slots are folded into the text
 K/V (one concatenation per layer per 32 tokens) so that sequences longer than BG_MAX_SLOTS decode too.  Tokens are chosen by
 `bg_topn_select`: arg-max, or an exponential race `p / e` (`e ~ Exp(1)`), which draws from the categorical distribution p.
+
+With `cache_bits` 4 or 8 the keys / values live in a quantised cache instead (branchgan.kvcache): 0.5625 / 1.0625 bytes per value,
+new tokens written in place, no folding and no copies as the sequence grows.  The prompt itself is scored from its own keys /
+values as ever; the decoded tokens read all of the cache through its codes.
 """
 import numpy as np
 import torch
 
 from . import ops
-from .models import BranchPast
+from .kvcache import QuantizedKVCache
+from .models import BranchPast, CachePast, dropout_active
 
 FOLD = 32
 
@@ -32,10 +37,13 @@ def _lm_of(model):
 
 @torch.no_grad()
 def generate(model, input_ids, max_new_tokens=128, do_sample=False, temperature=1.0, pad_token_id=0, eos_token_id=None, num_beams=1,
-             num_return_sequences=1, generator=None, **unused):
+             num_return_sequences=1, generator=None, cache_bits=None, return_logprobs=False, **unused):
     """HF-`generate`-shaped: (B, S) prompt ids -> (B, S + max_new_tokens) ids, prompt included.  Greedy (`do_sample=False`) or
     ancestral sampling at `temperature`; after `eos_token_id` a sequence is filled with `pad_token_id`.  Beam search and
-    several return sequences are not offered.  `generator`: a torch.Generator on the device for reproducible sampling."""
+    several return sequences are not offered.  `generator`: a torch.Generator on the device for reproducible sampling.
+    `cache_bits` 4 or 8: decode over a quantised cache (models without dropout only).  `return_logprobs=True`: -> (ids, log-probs of the
+    new tokens (B, max_new_tokens) fp32 under the policy that chose them - softmax(logits / temperature) when sampling,
+    softmax(logits) when greedy -, 0 where a finished sequence was filled up): the `oldLogProbs` of losses.clippedPolicyLoss."""
     if num_beams != 1 or num_return_sequences != 1:
         raise NotImplementedError("generate: num_beams = num_return_sequences = 1 only")
     if do_sample and temperature <= 0:
@@ -48,6 +56,15 @@ def generate(model, input_ids, max_new_tokens=128, do_sample=False, temperature=
     if S + max_new_tokens > n_pos:
         raise ValueError(f"generate: {S} prompt + {max_new_tokens} new tokens exceed the model's {n_pos} positions")
 
+    if cache_bits is not None and dropout_active(lm):
+        raise NotImplementedError("generate: attention over a quantised cache draws no dropout; decode a model whose dropout is off")
+    logps = []
+
+    def score(logits, tok):                                         # log-probs of the tokens select() chose
+        if return_logprobs:
+            x = logits.float() / temperature if do_sample else logits
+            logps.append(torch.where(done, torch.zeros((), device=dev), ops.softmax_stats(x, tok)[1]))
+
     def select(logits):                                             # (B, V) -> (B, 1)
         if not do_sample:
             return ops.topn_select(logits, 1, blocked_value=float("-inf"))
@@ -57,11 +74,19 @@ def generate(model, input_ids, max_new_tokens=128, do_sample=False, temperature=
 
     out = lm(input_ids=ids, use_cache=True, returnLmLogits=True)
     L = len(out.past_key_values)
-    text = [out.past_key_values[l] for l in range(L)]
-    slots = [[] for _ in range(L)]
+    if cache_bits is not None:
+        k0 = out.past_key_values[0][0]
+        cache = QuantizedKVCache(L, B, k0.shape[1], S + max_new_tokens, k0.shape[3], bits=cache_bits, device=dev)
+        for l in range(L):
+            ops.kv_cache_append(cache.layer(l), *out.past_key_values[l])
+        held = torch.full((B,), S, dtype=torch.int32, device=dev)
+    else:
+        text = [out.past_key_values[l] for l in range(L)]
+        slots = [[] for _ in range(L)]
     s_text = S
     done = torch.zeros(B, 1, dtype=torch.bool, device=dev)
     tok = select(out.logits[:, -1])
+    score(out.logits[:, -1], tok)
     new = []
     for t in range(max_new_tokens):
         if eos_token_id is not None:
@@ -70,6 +95,13 @@ def generate(model, input_ids, max_new_tokens=128, do_sample=False, temperature=
         new.append(tok)
         if t == max_new_tokens - 1:
             break
+        if cache_bits is not None:
+            past = CachePast(cache, held, max_keys=S + t + 1)
+            step = lm(input_ids=tok, position_ids=held.view(B, 1), textualPast=past, returnLmLogits=True)
+            held = held + 1
+            tok = select(step.logits[:, -1])
+            score(step.logits[:, -1], tok)
+            continue
         d = len(slots[0])
         if d == FOLD:                                               # fold the generated tokens' K/V into the text
             text = [(torch.cat([text[l][0]] + [s[0] for s in slots[l]], dim=2), torch.cat([text[l][1]] + [s[1] for s in slots[l]], dim=2))
@@ -82,7 +114,9 @@ def generate(model, input_ids, max_new_tokens=128, do_sample=False, temperature=
         for l in range(L):
             slots[l] = slots[l] + [step.past_key_values[l]]
         tok = select(step.logits[:, -1])
-    return torch.cat([ids] + new, dim=1)
+        score(step.logits[:, -1], tok)
+    seq = torch.cat([ids] + new, dim=1)
+    return (seq, torch.cat(logps, dim=1)[:, :max_new_tokens]) if return_logprobs else seq
 
 
 def generateTexts(generator, data, settings, device, tokenizer=None, generationLength=128, startIndex=None, maxNumSamples=None,

@@ -154,3 +154,15 @@ def calcGeneratorLoss(gannSetup, inputIDs, generatorLogits, generatorProbs, disc
     genLosses['loss-RL'] = rlLoss
     genLosses['loss'] = genLosses['loss-MLE'] * gannSetup.generatorMleLossWeight + rlLoss * gannSetup.generatorRlLossWeight
     return genLosses
+
+
+def clippedPolicyLoss(logits, ids, oldLogProbs, advantages, mask=None, refLogProbs=None, refLogits=None, clipRange=(0.2, 0.2), klWeight=0.0,
+                      temperature=1.0, denominator=None):
+    """Policy-gradient loss of sampled tokens against the policy that sampled them (no counterpart in the reference, whose
+    REINFORCE loss, ReinforceLoss.py:21-52, is on-policy): with ratio = exp(logp - oldLogProbs),
+        max(-advantages * ratio, -advantages * clamp(ratio, 1 - clipRange[0], 1 + clipRange[1])) + klWeight * KL(policy | reference),
+    summed over the tokens mask counts and divided by their number (or by denominator).  What to use for tokens that
+    `generate(..., return_logprobs=True)` sampled - behind a quantised cache, some optimizer steps ago, or both.  One reading of
+    the logits forward, one backward (bg_policy_loss_*).  -> (loss, logProbs, kl), the last two per token, without gradient."""
+    return ops.policy_loss(logits, ids, oldLogProbs, advantages, weights=mask, ref_logp=refLogProbs, ref_logits=refLogits,
+                           clip_low=clipRange[0], clip_high=clipRange[1], kl_coef=klWeight, temperature=temperature, denominator=denominator)

@@ -45,6 +45,28 @@ class BranchPast:
                                ctx_len=self.ctx_len, paths=self.paths, n_query_nodes=self.n_query_nodes, merged_text=self.merged_text)
 
 
+class CachePast(BranchPast):
+    """Context of one decoding forward over a quantised cache (branchgan.kvcache.QuantizedKVCache): every layer appends the keys /
+    values of its T new tokens and attends over what it then holds.  start int32 (B,): tokens held before; counts int32 (B,) or
+    None: how many of the T belong to each sequence; max_keys: the most any sequence holds after the append."""
+
+    def __init__(self, cache, start, counts=None, max_keys=None):
+        super().__init__(text=None, ancestors=None, ctx_len=start, paths=None)
+        self.cache, self.start, self.counts, self.max_keys = cache, start, counts, max_keys
+
+    def layer(self, i):
+        return SimpleNamespace(cache=self.cache.layer(i), ctx_len=self.ctx_len, start=self.start, counts=self.counts, max_keys=self.max_keys,
+                               n_query_nodes=1, merged_text=0)
+
+
+def cached_attention_core(q, k, v, lp, scale, return_weights=False, p_drop=0.0):
+    """q, k, v (B,H,T,Dh) of the new tokens, lp = layer view of a CachePast: append, then attend.  -> (B,H,T,Dh)."""
+    if return_weights or p_drop:
+        raise NotImplementedError("attention over a quantised cache: no attention weights, no dropout")
+    ops.kv_cache_append(lp.cache, k, v, start=lp.start, counts=lp.counts)
+    return ops.kv_cache_attention(q, lp.cache, start=lp.start, counts=lp.counts, scale=scale, max_keys=lp.max_keys)[0]
+
+
 def descriptor_from_bool_mask(mask, K, C):
     """Reference mask (B,1,K,C+1) -> (ctx_len (K,) int32, n_anc).  Accepts exactly the T1 pattern
     [text prefix | n_anc identity blocks | self column] (MultiStepPrediction.py:92-127), identical over the batch."""
@@ -85,6 +107,8 @@ def branch_attention_core(q, k, v, lp, scale, return_weights=False, p_drop=0.0):
     the softmax weights the reference materialises ((B,H,K,C+1) for one query node, (B,H,NQ,K,W) for several), rebuilt by
     bg_branch_attn_weights from the forward's log-sum-exp.  p_drop: dropout on the attention probabilities, inside the
     kernel (the weights handed out are then the ones after dropout, as in the reference)."""
+    if getattr(lp, "cache", None) is not None:
+        return cached_attention_core(q, k, v, lp, scale, return_weights, p_drop)
     NQ = lp.n_query_nodes
     K = q.shape[2] // NQ
     q5, k5, v5 = q.unflatten(2, (NQ, K)), k.unflatten(2, (NQ, K)), v.unflatten(2, (NQ, K))

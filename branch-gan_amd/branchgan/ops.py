@@ -799,3 +799,198 @@ def reinforce_terms(probs, advantages, mask_zone_c=None, use_min_prob_limit=Fals
     """bg_reinforce_terms_* (ReinforceLoss.py:21-52): per-element REINFORCE loss, mirrored inside zone C when a mask is given;
     differentiable in probs."""
     return _ReinforceTerms.apply(probs, advantages, mask_zone_c, use_min_prob_limit, neg_push_prob_limit, eps)
+
+
+# ---------------------------------------------------------------------------------------------------
+# Key / value cache in 4 or 8 bits: written as tokens come, read back, attended.  No gradient: decoding only.
+# ---------------------------------------------------------------------------------------------------
+KV_TILE = 32          # keys per tile of the cache
+
+
+class KVCacheLayer:
+    """One layer's cache: `data` uint8 (B, H, tiles * tile bytes) on the GPU, `bits` 4 or 8 (branchgan.kvcache.QuantizedKVCache
+    makes them).  The bytes' order is the library's own; kv_cache_read gives the values."""
+
+    def __init__(self, data, bits, head_dim, capacity):
+        tile = C.lib().bg_kv_cache_tile_bytes(int(bits), int(head_dim))
+        if tile == 0:
+            raise ValueError(f"a quantised cache takes bits 4 or 8 and head sizes 32, 64, 128 or 256, got bits={bits}, head_dim={head_dim}")
+        if not 0 < int(capacity) < 1 << 30:
+            raise ValueError(f"cache capacity {capacity}")
+        if data.dtype != torch.uint8 or data.dim() != 3 or data.stride(-1) != 1 or data.shape[-1] != -(-int(capacity) // KV_TILE) * tile:
+            raise ValueError(f"cache data must be uint8 (batch, heads, {-(-int(capacity) // KV_TILE) * tile}) with a dense last dimension")
+        self.data, self.bits, self.head_dim, self.capacity = data, int(bits), int(head_dim), int(capacity)
+
+    def _struct(self):
+        sh = C.KvCache()
+        sh.bits, sh.B, sh.H, sh.Dh, sh.capacity = self.bits, self.data.shape[0], self.data.shape[1], self.head_dim, self.capacity
+        sh.c_sb, sh.c_sh = self.data.stride(0), self.data.stride(1)
+        return sh
+
+
+def _kv_rows(name, t, B, dev):
+    """start / counts of the cache calls: int32 (B,) on the cache's device, or None."""
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or t.shape != (B,) or t.device != dev:
+        raise ValueError(f"{name} must be int32 of shape ({B},) on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.contiguous()
+
+
+def _no_grad_wanted(what, *tensors):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
+
+
+def kv_cache_append(layer, k, v, start=None, counts=None):
+    """bg_kv_cache_append: quantises k, v (B, H, T, Dh) - fp32 or bf16, any strides - into the cache at positions start[b] .. .
+    start int32 (B,) or None (= 0): tokens each sequence holds already; counts int32 (B,) or None (= T): how many of the T are
+    the sequence's own, the rest is padding.  Positions outside the cache and padding are not written."""
+    C.require_cuda(layer.data, k, v, start, counts)
+    B, H = layer.data.shape[:2]
+    if k.dim() != 4 or k.shape != v.shape or k.shape[0] != B or k.shape[1] != H or k.shape[3] != layer.head_dim:
+        raise ValueError(f"k and v must be ({B}, {H}, T, {layer.head_dim}), got {tuple(k.shape)} and {tuple(v.shape)}")
+    if k.dtype != v.dtype or k.device != layer.data.device or v.device != layer.data.device:
+        raise ValueError(f"k and v must share one dtype and the cache's device, got {k.dtype} on {k.device}, {v.dtype} on {v.device}")
+    _no_grad_wanted("kv_cache_append", k, v)
+    start, counts = _kv_rows("start", start, B, k.device), _kv_rows("counts", counts, B, k.device)
+    code, T = C.dtype_code(k), k.shape[2]
+    if T == 0 or B == 0 or H == 0:
+        return
+    k, v = _unit_last(k), _unit_last(v)
+    sh = layer._struct()
+    with torch.cuda.device(k.device), _timed("kv_cache_append"):
+        C.check(C.lib().bg_kv_cache_append(ctypes.byref(sh), C.ptr(layer.data), C.ptr(k), C.ptr(v), code, T, *k.stride()[:3], *v.stride()[:3],
+                                           C.ptr(start), C.ptr(counts), C.stream_ptr()), "bg_kv_cache_append")
+
+
+def kv_cache_read(layer, n, start=None, counts=None, dtype=torch.bfloat16):
+    """bg_kv_cache_read -> k, v (B, H, n, Dh) in dtype: the values held at positions start[b] .. start[b] + n - 1; zeros for rows
+    t >= counts[b] and outside the cache."""
+    C.require_cuda(layer.data, start, counts)
+    B, H = layer.data.shape[:2]
+    dev = layer.data.device
+    start, counts = _kv_rows("start", start, B, dev), _kv_rows("counts", counts, B, dev)
+    if int(n) < 0:
+        raise ValueError(f"kv_cache_read: n = {n}")
+    k, v = [torch.empty((B, H, int(n), layer.head_dim), dtype=dtype, device=dev) for _ in range(2)]
+    code = C.dtype_code(k)
+    if k.numel() == 0:
+        return k, v
+    sh = layer._struct()
+    with torch.cuda.device(dev), _timed("kv_cache_read"):
+        C.check(C.lib().bg_kv_cache_read(ctypes.byref(sh), C.ptr(layer.data), C.ptr(k), C.ptr(v), code, int(n), *k.stride()[:3], C.ptr(start),
+                                         C.ptr(counts), C.stream_ptr()), "bg_kv_cache_read")
+    return k, v
+
+
+def kv_cache_attention(q, layer, start=None, counts=None, scale=None, max_keys=None):
+    """bg_kv_cache_attn_fwd: attention of T new tokens, whose keys / values the cache holds already.  q (B, Hq, T, Dh), Hq a multiple
+    of the cache's heads; token t of sequence b sees keys 0 .. start[b] + t; start / counts as kv_cache_append got them.  Rows that
+    see nothing (padding) are zeros.  max_keys: the most keys any sequence holds after the append, if the host knows it (default:
+    the capacity); keys past it are not read.  -> (out like q [a (B, T, Hq, Dh)-contiguous view], lse fp32 (B, Hq, T))."""
+    C.require_cuda(q, layer.data, start, counts)
+    B, H = layer.data.shape[:2]
+    if q.dim() != 4 or q.shape[0] != B or q.shape[3] != layer.head_dim or q.shape[1] == 0 or q.shape[1] % max(H, 1):
+        raise ValueError(f"q must be ({B}, a multiple of {H} heads, T, {layer.head_dim}), got {tuple(q.shape)}")
+    if q.device != layer.data.device:
+        raise ValueError(f"q is on {q.device}, the cache on {layer.data.device}")
+    _no_grad_wanted("kv_cache_attention", q)
+    start, counts = _kv_rows("start", start, B, q.device), _kv_rows("counts", counts, B, q.device)
+    max_keys = layer.capacity if max_keys is None else int(max_keys)
+    if not 0 < max_keys <= layer.capacity:
+        raise ValueError(f"max_keys {max_keys} is not in 1 .. {layer.capacity} (the capacity)")
+    code, (_, Hq, T, Dh) = C.dtype_code(q), q.shape
+    out = torch.empty((B, T, Hq, Dh), dtype=q.dtype, device=q.device).permute(0, 2, 1, 3)
+    lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device)
+    if out.numel() == 0:
+        return out, lse
+    q = _unit_last(q)
+    if scale is None:
+        scale = 1.0 / math.sqrt(Dh)
+    sh = layer._struct()
+    with torch.cuda.device(q.device), _timed("kv_cache_attention"):
+        # a workspace of the call's own (the caching allocator's, so a captured graph keeps its own too): calls on several streams
+        # and graphs replayed side by side must not share one
+        ws_bytes = C.lib().bg_kv_cache_attn_workspace_bytes(ctypes.byref(sh), Hq, T, max_keys)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+        C.check(C.lib().bg_kv_cache_attn_fwd(ctypes.byref(sh), C.ptr(layer.data), C.ptr(q), code, Hq, T, *q.stride()[:3], C.ptr(start), C.ptr(counts),
+                                             max_keys, float(scale), C.ptr(out), *out.stride()[:3], C.ptr(lse), C.ptr(ws), ws_bytes,
+                                             C.stream_ptr()), "bg_kv_cache_attn_fwd")
+    return out, lse
+
+
+# ---------------------------------------------------------------------------------------------------
+# Clipped policy loss with a KL term
+# ---------------------------------------------------------------------------------------------------
+class _PolicyLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, old_logp, advantages, weights, ref_logp, ref_logits, denominator, clip_low, clip_high, kl_coef, temperature):
+        V = logits.shape[-1]
+        dense = lambda t: t if t.stride(0) >= V or t.shape[0] == 1 else t.contiguous()       # expanded rows
+        x = dense(_rows_2d(logits.detach()))
+        y = dense(_rows_2d(ref_logits.detach())) if ref_logits is not None else None
+        rows, dev = x.shape[0], x.device
+        ids = ids.reshape(rows).to(torch.int64).contiguous()
+        flat = lambda t: None if t is None else _f32c(t.detach().reshape(rows))
+        sh = C.PolicyShape()
+        sh.dtype, sh.rows, sh.V = C.dtype_code(x), rows, V
+        sh.x_stride, sh.ref_stride = max(x.stride(0), V), (max(y.stride(0), V) if y is not None else 0)
+        sh.temperature, sh.clip_low, sh.clip_high, sh.kl_coef = temperature, clip_low, clip_high, kl_coef
+        out = torch.empty(1, dtype=torch.float32, device=dev)
+        logp, kl = [torch.empty(rows, dtype=torch.float32, device=dev) for _ in range(2)]
+        stats = torch.empty(rows * C.POLICY_STATS + 1, dtype=torch.float32, device=dev)
+        args = [flat(t) for t in (old_logp, ref_logp, advantages, weights)] + [denominator]
+        with torch.cuda.device(dev), _timed(f"policy_loss_fwd[{rows}]"):
+            C.check(C.lib().bg_policy_loss_fwd(ctypes.byref(sh), C.ptr(x), C.ptr(y), C.ptr(ids), *[C.ptr(t) for t in args], C.ptr(out), C.ptr(logp),
+                                               C.ptr(kl), C.ptr(stats), C.stream_ptr()), "bg_policy_loss_fwd")
+        ctx.save_for_backward(x, ids, stats, *(() if y is None else (y,)))
+        ctx.sh, ctx.in_shape = sh, logits.shape
+        loss, logp, kl = out.view(()), logp.view(logits.shape[:-1]), kl.view(logits.shape[:-1])
+        ctx.mark_non_differentiable(logp, kl)
+        return loss, logp, kl
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_loss, _g_logp, _g_kl):
+        x, ids, stats = ctx.saved_tensors[:3]
+        y = ctx.saved_tensors[3] if len(ctx.saved_tensors) > 3 else None
+        g = g_loss.reshape(1).contiguous().float()
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        with torch.cuda.device(x.device), _timed(f"policy_loss_bwd[{x.shape[0]}]"):
+            C.check(C.lib().bg_policy_loss_bwd(ctypes.byref(ctx.sh), C.ptr(x), C.ptr(y), C.ptr(ids), C.ptr(stats), C.ptr(g), C.ptr(dx),
+                                               C.stream_ptr()), "bg_policy_loss_bwd")
+        return (dx.view(ctx.in_shape),) + (None,) * 11
+
+
+def policy_loss(logits, ids, old_logp, advantages, weights=None, ref_logp=None, ref_logits=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0,
+                temperature=1.0, denominator=None):
+    """Clipped policy loss with a KL term (bg_policy_loss_*), differentiable in logits (..., V) fp32 / bf16.  ids (...) int64: the
+    sampled tokens; old_logp (...): their log-probs when they were sampled; advantages (...); weights (...) or None: per token,
+    0 = does not count; ref_logits (like logits) -> the KL over the vocabulary, or ref_logp (...) -> exp(d) - d - 1 of the
+    sampled token, d = ref_logp - logp.  All log-probs are those of softmax(logits / temperature).  denominator: what the sum over tokens
+    is divided by (a number, or a one-element tensor on the device - a token count over micro-batches or ranks); default the
+    sum of the weights that count.  -> (loss fp32 scalar, logp (...), kl (...); the last two carry no gradient)."""
+    C.require_cuda(logits, ids, old_logp, advantages, weights, ref_logp, ref_logits)
+    if logits.dim() < 2 or logits.numel() == 0:
+        raise ValueError(f"policy_loss: logits must be (..., V) with at least one row, got {tuple(logits.shape)}")
+    for name, t in (("ids", ids), ("old_logp", old_logp), ("advantages", advantages), ("weights", weights), ("ref_logp", ref_logp)):
+        if t is not None and (t.shape != logits.shape[:-1] or t.device != logits.device):
+            raise ValueError(f"policy_loss: {name} must be {tuple(logits.shape[:-1])} on {logits.device}, got {tuple(t.shape)} on {t.device}")
+    if ids.is_floating_point() or ids.dtype == torch.bool:
+        raise TypeError(f"policy_loss: ids must be integers, got {ids.dtype}")
+    if ref_logits is not None and (ref_logits.shape != logits.shape or ref_logits.dtype != logits.dtype or ref_logits.device != logits.device):
+        raise ValueError("policy_loss: ref_logits must be like logits in shape, dtype and device")
+    if ref_logits is not None and ref_logp is not None:
+        raise ValueError("policy_loss: ref_logits or ref_logp, not both")
+    if not temperature > 0 or not clip_low >= 0 or not clip_high >= 0:
+        raise ValueError(f"policy_loss: temperature {temperature} must be positive, the clip range ({clip_low}, {clip_high}) not negative")
+    if denominator is not None:
+        if torch.is_tensor(denominator):
+            if denominator.numel() != 1 or denominator.device != logits.device:
+                raise ValueError("policy_loss: denominator must be a number or one element on the logits' device")
+            denominator = _f32c(denominator.detach().reshape(1))
+        else:
+            denominator = torch.full((1,), float(denominator), dtype=torch.float32, device=logits.device)
+    return _PolicyLoss.apply(logits, ids, old_logp, advantages, weights, ref_logp, ref_logits, denominator, float(clip_low), float(clip_high),
+                             float(kl_coef), float(temperature))

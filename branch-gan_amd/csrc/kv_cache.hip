@@ -1,0 +1,382 @@
+// The quantised key / value cache: bg_kv_cache_append writes new tokens into it, bg_kv_cache_read gives back the values it holds.
+//
+// Per (token, head, 32 channels), a = the largest magnitude, L = 7 or 127:
+//   s = bf16(fp32(a / L)),  c = clamp(round-half-even(x / s), -L, L),  the value held is s * c (exact in fp32: 8 + 7 bits at most)
+// s is 0 (the group reads as zeros) when it would be subnormal; a group with a NaN, an infinity or a magnitude above 2^127 gets
+// s = NaN and reads as NaN, so a broken activation shows instead of turning into a large finite number.
+// The code is that of the REAL quotient x / s, not of a rounded one: with r = 1 / s correctly rounded, q0 = x r, q = q0 + (x - q0 s) r
+// is the correctly rounded quotient (Markstein).  For bf16 x it lands on k + 1/2 only if the real quotient does (both have 8
+// significant bits); for fp32 x the sign of x - q s decides there.
+//
+// Bound by HBM for prompts (bytes in + 0.56 or 1.06 bytes per value out), by latency for one token.
+#include "kv_cache.h"
+
+namespace bg {
+
+__device__ __forceinline__ uint16_t f32_to_bf16_bits(float x) {          // round to nearest even, finite x
+  const uint32_t u = __float_as_uint(x);
+  return (uint16_t)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
+}
+
+// scale bits of a group from the bits of its largest magnitude (ordered as integers: finite < inf < NaN); rs = 1 / s or 0
+template <int TOP> __device__ __forceinline__ uint16_t group_scale(uint32_t amax_bits, float& s, float& rs) {
+  if (amax_bits > 0x7F000000u) { s = 0.f; rs = 0.f; return 0x7FC0; }
+  uint16_t b = f32_to_bf16_bits(__uint_as_float(amax_bits) / (float)TOP);
+  if (b < 0x0080) b = 0;
+  s = bf16_bits_to_f32(b);
+  rs = b ? 1.0f / s : 0.f;
+  return b;
+}
+
+template <typename T, int TOP> __device__ __forceinline__ int code_of(float x, float s, float rs) {
+  const float q0 = x * rs;
+  const float e0 = __builtin_fmaf(-q0, s, x);
+  const float q = __builtin_fmaf(e0, rs, q0);
+  float c = __builtin_rintf(q);
+  if constexpr (sizeof(T) == 4) {
+    const float h = q - c;
+    if (__builtin_fabsf(h) == 0.5f) {
+      const float e = __builtin_fmaf(-q, s, x);
+      if (e != 0.f) c = e > 0.f ? q + 0.5f : q - 0.5f;
+    }
+  }
+  c = __builtin_fminf(__builtin_fmaxf(c, (float)-TOP), (float)TOP);        // s = 0 (zeros, NaN groups): rs = 0 and c = 0 or NaN -> below
+  return rs == 0.f ? 0 : (int)c;
+}
+
+// One token per sequence: a thread per (K or V, batch, head, channel).  The 32 lanes of a group share its scale through shuffles;
+// K words are put together by 8 lanes, a V code is one nibble of its channel's byte (read, changed, written by its one owner).
+template <typename T, int BITS, int DH>
+__global__ __launch_bounds__(256) void kv_append_token_kernel(KvArgs a, const T* k, const T* v, int64_t k_sb, int64_t k_sh, int64_t v_sb,
+                                                              int64_t v_sh) {
+  using L = KvTile<BITS, DH>;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t per = (int64_t)a.B * a.H * DH;
+  if (id >= 2 * per) return;                                   // whole groups of 32 lanes (DH is a multiple of 32)
+  const bool is_v = id >= per;
+  const int64_t j = is_v ? id - per : id;
+  const int c = (int)(j % DH), h = (int)((j / DH) % a.H), b = (int)(j / DH / a.H);
+  const int pos = a.first(b);
+  if (a.count(b) < 1 || pos < 0 || pos >= a.capacity) return;
+  const float x = to_f32(is_v ? v[b * v_sb + h * v_sh + c] : k[b * k_sb + h * k_sh + c]);
+  uint32_t m = __float_as_uint(x) & 0x7FFFFFFFu;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
+  float s, rs;
+  const uint16_t sb = group_scale<L::TOP>(m, s, rs);
+  const uint32_t code = (uint32_t)(code_of<T, L::TOP>(x, s, rs) + L::OFF);
+  uint8_t* tile = a.data + b * a.c_sb + h * a.c_sh + (int64_t)(pos / KV_TILE) * L::BYTES;
+  const int key = pos % KV_TILE, g = c / KV_GROUP, kg = (c / 8) % 4;
+  if ((c & 31) == 0) *(uint16_t*)(tile + (is_v ? L::VS : L::KS) + L::scale_at(key, g)) = sb;
+  if (!is_v) {
+    if constexpr (BITS == 4) {
+      uint32_t w = code << (4 * kv_nibble(c & 7));
+      w |= __shfl_xor(w, 1);
+      w |= __shfl_xor(w, 2);
+      w |= __shfl_xor(w, 4);
+      if ((c & 7) == 0) *(uint32_t*)(tile + key * L::KROW + (kg * L::NG + g) * 4) = w;
+    } else {
+      tile[key * L::KROW + (kg * L::NG + g) * 8 + (c & 7)] = (uint8_t)code;
+    }
+  } else {
+    uint8_t* row = tile + L::V + c * L::VROW;
+    if constexpr (BITS == 4) {
+      const int nib = kv_nibble(key & 7);
+      uint8_t* p = row + (key >> 3) * 4 + (nib >> 1);
+      const int sh = 4 * (nib & 1);
+      *p = (uint8_t)((*p & ~(15u << sh)) | (code << sh));
+    } else {
+      row[key] = (uint8_t)code;
+    }
+  }
+}
+
+template <typename T, bool VEC> __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+  if constexpr (!VEC) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = to_f32(p[j]);
+  } else if constexpr (sizeof(T) == 2) {
+    const bf16x8 r = *(const bf16x8*)p;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = (float)r[j];
+  } else {
+    const f32x4 r0 = *(const f32x4*)p, r1 = *(const f32x4*)(p + 4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { x[j] = r0[j]; x[4 + j] = r1[j]; }
+  }
+}
+
+template <typename T, bool VEC> __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+  if constexpr (!VEC) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) p[j] = from_f32<T>(x[j]);
+  } else if constexpr (sizeof(T) == 2) {
+    bf16x8 r;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = (bf16_t)x[j];
+    *(bf16x8*)p = r;
+  } else {
+    f32x4 r0, r1;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { r0[j] = x[j]; r1[j] = x[4 + j]; }
+    *(f32x4*)p = r0;
+    *(f32x4*)(p + 4) = r1;
+  }
+}
+
+// Several tokens: 128 threads take 256 / DH tiles, a thread the 8 keys x 8 channels of one word column of K and of V (so that the
+// transposition of V stays in its registers).  The tile is put together in LDS and leaves as whole 16-byte rows; a tile that the
+// new tokens cover only in part is read first, and the codes and scales of its other keys go back as they were.
+template <typename T, int BITS, int DH, bool VEC>
+__global__ __launch_bounds__(128) void kv_append_tiles_kernel(KvArgs a, const T* k, const T* v, int64_t k_sb, int64_t k_sh, int64_t k_st,
+                                                              int64_t v_sb, int64_t v_sh, int64_t v_st, int blocks_per_head) {
+  using L = KvTile<BITS, DH>;
+  constexpr int TPW = 256 / DH, NTH = DH / 2, U = DH / 8;
+  __shared__ __attribute__((aligned(16))) uint8_t image[TPW * L::BYTES];
+  const int tid = threadIdx.x, lt = tid / NTH, ti = tid % NTH, u = ti % U, oct = ti / U;
+  const int64_t bh = blockIdx.x / blocks_per_head;
+  const int b = (int)(bh / a.H), h = (int)(bh % a.H);
+  const int start = a.first(b), count = a.count(b);
+  // new tokens that fit: positions lo .. hi - 1
+  const int64_t hi64 = (int64_t)start + count;
+  const int lo = start < 0 ? 0 : min(start, a.capacity), hi = (int)(hi64 < 0 ? 0 : (hi64 > a.capacity ? a.capacity : hi64));
+  const int tile = lo / KV_TILE + (int)(blockIdx.x % blocks_per_head) * TPW + lt;
+  const int k0 = tile * KV_TILE;                               // (a capacity below 2^31 - 4096 is required)
+  const bool any = k0 < hi && lo < hi;                         // tiles past the last token: nothing to do
+  const bool whole = k0 >= lo && k0 + KV_TILE <= hi;
+  uint8_t* out = a.data + b * a.c_sb + h * a.c_sh + (int64_t)tile * L::BYTES;
+  uint8_t* img = image + lt * L::BYTES;
+  if (any && !whole)
+    for (int i = ti; i < L::BYTES / 16; i += NTH) *(uint4*)(img + 16 * i) = *(const uint4*)(out + 16 * i);
+  __syncthreads();
+  if (any) {
+    const int g = u / 4, kg = u % 4;
+    const int key0 = k0 + 8 * oct;
+    const T* src[2] = {k + b * k_sb + h * k_sh + 8 * u, v + b * v_sb + h * v_sh + 8 * u};
+    const int64_t st[2] = {k_st, v_st};
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      float x[8][8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int pos = key0 + e;
+        if (pos >= lo && pos < hi) {
+          load8<T, VEC>(src[kv] + (int64_t)(pos - start) * st[kv], x[e]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[e][j] = 0.f;
+        }
+      }
+      uint32_t vw[8][BITS == 4 ? 1 : 2] = {};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool in = key0 + e >= lo && key0 + e < hi;
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[e][j]) & 0x7FFFFFFFu);
+        m = max(m, (uint32_t)__shfl_xor((int)m, 1));
+        m = max(m, (uint32_t)__shfl_xor((int)m, 2));
+        float s, rs;
+        const uint16_t sb = group_scale<L::TOP>(m, s, rs);
+        const int key = 8 * oct + e;
+        if (in && kg == 0) *(uint16_t*)(img + (kv ? L::VS : L::KS) + L::scale_at(key, g)) = sb;
+        uint32_t kw[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t code = (uint32_t)(code_of<T, L::TOP>(x[e][j], s, rs) + L::OFF);
+          if constexpr (BITS == 4) {
+            if (kv == 0) kw[0] |= code << (4 * kv_nibble(j));
+            else vw[j][0] |= code << (4 * kv_nibble(e));
+          } else {
+            if (kv == 0) kw[j / 4] |= code << (8 * (j % 4));
+            else vw[j][e / 4] |= code << (8 * (e % 4));
+          }
+        }
+        if (kv == 0 && in) {
+          uint32_t* p = (uint32_t*)(img + key * L::KROW + (kg * L::NG + g) * L::WORD);
+          p[0] = kw[0];
+          if constexpr (BITS == 8) p[1] = kw[1];
+        }
+      }
+      if (kv == 1) {
+        uint32_t mask[2] = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const bool in = key0 + e >= lo && key0 + e < hi;
+          if constexpr (BITS == 4) mask[0] |= in ? 15u << (4 * kv_nibble(e)) : 0u;
+          else mask[e / 4] |= in ? 255u << (8 * (e % 4)) : 0u;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          uint32_t* p = (uint32_t*)(img + L::V + (8 * u + j) * L::VROW + oct * L::WORD);
+#pragma unroll
+          for (int w = 0; w < BITS / 4; ++w) p[w] = whole ? vw[j][w] : ((p[w] & ~mask[w]) | (vw[j][w] & mask[w]));
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (any)
+    for (int i = ti; i < L::BYTES / 16; i += NTH) *(uint4*)(out + 16 * i) = *(const uint4*)(img + 16 * i);
+}
+
+// Values back: the same 8 x 8 blocks, codes straight from memory.  Row t of the output is position start + t; rows at or past the
+// sequence's count, and positions outside the cache, are zeros.
+template <typename T, int BITS, int DH, bool VEC>
+__global__ __launch_bounds__(128) void kv_read_kernel(KvArgs a, T* k, T* v, int64_t o_sb, int64_t o_sh, int64_t o_st, int blocks_per_head) {
+  using L = KvTile<BITS, DH>;
+  constexpr int TPW = 256 / DH, NTH = DH / 2, U = DH / 8;
+  const int tid = threadIdx.x, lt = tid / NTH, ti = tid % NTH, u = ti % U, oct = ti / U;
+  const int64_t bh = blockIdx.x / blocks_per_head;
+  const int b = (int)(bh / a.H), h = (int)(bh % a.H);
+  const int64_t start = a.first(b);
+  const int count = a.count(b);
+  const int64_t floor_tile = start >= 0 ? start / KV_TILE : -((KV_TILE - 1 - start) / KV_TILE);
+  const int64_t tile = floor_tile + (int64_t)(blockIdx.x % blocks_per_head) * TPW + lt;
+  const int64_t pos0 = tile * KV_TILE + 8 * oct;               // this thread's 8 positions
+  if (pos0 + 8 <= start || pos0 >= start + a.T) return;
+  const int g = u / 4, kg = u % 4;
+  const uint8_t* t = a.data + b * a.c_sb + h * a.c_sh + tile * L::BYTES;
+  bool held[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int64_t pos = pos0 + e;
+    held[e] = pos >= start && pos < start + count && pos >= 0 && pos < a.capacity;
+  }
+  const bool inside = tile >= 0 && tile * KV_TILE < a.capacity;      // the tile exists
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    float x[8][8];
+    uint32_t w[8][BITS / 4] = {};
+    uint16_t sc[8] = {};
+    if (inside) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t* p = kv == 0 ? (const uint32_t*)(t + (8 * oct + i) * L::KROW + (kg * L::NG + g) * L::WORD)
+                                    : (const uint32_t*)(t + L::V + (8 * u + i) * L::VROW + oct * L::WORD);
+#pragma unroll
+        for (int q = 0; q < BITS / 4; ++q) w[i][q] = p[q];
+        sc[i] = *(const uint16_t*)(t + (kv ? L::VS : L::KS) + L::scale_at(8 * oct + i, g));
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float s = bf16_bits_to_f32(sc[e]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int row = kv == 0 ? e : j, el = kv == 0 ? j : e;      // K words run along the channels, V words along the keys
+        int code;
+        if constexpr (BITS == 4) code = (int)((w[row][0] >> (4 * kv_nibble(el))) & 15u) - L::OFF;
+        else code = (int)((w[row][el / 4] >> (8 * (el % 4))) & 255u) - L::OFF;
+        x[e][j] = held[e] ? s * (float)code : 0.f;
+      }
+    }
+    T* out = (kv ? v : k) + b * o_sb + h * o_sh + 8 * u;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int64_t row = pos0 + e - start;
+      if (row >= 0 && row < a.T) store8<T, VEC>(out + row * o_st, x[e]);
+    }
+  }
+}
+
+int kv_check(const char* who, const bg_kv_cache* c, const void* data, int dtype, int64_t T) {
+  BG_REQUIRE(c && data, "%s: null cache", who);
+  BG_REQUIRE(c->bits == 4 || c->bits == 8, "%s: bits=%d (4 or 8)", who, c->bits);
+  BG_REQUIRE(c->Dh == 32 || c->Dh == 64 || c->Dh == 128 || c->Dh == 256, "%s: Dh=%d (32, 64, 128 or 256)", who, c->Dh);
+  BG_REQUIRE(dtype == BG_F32 || dtype == BG_BF16, "%s: dtype %d", who, dtype);
+  BG_REQUIRE(c->B > 0 && c->H > 0 && c->capacity > 0 && c->capacity < (1 << 30) && T > 0 && T < (1 << 30),
+             "%s: B=%d H=%d capacity=%d T=%lld", who, c->B, c->H, c->capacity, (long long)T);
+  const int64_t tiles = cdiv(c->capacity, KV_TILE), bytes = tiles * (int64_t)bg_kv_cache_tile_bytes(c->bits, c->Dh);
+  BG_REQUIRE(((uintptr_t)data & 15) == 0 && c->c_sb % 16 == 0 && c->c_sh % 16 == 0, "%s: the cache must lie on 16-byte boundaries", who);
+  BG_REQUIRE((c->H == 1 || c->c_sh >= bytes) && (c->B == 1 || c->c_sb >= bytes), "%s: cache strides %lld, %lld overlap (%lld bytes per head)", who,
+             (long long)c->c_sb, (long long)c->c_sh, (long long)bytes);
+  return BG_OK;
+}
+
+}  // namespace bg
+
+using namespace bg;
+
+extern "C" size_t bg_kv_cache_tile_bytes(int bits, int Dh) {
+  if ((bits != 4 && bits != 8) || (Dh != 32 && Dh != 64 && Dh != 128 && Dh != 256)) return 0;
+  return (size_t)(2 * KV_TILE * Dh * bits / 8 + 2 * KV_TILE * (Dh / KV_GROUP) * 2);
+}
+
+static KvArgs kv_args(const bg_kv_cache* c, void* data, const int32_t* start, const int32_t* counts, int T) {
+  KvArgs a;
+  a.data = (uint8_t*)data;
+  a.B = c->B; a.H = c->H; a.capacity = c->capacity;
+  a.c_sb = c->c_sb; a.c_sh = c->c_sh;
+  a.start = start; a.counts = counts; a.T = T;
+  return a;
+}
+
+static bool aligned16(const void* p, int64_t s0, int64_t s1, int64_t s2, int e) {
+  return (((uintptr_t)p | (uintptr_t)(s0 * e) | (uintptr_t)(s1 * e) | (uintptr_t)(s2 * e)) & 15) == 0;
+}
+
+extern "C" int bg_kv_cache_append(const bg_kv_cache* cache, void* data, const void* k, const void* v, int dtype, int T,
+                                  int64_t k_sb, int64_t k_sh, int64_t k_st, int64_t v_sb, int64_t v_sh, int64_t v_st,
+                                  const int32_t* start, const int32_t* counts, void* stream) {
+  if (int rc = kv_check("bg_kv_cache_append", cache, data, dtype, T)) return rc;
+  BG_REQUIRE(k && v, "bg_kv_cache_append: null k / v");
+  const KvArgs a = kv_args(cache, data, start, counts, T);
+  hipStream_t st = (hipStream_t)stream;
+  const int e = dtype == BG_F32 ? 4 : 2;
+  const bool vec = aligned16(k, k_sb, k_sh, k_st, e) && aligned16(v, v_sb, v_sh, v_st, e);
+  const int64_t heads = (int64_t)cache->B * cache->H;
+  if (T == 1) {
+    const int64_t blocks = cdiv(2 * heads * cache->Dh, 256);
+    BG_REQUIRE(blocks < (1ll << 31), "bg_kv_cache_append: %lld blocks", (long long)blocks);
+#define BG_GO(BITS, DH)                                                                                                              \
+  if (dtype == BG_F32)                                                                                                               \
+    hipLaunchKernelGGL((kv_append_token_kernel<float, BITS, DH>), dim3((unsigned)blocks), dim3(256), 0, st, a, (const float*)k,      \
+                       (const float*)v, k_sb, k_sh, v_sb, v_sh);                                                                     \
+  else                                                                                                                               \
+    hipLaunchKernelGGL((kv_append_token_kernel<bf16_t, BITS, DH>), dim3((unsigned)blocks), dim3(256), 0, st, a, (const bf16_t*)k,    \
+                       (const bf16_t*)v, k_sb, k_sh, v_sb, v_sh)
+    BG_KV_DISPATCH(cache->bits, cache->Dh, BG_GO)
+#undef BG_GO
+    BG_CHECK_LAUNCH("bg_kv_cache_append");
+    return BG_OK;
+  }
+  const int64_t tiles = cdiv((int64_t)T + KV_TILE - 1, KV_TILE);            // T tokens at any offset touch at most this many
+  const int64_t per_head = cdiv(tiles, 256 / cache->Dh), blocks = per_head * heads;
+  BG_REQUIRE(blocks < (1ll << 31), "bg_kv_cache_append: %lld blocks", (long long)blocks);
+#define BG_GO2(TT, BITS, DH, VEC)                                                                                                   \
+  hipLaunchKernelGGL((kv_append_tiles_kernel<TT, BITS, DH, VEC>), dim3((unsigned)blocks), dim3(128), 0, st, a, (const TT*)k,        \
+                     (const TT*)v, k_sb, k_sh, k_st, v_sb, v_sh, v_st, (int)per_head)
+#define BG_GO(BITS, DH)                                                                                    \
+  if (dtype == BG_F32) { if (vec) BG_GO2(float, BITS, DH, true); else BG_GO2(float, BITS, DH, false); }    \
+  else { if (vec) BG_GO2(bf16_t, BITS, DH, true); else BG_GO2(bf16_t, BITS, DH, false); }
+  BG_KV_DISPATCH(cache->bits, cache->Dh, BG_GO)
+#undef BG_GO
+#undef BG_GO2
+  BG_CHECK_LAUNCH("bg_kv_cache_append");
+  return BG_OK;
+}
+
+extern "C" int bg_kv_cache_read(const bg_kv_cache* cache, const void* data, void* k, void* v, int dtype, int T, int64_t o_sb, int64_t o_sh,
+                                int64_t o_st, const int32_t* start, const int32_t* counts, void* stream) {
+  if (int rc = kv_check("bg_kv_cache_read", cache, data, dtype, T)) return rc;
+  BG_REQUIRE(k && v, "bg_kv_cache_read: null k / v");
+  const KvArgs a = kv_args(cache, (void*)data, start, counts, T);
+  hipStream_t st = (hipStream_t)stream;
+  const int e = dtype == BG_F32 ? 4 : 2;
+  const bool vec = aligned16(k, o_sb, o_sh, o_st, e) && aligned16(v, 0, 0, 0, e);
+  const int64_t tiles = cdiv((int64_t)T + KV_TILE - 1, KV_TILE);
+  const int64_t per_head = cdiv(tiles, 256 / cache->Dh), blocks = per_head * cache->B * cache->H;
+  BG_REQUIRE(blocks < (1ll << 31), "bg_kv_cache_read: %lld blocks", (long long)blocks);
+#define BG_GO2(TT, BITS, DH, VEC)                                                                                                 \
+  hipLaunchKernelGGL((kv_read_kernel<TT, BITS, DH, VEC>), dim3((unsigned)blocks), dim3(128), 0, st, a, (TT*)k, (TT*)v, o_sb,      \
+                     o_sh, o_st, (int)per_head)
+#define BG_GO(BITS, DH)                                                                                    \
+  if (dtype == BG_F32) { if (vec) BG_GO2(float, BITS, DH, true); else BG_GO2(float, BITS, DH, false); }    \
+  else { if (vec) BG_GO2(bf16_t, BITS, DH, true); else BG_GO2(bf16_t, BITS, DH, false); }
+  BG_KV_DISPATCH(cache->bits, cache->Dh, BG_GO)
+#undef BG_GO
+#undef BG_GO2
+  BG_CHECK_LAUNCH("bg_kv_cache_read");
+  return BG_OK;
+}

@@ -481,6 +481,76 @@ int bg_reinforce_terms_bwd(const float* probs, const float* advantages, const fl
 int bg_graph_node_census(void* graph, int* n_nodes, int* n_kernel, int* n_memset, int* n_memcpy);
 int bg_graph_replace_memset_nodes(void* graph, int* n_replaced);
 
+/* ------------------------------------------------------------------------------------------------
+ * Key / value cache held in 4 or 8 bits, for decoding (the reference decodes through HuggingFace's `generate`,
+ * Inference/GenerateTexts.py:19, whose cache holds the model's own dtype: none of this has a counterpart there).
+ *
+ * Every 32 channels of a token's key (value) of one head share a scale.  With a = the largest magnitude among them and L = 7
+ * (4 bits) or 127 (8 bits):  s = bf16(fp32(a / L)),  c = clamp(round-half-even(x / s), -L, L),  held value = s * c.
+ * s is 0 - the group reads as zeros - when it would be below 2^-126; a group holding a NaN, an infinity or a magnitude above
+ * 2^127 reads as NaN.  A value takes 0.5625 (1.0625) bytes.
+ *
+ * The cache is one byte buffer: per (batch, head) ceil(capacity / 32) tiles of bg_kv_cache_tile_bytes(bits, Dh) bytes, c_sb /
+ * c_sh BYTES apart (multiples of 16; the buffer itself on a 16-byte boundary).  The order of codes and scales inside a tile is
+ * the library's own: use bg_kv_cache_read to see values.  Dh: 32, 64, 128 or 256.
+ *
+ * start (int32 (B), NULL = 0 everywhere): tokens each sequence held before the call.  counts (int32 (B), NULL = T everywhere): how
+ * many of the T new tokens belong to sequence b; the rest is padding.  New token t of sequence b is position start[b] + t.
+ */
+typedef struct {
+  int bits, B, H, Dh, capacity, reserved;
+  int64_t c_sb, c_sh;
+} bg_kv_cache;
+
+size_t bg_kv_cache_tile_bytes(int bits, int Dh);     /* 0 for sizes there is no kernel for */
+/* k, v [B][H][T][Dh] with element strides (sb, sh, st).  Positions outside [0, capacity) and padding rows are not written; every
+ * other key of the cache stays as it was.  Calls on one cache must be ordered (one stream, or events). */
+int bg_kv_cache_append(const bg_kv_cache* cache, void* data, const void* k, const void* v, int dtype, int T,
+                       int64_t k_sb, int64_t k_sh, int64_t k_st, int64_t v_sb, int64_t v_sh, int64_t v_st,
+                       const int32_t* start, const int32_t* counts, void* stream);
+/* k, v [B][H][T][Dh] (one set of element strides): the values held at positions start[b] .. start[b] + T - 1, rounded once to
+ * dtype; zeros for rows t >= counts[b] and positions outside the cache. */
+int bg_kv_cache_read(const bg_kv_cache* cache, const void* data, void* k, void* v, int dtype, int T,
+                     int64_t o_sb, int64_t o_sh, int64_t o_st, const int32_t* start, const int32_t* counts, void* stream);
+/* Attention of T new tokens over the cache (their own keys / values are in it already): q [B][Hq][T][Dh], Hq a multiple of the
+ * cache's H (query head h reads cache head h / (Hq / H)); row (b, t) sees keys 0 .. start[b] + t.
+ *   out = softmax(scale * q k^T) v over the values the codes stand for, fp32 sums;  lse (optional, fp32 [B][Hq][T]) = log-sum-exp.
+ * A row that sees nothing (t >= counts[b], or start[b] + t < 0) is written as zeros, lse -inf.
+ * max_keys (host): no sequence holds more keys than this after the call, 1 .. capacity - it sizes the split of the key range over
+ * workgroups (keys past it are NOT read).  workspace: bg_kv_cache_attn_workspace_bytes bytes (0: may be NULL), contents irrelevant;
+ * calls that overlap in time need workspaces of their own. */
+size_t bg_kv_cache_attn_workspace_bytes(const bg_kv_cache* cache, int Hq, int T, int max_keys);
+int bg_kv_cache_attn_fwd(const bg_kv_cache* cache, const void* data, const void* q, int dtype, int Hq, int T,
+                         int64_t q_sb, int64_t q_sh, int64_t q_st, const int32_t* start, const int32_t* counts, int max_keys,
+                         float scale, void* out, int64_t o_sb, int64_t o_sh, int64_t o_st, float* lse,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Clipped policy loss with a KL term, straight from the logits of the policy being trained (beside bg_rl_loss_*, the reference's
+ * REINFORCE loss, Models/Losses/ReinforceLoss.py:21-52, which it does not replace).  Row r is one sampled token, x = logits / T:
+ *   logp = x[id] - lse(x),  ratio = exp(logp - old_logp[r]),
+ *   pg   = max(-A ratio, -A clamp(ratio, 1 - clip_low, 1 + clip_high)),
+ *   kl   = sum_j p_j (log p_j - log q_j), q = softmax(ref_logits / T)         when ref_logits is given,
+ *        = exp(d) - d - 1, d = ref_logp[r] - logp                             when ref_logp is given, 0 with neither,
+ *   loss = sum_r w_r (pg + kl_coef kl) / N,  N = *denominator, or sum_r w_r over the rows that count when it is NULL
+ *          (N = 0: loss and gradient are 0).
+ * weights (fp32, NULL = 1): a row with weight 0 or an id outside [0, V) does not count - its logits are not read, its logp and
+ * kl are 0, its gradient is 0.  A logit of -inf (or the type's lowest value) has probability 0 and adds nothing to the KL.
+ * _fwd writes out_loss (1 float), out_logp / out_kl (rows) and stats (rows x BG_POLICY_STATS + 1 floats on
+ * an 8-byte boundary: what _bwd needs);  _bwd writes dlogits ([rows][V], dtype of logits) = *g_loss * dloss / dlogits.
+ */
+#define BG_POLICY_STATS 8
+typedef struct {
+  int dtype, reserved;
+  int64_t rows, V, x_stride, ref_stride;
+  double temperature, clip_low, clip_high, kl_coef;
+} bg_policy_shape;
+int bg_policy_loss_fwd(const bg_policy_shape* sh, const void* logits, const void* ref_logits, const int64_t* ids, const float* old_logp,
+                       const float* ref_logp, const float* advantages, const float* weights, const float* denominator,
+                       float* out_loss, float* out_logp, float* out_kl, float* stats, void* stream);
+int bg_policy_loss_bwd(const bg_policy_shape* sh, const void* logits, const void* ref_logits, const int64_t* ids, const float* stats,
+                       const float* g_loss, void* dlogits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
