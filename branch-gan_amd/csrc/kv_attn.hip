@@ -1,91 +1,445 @@
 // Attention over the quantised key / value cache (bg_kv_cache_attn_fwd).
 //
-// One workgroup per (query row, batch): its four waves take every fourth tile of 32 keys.  A lane scores one key (half of its
-// channels), the tile's probabilities go through LDS, and a lane then owns output channels.  Running maximum and sum per wave, the
-// four states joined at the end.  All sums in fp32; the held values are exact in fp32.
+// Mathematics.  With codes c and scales s per 32 channels g,
+//   q . k = sum_g s_kg (q_g . c_kg)         o_ch = sum_k (p_k s_vg) c_v,ch
+// so the codes themselves are the matrix operands: as bf16 they are exact (4 bits: as c + 24, whose part is taken out of the sums; 8
+// bits: signed), the scales join in fp32 - on the scores after the product, on the probabilities before it.  Nothing held is rounded again.  bf16
+// queries are exact operands; fp32 queries go in as three bf16 pieces (24 bits), probabilities as two (16 bits, for bf16 outputs) or three.
+//
+// Layout.  One wave takes 4 tiles (128 keys) per turn with v_mfma_f32_16x16x32_bf16; lane = (n = lane % 16, j = lane / 16).
+//   scores   A = K codes: row rr of 16 is key 4 t + rr % 4 of tile rr / 4, B = queries: column n.  The result gives lane (n, j) the
+//            scores of column n against keys 4 t + r (r = 0..3) of tile j: over t, the 32 keys of ITS tile.
+//   output   A = probabilities: row n, lane group j holds 8 keys of tile j - what the lane already has -, B = V codes: lane (n, j) holds
+//            channel n's 8 keys of tile j.  Codes go from memory to operands with one shift and one mask-or per pair; P never
+//            leaves its lane; no LDS in the loop.
+// Columns.  PACKED (rows <= 16 / NG, decoding): column n = (row n / NG, channel group n % NG), its query zero outside its group: the
+//   NG partial scores of a row land in NG adjacent lanes, each with its own scale, and are summed by DPP; the output's A rows
+//   are (row, group) pairs, of which a column block uses the ones of its group.  One scale per key and lane instead of NG.
+//   Otherwise a column is a row and the groups are separate products.  (Which is faster depends on the rows only: a packed tile holds
+//   16 / NG of them at about half the vector work of a general one with 16.)
+// Softmax.  The running maximum of a row moves only when a score passes it by 2^8 (probabilities stay below 256), so that
+//   the usual turn needs no exchange between lanes.
+// Work.  Four waves per workgroup take turns round robin; the key range is split over workgroups when there are too few of
+//   them to fill 256 CUs (kv_attn_plan), the partial states joined by a second kernel.
+// Bound by HBM: 0.5625 or 1.0625 bytes per cached value.
 #include "kv_cache.h"
 
 namespace bg {
 
-template <typename T, int BITS, int DH>
-__global__ __launch_bounds__(256) void kv_attn_kernel(KvArgs a, const T* q, int G, int64_t q_sb, int64_t q_sh, int64_t q_st, int max_keys,
-                                                      float scale, T* out, int64_t o_sb, int64_t o_sh, int64_t o_st, float* lse) {
+constexpr int KW = 4;                       // waves per workgroup
+constexpr int KV_TURN = 4 * KV_TILE;        // keys a wave takes per turn
+
+// Turn of a wave in steps of TS rows of four keys per tile, so that the codes in flight fit the registers beside the accumulators
+template <int BITS, int DH, bool PACKED> constexpr int kv_steps() {
+  return PACKED ? (DH * BITS <= 512 ? 8 : DH * BITS <= 1024 ? 4 : 2) : (DH * BITS <= 512 ? 4 : 2);
+}
+
+struct KvAttnArgs {
+  KvArgs kv;
+  const void* q;
+  int64_t q_sb, q_sh, q_st;
+  void* out;
+  int64_t o_sb, o_sh, o_st;
+  float* lse;
+  float* part;                              // [row][split][Dh + 2]: unnormalised output, maximum (log2), sum
+  int G, max_keys, splits, row_tiles, negate;
+  float scale_log2;                         // |scale| log2(e)
+};
+
+template <int N> __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 v = ((const uint4*)p)[i];
+      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+    }
+  } else if constexpr (N == 2) {
+    const uint2 v = *(const uint2*)p;
+    w[0] = v.x; w[1] = v.y;
+  } else {
+    w[0] = *(const uint32_t*)p;
+  }
+}
+
+union Frag {
+  uint32_t u[4];
+  bf16x8 v;
+};
+
+// 8 codes -> 8 bf16 numbers code + OFFT.  4 bits: the nibble as bits 3..6 of a bf16 in [16, 32) is 16 + stored code; 8 bits: converted
+// (a conversion that takes its byte from the word, and half a pack).
+template <int BITS> constexpr float kv_offset() { return BITS == 4 ? 24.f : 0.f; }
+template <int BITS> __device__ __forceinline__ bf16x8 unpack_codes(const uint32_t* w) {
+  Frag f;
+  if constexpr (BITS == 4) {
+    f.u[0] = ((w[0] << 3) & 0x00780078u) | 0x41804180u;
+    f.u[1] = ((w[0] >> 1) & 0x00780078u) | 0x41804180u;
+    f.u[2] = ((w[0] >> 5) & 0x00780078u) | 0x41804180u;
+    f.u[3] = ((w[0] >> 9) & 0x00780078u) | 0x41804180u;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f.v[i] = (bf16_t)(float)(int8_t)(w[i / 4] >> (8 * (i % 4)));
+  }
+  return f.v;
+}
+
+// x -> N bf16 pieces that add up to it (8 bits each)
+template <int N> __device__ __forceinline__ void split_bf16(const float (&x)[8], bf16x8 (&piece)[N]) {
+  float rest[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) rest[e] = x[e];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      piece[i][e] = (bf16_t)rest[e];
+      if (i + 1 < N) rest[e] -= (float)piece[i][e];
+    }
+  }
+}
+
+template <int CTRL> __device__ __forceinline__ float dpp_add(float x) {
+  return x + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xF, 0xF, true));
+}
+template <int NG> __device__ __forceinline__ float group_sum(float x) {      // over NG adjacent lanes
+  if constexpr (NG >= 2) x = dpp_add<0xB1>(x);                              // quad_perm 1,0,3,2
+  if constexpr (NG >= 4) x = dpp_add<0x4E>(x);                              // quad_perm 2,3,0,1
+  if constexpr (NG >= 8) x = dpp_add<0x141>(x);                             // row_half_mirror
+  return x;
+}
+
+__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+
+// waves per SIMD the kernel is built for: two, but one (512 registers) where two would spill
+template <typename T, int BITS, int DH, bool PACKED> constexpr int kv_waves() {
+  return DH == 256 && (!PACKED || sizeof(T) == 4) ? 1 : DH == 128 && BITS == 4 && (!PACKED || sizeof(T) == 4) ? 1 : 2;
+}
+
+template <typename T, int BITS, int DH, bool PACKED>
+__global__ __launch_bounds__(64 * KW, (kv_waves<T, BITS, DH, PACKED>())) void kv_attn_kernel(KvAttnArgs a) {
   using L = KvTile<BITS, DH>;
-  constexpr int PER = DH > 64 ? DH / 64 : 1;
-  __shared__ float sh_q[DH], sh_p[4][KV_TILE], sh_m[4], sh_l[4], sh_o[4][DH];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int Hq = a.H * G;
-  const int t = blockIdx.x / Hq, hq = blockIdx.x % Hq, b = blockIdx.y, h = hq / G;
-  for (int i = tid; i < DH; i += 256) sh_q[i] = to_f32(q[b * q_sb + hq * q_sh + t * q_st + i]) * scale;
-  __syncthreads();
-  const int n = min(a.visible(b, t), max_keys);
-  const uint8_t* base = a.data + b * a.c_sb + h * a.c_sh;
-  float m = -INFINITY, l = 0.f, o[PER] = {};
-  const int key = lane & 31, half = lane >> 5;
-  for (int t0 = wave * KV_TILE; t0 < n; t0 += 4 * KV_TILE) {
-    const uint8_t* tile = base + (int64_t)(t0 / KV_TILE) * L::BYTES;
-    float s = 0.f;
-    for (int g = 0; g < L::NG; ++g) {
-      float d = 0.f;
-      for (int kk = 0; kk < 2; ++kk) {
-        const int kg = 2 * half + kk;
-        const uint32_t* w = (const uint32_t*)(tile + key * L::KROW + (kg * L::NG + g) * L::WORD);
+  constexpr int NG = L::NG, TS = kv_steps<BITS, DH, PACKED>(), NO = TS / 2, CB = DH / 16;
+  constexpr int ROWS = PACKED ? 16 / NG : 16, GL = PACKED ? 1 : NG;         // rows per tile; groups whose scales a lane needs
+  constexpr int NQ = sizeof(T) == 4 ? 3 : 1, NP = sizeof(T) == 4 ? 3 : 2;   // bf16 pieces of queries / probabilities
+  constexpr float OFFT = kv_offset<BITS>();
+  constexpr int KWORDS = NG * L::WORD / 4, VWORDS = NO * L::WORD / 4;
+  __shared__ float sh_o[KW][ROWS][DH];
+  __shared__ float sh_m[KW][16], sh_l[KW][16];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, j = lane >> 4;
+  const int64_t blk = blockIdx.x;
+  const int split = (int)(blk % a.splits), rt = (int)(blk / a.splits % a.row_tiles);
+  const int64_t bh = blk / a.splits / a.row_tiles;
+  const int b = (int)(bh / a.kv.H), h = (int)(bh % a.kv.H);
+  const int R = a.kv.T * a.G, row0 = rt * ROWS;                             // rows (t, g) of this cache head: rho = t G + g
+
+  // this lane's column: its row, and what that row sees
+  const int rho = row0 + (PACKED ? n / NG : n), my_g = PACKED ? n % NG : 0;
+  const bool real = rho < R;
+  const int vis = real ? min(a.kv.visible(b, rho / a.G), a.max_keys) : 0x7FFFFFFF;
+  int n_max = real ? vis : 0, n_min = vis;
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) {
+    n_max = max(n_max, __shfl_xor(n_max, o));
+    n_min = min(n_min, __shfl_xor(n_min, o));
+  }
+  n_max = __builtin_amdgcn_readfirstlane(n_max);
+  n_min = __builtin_amdgcn_readfirstlane(n_min);
+
+  // queries: B operand of step g = channels 32 g + 8 j + 0..7 of column n's row
+  bf16x8 qf[NG][NQ];
+  float q0[GL];                                                              // what the offset of the codes adds to a score
+  {
+    const T* q = (const T*)a.q + b * a.q_sb + (int64_t)(h * a.G + rho % a.G) * a.q_sh + (int64_t)(rho / a.G) * a.q_st;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      float x[8], sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float v = real && (!PACKED || g == my_g) ? to_f32(q[32 * g + 8 * j + e]) : 0.f;
+        x[e] = a.negate ? -v : v;
+        sum += x[e];
+      }
+      split_bf16<NQ>(x, qf[g]);
+      sum += __shfl_xor(sum, 16);
+      sum += __shfl_xor(sum, 32);
+      if constexpr (PACKED) q0[0] = g == 0 ? sum : q0[0] + sum;              // one group is not zero
+      else q0[g] = sum;
+    }
+#pragma unroll
+    for (int g = 0; g < GL; ++g) q0[g] *= -OFFT;
+  }
+
+  f32x4 acc[CB], off = {0.f, 0.f, 0.f, 0.f};                                 // PACKED: one offset sum; else one per group
+  f32x4 offg[PACKED ? 1 : NG];
+#pragma unroll
+  for (int c = 0; c < CB; ++c) acc[c] = off;
+#pragma unroll
+  for (int g = 0; g < (PACKED ? 1 : NG); ++g) offg[g] = off;
+  float mc = -INFINITY, l = 0.f;                                             // maximum in log2 units, this lane's share of the sum
+  Frag ones;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ones.v[i] = (bf16_t)OFFT;
+
+  const uint8_t* base = a.kv.data + b * a.kv.c_sb + h * a.kv.c_sh;
+  const int last_tile = (a.kv.capacity - 1) / KV_TILE;
+  const int turns = (n_max + KV_TURN - 1) / KV_TURN;
+  const int t_begin = (int)((int64_t)turns * split / a.splits), t_end = (int)((int64_t)turns * (split + 1) / a.splits);
+  constexpr int SUB = 8 / TS;                                                // steps of a turn
+  const int my_turns = t_end - t_begin > wave ? (t_end - t_begin - wave + KW - 1) / KW : 0;
+  const int steps = my_turns * SUB;
+
+  uint32_t kw[TS][KWORDS], ks[GL][TS * 2], vw[CB][VWORDS], vs[GL][TS * 2];
+  auto key_base = [&](int step, int tile_in_turn) __attribute__((always_inline)) -> const uint8_t* {
+    const int tile = (t_begin + wave + KW * (step / SUB)) * 4 + tile_in_turn;
+    return base + (int64_t)min(tile, last_tile) * L::BYTES;
+  };
+  auto load_k = [&](int step) __attribute__((always_inline)) {
+    const int s = step % SUB;
+    const uint8_t* kt = key_base(step, n >> 2);
+#pragma unroll
+    for (int t = 0; t < TS; ++t) load_words<KWORDS>(kt + (4 * (s * TS + t) + (n & 3)) * L::KROW + j * NG * L::WORD, kw[t]);
+    const uint8_t* st = key_base(step, j) + L::KS + s * TS * 8;
+#pragma unroll
+    for (int g = 0; g < GL; ++g) load_words<TS * 2>(st + (PACKED ? my_g : g) * KV_TILE * 2, ks[g]);
+  };
+  auto load_v = [&](int step) __attribute__((always_inline)) {
+    const int s = step % SUB;
+    const uint8_t* vt = key_base(step, j);
+#pragma unroll
+    for (int c = 0; c < CB; ++c) load_words<VWORDS>(vt + L::V + (16 * c + n) * L::VROW + s * NO * L::WORD, vw[c]);
+#pragma unroll
+    for (int g = 0; g < GL; ++g) load_words<TS * 2>(vt + L::VS + s * TS * 8 + (PACKED ? my_g : g) * KV_TILE * 2, vs[g]);
+  };
+
+  if (steps > 0) load_k(0);
+  for (int step = 0; step < steps; ++step) {
+    load_v(step);
+    // scores
+    float sc[TS][4];
+#pragma unroll
+    for (int t = 0; t < TS; ++t) {
+      if constexpr (PACKED) {
+        f32x4 d = {q0[0], q0[0], q0[0], q0[0]};
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const bf16x8 kf = unpack_codes<BITS>(&kw[t][g * L::WORD / 4]);
+#pragma unroll
+          for (int i = 0; i < NQ; ++i) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[g][i], d, 0, 0, 0);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float k_scale = r & 1 ? bf16_hi(ks[0][2 * t + r / 2]) : bf16_lo(ks[0][2 * t + r / 2]);
+          sc[t][r] = group_sum<NG>(d[r] * k_scale);
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sc[t][r] = 0.f;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const bf16x8 kf = unpack_codes<BITS>(&kw[t][g * L::WORD / 4]);
+          f32x4 d = {q0[g], q0[g], q0[g], q0[g]};
+#pragma unroll
+          for (int i = 0; i < NQ; ++i) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[g][i], d, 0, 0, 0);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float k_scale = r & 1 ? bf16_hi(ks[g][2 * t + r / 2]) : bf16_lo(ks[g][2 * t + r / 2]);
+            sc[t][r] = __builtin_fmaf(d[r], k_scale, sc[t][r]);
+          }
+        }
+      }
+    }
+    if (step + 1 < steps) load_k(step + 1);
+    // keys of this lane: key0 + 4 t + r
+    const int turn0 = (t_begin + wave + KW * (step / SUB)) * KV_TURN;
+    const bool partial = turn0 + KV_TURN > n_min;                            // some row does not see all of this turn
+    const int key0 = turn0 + j * KV_TILE + (step % SUB) * TS * 4;
+    if (partial) {
+#pragma unroll
+      for (int t = 0; t < TS; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sc[t][r] = key0 + 4 * t + r < vis ? sc[t][r] : -INFINITY;
+    }
+    float top = sc[0][0];
+#pragma unroll
+    for (int t = 0; t < TS; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) top = fmaxf(top, sc[t][r]);
+    top *= a.scale_log2;
+    if (step == 0 || __any(top > mc + 8.f)) {
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float m_new = fmaxf(mc, top);
+      const float keep = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mc - m_new);
+      mc = m_new;
+      l *= keep;
+      if (step != 0) {
+        float f[4];                                                          // of the accumulators' rows 4 j + r: lane 4 j + r has it
+#pragma unroll
+        for (int r = 0; r < 4; ++r) f[r] = __shfl(keep, 4 * j + r);
+#pragma unroll
+        for (int c = 0; c < CB; ++c)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[c][r] *= f[r];
+#pragma unroll
+        for (int g = 0; g < (PACKED ? 1 : NG); ++g)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) offg[g][r] *= f[r];
+      }
+    }
+    const float ms = mc == -INFINITY ? 0.f : mc;
+    float p[TS][4];
+#pragma unroll
+    for (int t = 0; t < TS; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) p[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][r], a.scale_log2, -ms));
+    if (partial) {                                                           // keys not seen: no weight, and no scale (it may be anything)
+#pragma unroll
+      for (int t = 0; t < TS; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const bool seen = key0 + 4 * t + r < vis;
+          p[t][r] = seen ? p[t][r] : 0.f;
+          if (!seen) {
+#pragma unroll
+            for (int g = 0; g < GL; ++g) vs[g][2 * t + r / 2] &= r & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+          }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < TS; ++t) l += (p[t][0] + p[t][1]) + (p[t][2] + p[t][3]);
+    // output
+#pragma unroll
+    for (int o = 0; o < NO; ++o) {
+      bf16x8 pf[GL][NP];
+#pragma unroll
+      for (int g = 0; g < GL; ++g) {
+        float x[8];
+#pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int code = BITS == 4 ? (int)((w[0] >> (4 * kv_nibble(e))) & 15u) : (int)((w[e / 4] >> (8 * (e % 4))) & 255u);
-          d += sh_q[32 * g + 8 * kg + e] * (float)(code - L::OFF);
+          const uint32_t w = vs[g][4 * o + e / 2];
+          x[e] = p[2 * o + e / 4][e % 4] * (e & 1 ? bf16_hi(w) : bf16_lo(w));
         }
-      }
-      s += d * bf16_bits_to_f32(*(const uint16_t*)(tile + L::KS + L::scale_at(key, g)));
-    }
-    s += __shfl_xor(s, 32);
-    const bool seen = t0 + key < n;
-    s = seen ? s : -INFINITY;
-    const float mn = fmaxf(m, wave_max(s)), ms = mn == -INFINITY ? 0.f : mn;
-    const float p = seen ? expf(s - ms) : 0.f, keep = expf(m - ms);
-    l = l * keep + 0.5f * wave_sum(p);                         // both halves of the wave hold the 32 keys
-    m = mn;
-    if (half == 0) sh_p[wave][key] = p;
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        split_bf16<NP>(x, pf[g]);
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int c = lane + 64 * j;
-      if (c < DH) {
-        float acc = 0.f;
-        const uint32_t* w = (const uint32_t*)(tile + L::V + c * L::VROW);
-        for (int k = 0; k < KV_TILE && t0 + k < n; ++k) {
-          const int code = BITS == 4 ? (int)((w[k / 8] >> (4 * kv_nibble(k % 8))) & 15u) : (int)((w[k / 4] >> (8 * (k % 4))) & 255u);
-          acc += sh_p[wave][k] * (bf16_bits_to_f32(*(const uint16_t*)(tile + L::VS + L::scale_at(k, c / KV_GROUP))) * (float)(code - L::OFF));
-        }
-        o[j] = o[j] * keep + acc;
+        for (int i = 0; i < NP && OFFT != 0.f; ++i) offg[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf[g][i], ones.v, offg[g], 0, 0, 0);
+      }
+#pragma unroll
+      for (int c = 0; c < CB; ++c) {
+        const bf16x8 vf = unpack_codes<BITS>(&vw[c][o * L::WORD / 4]);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf[PACKED ? 0 : c / 2][i], vf, acc[c], 0, 0, 0);
       }
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
   }
-  if (lane == 0) { sh_m[wave] = m; sh_l[wave] = l; }
+
+  // this wave's state -> LDS (accumulator row 4 j + r, channel 16 c + n)
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  if (j == 0 && my_g == 0) { sh_m[wave][rho - row0] = mc; sh_l[wave][rho - row0] = l; }
 #pragma unroll
-  for (int j = 0; j < PER; ++j)
-    if (lane + 64 * j < DH) sh_o[wave][lane + 64 * j] = o[j];
+  for (int c = 0; c < CB; ++c)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int ar = 4 * j + r;
+      if (PACKED && ar % NG != c / 2) continue;
+      sh_o[wave][PACKED ? ar / NG : ar][16 * c + n] = acc[c][r] - offg[PACKED ? 0 : c / 2][r];
+    }
   __syncthreads();
-  float M = -INFINITY, S = 0.f;
-  for (int w = 0; w < 4; ++w) M = fmaxf(M, sh_m[w]);
-  const float Ms = M == -INFINITY ? 0.f : M;
-  float f[4];
-  for (int w = 0; w < 4; ++w) { f[w] = expf(sh_m[w] - Ms); S += f[w] * sh_l[w]; }
-  for (int c = tid; c < DH; c += 256) {
-    float acc = 0.f;
-    for (int w = 0; w < 4; ++w) acc += f[w] * sh_o[w][c];
-    out[b * o_sb + hq * o_sh + t * o_st + c] = from_f32<T>(n > 0 ? acc / S : 0.f);
+  for (int i = tid; i < ROWS * DH; i += 64 * KW) {
+    const int row = i / DH, ch = i % DH, rr = row0 + row;
+    if (rr >= R) break;
+    float M = sh_m[0][row];
+#pragma unroll
+    for (int w = 1; w < KW; ++w) M = fmaxf(M, sh_m[w][row]);
+    const float Ms = M == -INFINITY ? 0.f : M;
+    float S = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < KW; ++w) {
+      const float f = __builtin_amdgcn_exp2f(sh_m[w][row] - Ms);
+      S += f * sh_l[w][row];
+      o += f * sh_o[w][row][ch];
+    }
+    const int t = rr / a.G, hq = h * a.G + rr % a.G;
+    if (a.splits == 1) {
+      const bool any = a.kv.visible(b, t) > 0;
+      ((T*)a.out)[b * a.o_sb + hq * a.o_sh + t * a.o_st + ch] = from_f32<T>(any ? o / S : 0.f);
+      if (a.lse && ch == 0) a.lse[((int64_t)b * a.kv.H * a.G + hq) * a.kv.T + t] = any ? (M + __log2f(S)) * 0.6931471805599453f : -INFINITY;
+    } else {
+      float* part = a.part + ((bh * R + rr) * a.splits + split) * (DH + 2);
+      part[ch] = o;
+      if (ch == 0) { part[DH] = M; part[DH + 1] = S; }
+    }
   }
-  if (lse && tid == 0) lse[((int64_t)b * Hq + hq) * a.T + t] = n > 0 ? M + logf(S) : -INFINITY;
+}
+
+// Joins the splits of a row: one wave per row.
+template <typename T, int DH>
+__global__ __launch_bounds__(256) void kv_attn_join_kernel(KvAttnArgs a, int64_t rows) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const int R = a.kv.T * a.G;
+  const int64_t bh = row / R;
+  const int rr = (int)(row % R), b = (int)(bh / a.kv.H), h = (int)(bh % a.kv.H), t = rr / a.G, hq = h * a.G + rr % a.G;
+  const float* part = a.part + row * a.splits * (DH + 2);
+  float M = -INFINITY;
+  for (int s = lane; s < a.splits; s += 64) M = fmaxf(M, part[(int64_t)s * (DH + 2) + DH]);
+  M = wave_max(M);
+  const float Ms = M == -INFINITY ? 0.f : M;
+  float S = 0.f, o[(DH + 63) / 64] = {};
+  for (int s = 0; s < a.splits; ++s) {
+    const float* ps = part + (int64_t)s * (DH + 2);
+    const float f = __builtin_amdgcn_exp2f(ps[DH] - Ms);
+    S += f * ps[DH + 1];
+#pragma unroll
+    for (int i = 0; i < (DH + 63) / 64; ++i)
+      if (lane + 64 * i < DH) o[i] += f * ps[lane + 64 * i];
+  }
+  const bool any = a.kv.visible(b, t) > 0;
+#pragma unroll
+  for (int i = 0; i < (DH + 63) / 64; ++i)
+    if (lane + 64 * i < DH) ((T*)a.out)[b * a.o_sb + hq * a.o_sh + t * a.o_st + lane + 64 * i] = from_f32<T>(any ? o[i] / S : 0.f);
+  if (a.lse && lane == 0) a.lse[((int64_t)b * a.kv.H * a.G + hq) * a.kv.T + t] = any ? (M + __log2f(S)) * 0.6931471805599453f : -INFINITY;
+}
+
+// How many workgroups share a row tile's key range: enough to give every CU two (512), none with less than one turn for each wave.
+struct KvPlan {
+  bool packed;
+  int row_tiles, splits;
+};
+static KvPlan kv_attn_plan(const bg_kv_cache* c, int Hq, int T, int max_keys) {
+  KvPlan p;
+  const int64_t R = (int64_t)T * (Hq / c->H);
+  const int ng = c->Dh / KV_GROUP;
+  p.packed = R <= 16 / ng;
+  p.row_tiles = (int)cdiv(R, p.packed ? 16 / ng : 16);
+  const int64_t base = (int64_t)c->B * c->H * p.row_tiles;
+  const int64_t most = cdiv(max_keys, KV_TURN * KW), want = cdiv(512, base);
+  p.splits = (int)(want < most ? want : most);
+  return p;
 }
 
 }  // namespace bg
 
 using namespace bg;
 
-extern "C" size_t bg_kv_cache_attn_workspace_bytes(const bg_kv_cache*, int, int, int) { return 0; }
+extern "C" size_t bg_kv_cache_attn_workspace_bytes(const bg_kv_cache* cache, int Hq, int T, int max_keys) {
+  if (!cache || cache->H <= 0 || cache->B <= 0 || cache->Dh < 32 || Hq <= 0 || Hq % cache->H || T <= 0 || max_keys <= 0) return 0;
+  const KvPlan p = kv_attn_plan(cache, Hq, T, max_keys);
+  return p.splits == 1 ? 0 : (size_t)cache->B * Hq * T * p.splits * (cache->Dh + 2) * sizeof(float);
+}
+
+template <typename T, int BITS, int DH>
+static void kv_attn_launch(const KvAttnArgs& a, const KvPlan& p, int64_t blocks, hipStream_t st) {
+  if (p.packed) hipLaunchKernelGGL((kv_attn_kernel<T, BITS, DH, true>), dim3((unsigned)blocks), dim3(64 * KW), 0, st, a);
+  else hipLaunchKernelGGL((kv_attn_kernel<T, BITS, DH, false>), dim3((unsigned)blocks), dim3(64 * KW), 0, st, a);
+  if (p.splits > 1) {
+    const int64_t rows = (int64_t)a.kv.B * a.kv.H * a.kv.T * a.G;
+    hipLaunchKernelGGL((kv_attn_join_kernel<T, DH>), dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, st, a, rows);
+  }
+}
 
 extern "C" int bg_kv_cache_attn_fwd(const bg_kv_cache* cache, const void* data, const void* q, int dtype, int Hq, int T, int64_t q_sb,
                                     int64_t q_sh, int64_t q_st, const int32_t* start, const int32_t* counts, int max_keys, float scale,
@@ -95,23 +449,30 @@ extern "C" int bg_kv_cache_attn_fwd(const bg_kv_cache* cache, const void* data, 
   BG_REQUIRE(q && out, "bg_kv_cache_attn_fwd: null q / out");
   BG_REQUIRE(Hq > 0 && Hq % cache->H == 0, "bg_kv_cache_attn_fwd: Hq=%d query heads over %d cache heads", Hq, cache->H);
   BG_REQUIRE(max_keys > 0 && max_keys <= cache->capacity, "bg_kv_cache_attn_fwd: max_keys=%d of capacity %d", max_keys, cache->capacity);
-  BG_REQUIRE((int64_t)T * Hq < (1ll << 31) && cache->B <= 65535, "bg_kv_cache_attn_fwd: T=%d Hq=%d B=%d", T, Hq, cache->B);
-  (void)workspace; (void)workspace_bytes;
-  KvArgs a;
-  a.data = (uint8_t*)data;
-  a.B = cache->B; a.H = cache->H; a.capacity = cache->capacity;
-  a.c_sb = cache->c_sb; a.c_sh = cache->c_sh;
-  a.start = start; a.counts = counts; a.T = T;
-  const int G = Hq / cache->H;
+  BG_REQUIRE((int64_t)T * Hq < (1ll << 30), "bg_kv_cache_attn_fwd: T=%d Hq=%d", T, Hq);
+  const KvPlan p = kv_attn_plan(cache, Hq, T, max_keys);
+  const int64_t blocks = (int64_t)cache->B * cache->H * p.row_tiles * p.splits, rows = (int64_t)cache->B * Hq * T;
+  BG_REQUIRE(blocks < (1ll << 31) && rows < (1ll << 31), "bg_kv_cache_attn_fwd: %lld blocks, %lld rows", (long long)blocks, (long long)rows);
+  const size_t need = bg_kv_cache_attn_workspace_bytes(cache, Hq, T, max_keys);
+  if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 3))) {
+    set_error("bg_kv_cache_attn_fwd: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, need);
+    return BG_ERR_WORKSPACE;
+  }
+  KvAttnArgs a;
+  a.kv.data = (uint8_t*)data;
+  a.kv.B = cache->B; a.kv.H = cache->H; a.kv.capacity = cache->capacity;
+  a.kv.c_sb = cache->c_sb; a.kv.c_sh = cache->c_sh;
+  a.kv.start = start; a.kv.counts = counts; a.kv.T = T;
+  a.q = q; a.q_sb = q_sb; a.q_sh = q_sh; a.q_st = q_st;
+  a.out = out; a.o_sb = o_sb; a.o_sh = o_sh; a.o_st = o_st;
+  a.lse = lse; a.part = (float*)workspace;
+  a.G = Hq / cache->H; a.max_keys = max_keys; a.splits = p.splits; a.row_tiles = p.row_tiles;
+  a.negate = scale < 0.f;
+  a.scale_log2 = (float)((scale < 0.f ? -(double)scale : (double)scale) * 1.4426950408889634);
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)(T * Hq), (unsigned)cache->B);
-#define BG_GO(BITS, DH)                                                                                                              \
-  if (dtype == BG_F32)                                                                                                               \
-    hipLaunchKernelGGL((kv_attn_kernel<float, BITS, DH>), grid, dim3(256), 0, st, a, (const float*)q, G, q_sb, q_sh, q_st, max_keys, \
-                       scale, (float*)out, o_sb, o_sh, o_st, lse);                                                                   \
-  else                                                                                                                               \
-    hipLaunchKernelGGL((kv_attn_kernel<bf16_t, BITS, DH>), grid, dim3(256), 0, st, a, (const bf16_t*)q, G, q_sb, q_sh, q_st,         \
-                       max_keys, scale, (bf16_t*)out, o_sb, o_sh, o_st, lse)
+#define BG_GO(BITS, DH)                                                \
+  if (dtype == BG_F32) kv_attn_launch<float, BITS, DH>(a, p, blocks, st); \
+  else kv_attn_launch<bf16_t, BITS, DH>(a, p, blocks, st)
   BG_KV_DISPATCH(cache->bits, cache->Dh, BG_GO)
 #undef BG_GO
   BG_CHECK_LAUNCH("bg_kv_cache_attn_fwd");

@@ -3,11 +3,11 @@
 // A (batch, head) holds tiles of 32 consecutive keys.  One tile of head size DH, NG = DH / 32 groups of 32 channels:
 //   K codes    [32 keys][4 kg][NG g] words of the channels 32 g + 8 kg + 0..7 (8 codes: 4 bytes at 4 bits, 8 bytes at 8 bits)
 //   V codes    [DH channels][4 octets] words of the keys 8 octet + 0..7
-//   K scales   [8 t][NG g][4 r] bf16 of key 4 t + r
+//   K scales   [NG g][32 keys] bf16
 //   V scales   the same
 // A word is what one lane feeds to a 32-deep matrix instruction (8 consecutive elements of its row), for K along the channels and
 // for V along the keys: the codes go from memory to the matrix operand with no shuffle and no LDS.
-// Codes are stored offset by OFF (unsigned).  4-bit words keep element e in nibble (e >> 1) + 4 (e & 1), so that one mask over a
+// 8-bit codes are signed bytes; 4-bit ones are stored as code + 8, and their words keep element e in nibble (e >> 1) + 4 (e & 1), so that one mask over a
 // shifted word leaves elements 2i and 2i + 1 in the two halves of a register, the order of a bf16 pair.
 #pragma once
 #include "common.h"
@@ -20,7 +20,7 @@ constexpr int KV_GROUP = 32;       // channels per scale
 template <int BITS, int DH> struct KvTile {
   static constexpr int NG = DH / KV_GROUP;
   static constexpr int TOP = BITS == 4 ? 7 : 127;        // codes are -TOP .. TOP
-  static constexpr int OFF = BITS == 4 ? 8 : 128;
+  static constexpr int OFF = BITS == 4 ? 8 : 0;
   static constexpr int WORD = BITS;                      // bytes of 8 codes
   static constexpr int KROW = DH * BITS / 8;
   static constexpr int VROW = KV_TILE * BITS / 8;
@@ -28,7 +28,7 @@ template <int BITS, int DH> struct KvTile {
   static constexpr int KS = V + DH * VROW;
   static constexpr int VS = KS + KV_TILE * NG * 2;
   static constexpr int BYTES = VS + KV_TILE * NG * 2;
-  static constexpr int scale_at(int key, int g) { return (((key >> 2) * NG + g) * 4 + (key & 3)) * 2; }
+  static constexpr int scale_at(int key, int g) { return (g * KV_TILE + key) * 2; }
 };
 
 __device__ __forceinline__ constexpr int kv_nibble(int e) { return (e >> 1) + 4 * (e & 1); }

@@ -64,7 +64,7 @@ __global__ __launch_bounds__(256) void kv_append_token_kernel(KvArgs a, const T*
   for (int o = 1; o < 32; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
   float s, rs;
   const uint16_t sb = group_scale<L::TOP>(m, s, rs);
-  const uint32_t code = (uint32_t)(code_of<T, L::TOP>(x, s, rs) + L::OFF);
+  const uint32_t code = (uint32_t)(code_of<T, L::TOP>(x, s, rs) + L::OFF) & 255u;
   uint8_t* tile = a.data + b * a.c_sb + h * a.c_sh + (int64_t)(pos / KV_TILE) * L::BYTES;
   const int key = pos % KV_TILE, g = c / KV_GROUP, kg = (c / 8) % 4;
   if ((c & 31) == 0) *(uint16_t*)(tile + (is_v ? L::VS : L::KS) + L::scale_at(key, g)) = sb;
@@ -183,7 +183,7 @@ __global__ __launch_bounds__(128) void kv_append_tiles_kernel(KvArgs a, const T*
         uint32_t kw[2] = {0, 0};
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const uint32_t code = (uint32_t)(code_of<T, L::TOP>(x[e][j], s, rs) + L::OFF);
+          const uint32_t code = (uint32_t)(code_of<T, L::TOP>(x[e][j], s, rs) + L::OFF) & 255u;
           if constexpr (BITS == 4) {
             if (kv == 0) kw[0] |= code << (4 * kv_nibble(j));
             else vw[j][0] |= code << (4 * kv_nibble(e));
@@ -267,7 +267,7 @@ __global__ __launch_bounds__(128) void kv_read_kernel(KvArgs a, T* k, T* v, int6
         const int row = kv == 0 ? e : j, el = kv == 0 ? j : e;      // K words run along the channels, V words along the keys
         int code;
         if constexpr (BITS == 4) code = (int)((w[row][0] >> (4 * kv_nibble(el))) & 15u) - L::OFF;
-        else code = (int)((w[row][el / 4] >> (8 * (el % 4))) & 255u) - L::OFF;
+        else code = (int8_t)(w[row][el / 4] >> (8 * (el % 4)));
         x[e][j] = held[e] ? s * (float)code : 0.f;
       }
     }
