@@ -127,8 +127,8 @@ SIGNATURES = {
     "bg_kv_cache_attn_workspace_bytes": (c_sz, [ctypes.POINTER(KvCache), c_i32, c_i32, c_i32]),
     "bg_kv_cache_attn_fwd": (c_i32, [ctypes.POINTER(KvCache), c_vp, c_vp, c_i32, c_i32, c_i32, c_i64, c_i64, c_i64, c_vp, c_vp, c_i32, c_f32,
                                      c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_sz, c_vp]),
-    "bg_policy_loss_fwd": (c_i32, [ctypes.POINTER(PolicyShape)] + [c_vp] * 13),
-    "bg_policy_loss_bwd": (c_i32, [ctypes.POINTER(PolicyShape)] + [c_vp] * 7),
+    "bg_policy_loss_fwd": (c_i32, [ctypes.POINTER(PolicyShape)] + [c_vp] * 13 + [ctypes.POINTER(c_i32), c_vp]),
+    "bg_policy_loss_bwd": (c_i32, [ctypes.POINTER(PolicyShape)] + [c_vp] * 6 + [c_i32, c_vp]),
     "bg_graph_node_census": (c_i32, [c_vp] + [ctypes.POINTER(c_i32)] * 4),
     "bg_graph_replace_memset_nodes": (c_i32, [c_vp, ctypes.POINTER(c_i32)]),
     "bg_rl_loss_bwd": (c_i32, [ctypes.POINTER(RlLossShape)] + [c_vp] * 7 + [c_vp, c_vp, c_vp, c_vp]),

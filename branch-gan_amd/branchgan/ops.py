@@ -941,10 +941,14 @@ class _PolicyLoss(torch.autograd.Function):
         logp, kl = [torch.empty(rows, dtype=torch.float32, device=dev) for _ in range(2)]
         stats = torch.empty(rows * C.POLICY_STATS + 1, dtype=torch.float32, device=dev)
         args = [flat(t) for t in (old_logp, ref_logp, advantages, weights)] + [denominator]
+        # the gradient for an incoming gradient of 1 comes out of the same reading of the logits; backward hands this buffer out
+        dx = torch.empty((rows, V), dtype=x.dtype, device=dev) if ctx.needs_input_grad[0] else None
+        has = C.c_i32(0)
         with torch.cuda.device(dev), _timed(f"policy_loss_fwd[{rows}]"):
             C.check(C.lib().bg_policy_loss_fwd(ctypes.byref(sh), C.ptr(x), C.ptr(y), C.ptr(ids), *[C.ptr(t) for t in args], C.ptr(out), C.ptr(logp),
-                                               C.ptr(kl), C.ptr(stats), C.stream_ptr()), "bg_policy_loss_fwd")
+                                               C.ptr(kl), C.ptr(stats), C.ptr(dx), ctypes.byref(has), C.stream_ptr()), "bg_policy_loss_fwd")
         ctx.save_for_backward(x, ids, stats, *(() if y is None else (y,)))
+        ctx.dx = dx if has.value else None
         ctx.sh, ctx.in_shape = sh, logits.shape
         loss, logp, kl = out.view(()), logp.view(logits.shape[:-1]), kl.view(logits.shape[:-1])
         ctx.mark_non_differentiable(logp, kl)
@@ -956,10 +960,13 @@ class _PolicyLoss(torch.autograd.Function):
         x, ids, stats = ctx.saved_tensors[:3]
         y = ctx.saved_tensors[3] if len(ctx.saved_tensors) > 3 else None
         g = g_loss.reshape(1).contiguous().float()
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dx, ctx.dx = ctx.dx, None                     # the buffer is handed out once: a second backward computes its own
+        has = dx is not None
+        if not has:
+            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         with torch.cuda.device(x.device), _timed(f"policy_loss_bwd[{x.shape[0]}]"):
             C.check(C.lib().bg_policy_loss_bwd(ctypes.byref(ctx.sh), C.ptr(x), C.ptr(y), C.ptr(ids), C.ptr(stats), C.ptr(g), C.ptr(dx),
-                                               C.stream_ptr()), "bg_policy_loss_bwd")
+                                               int(has), C.stream_ptr()), "bg_policy_loss_bwd")
         return (dx.view(ctx.in_shape),) + (None,) * 11
 
 

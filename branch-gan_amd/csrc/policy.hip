@@ -1,17 +1,30 @@
 // Clipped policy loss with a KL term over the vocabulary, forward and backward (bg_policy_loss_fwd / _bwd).
 //
-// Per row, x = logits / T and c = log2(e) / T:  e_j = 2^(c (logit_j - m)), s = sum e_j, lse = m / T + log s;  with reference logits y
-// (the same m', s') the KL is  sum_j p_j ((x_j - x_id) - (y_j - y_id)) - ((lse_x - x_id) - (lse_y - y_id)): the differences are taken
-// before the sum and against the sampled token's logits, so neither the logits' size nor an offset between the two models' logits
-// (which softmax does not see) costs a policy close to its reference any digits.  c is carried in two floats (its rounding would shift every lse the
-// same way); lse, the token's log-prob and the row's loss are put together in fp64 - a handful of operations per row.
+// Per row, c = log2(e) / T and m the largest logit:  e_j = 2^(c (logit_j - m)), s = sum e_j, lse = m / T + log s;  with reference
+// logits (m', s') the KL is  sum_j p_j ((logit_j - m) - (ref_j - m')) / T - (log s - log s'): the differences are taken against the
+// maxima and before the sum, so neither the logits' size nor an offset between the two models' logits (which softmax does not
+// see) costs a policy close to its reference any digits.  c is carried in two floats (its rounding would shift every lse the same
+// way); the token's log-prob and the loss are put together in fp64 - a handful of operations per row.
 //
-// HBM-bound: forward reads the logits (and reference logits) once, backward reads them again and writes dlogits.
+// HBM-bound.  policy_row_kernel holds a row (and the reference's) in registers from its one reading to the gradient's writing: the
+// whole of value and gradient is logits in, dlogits out.  The gradient is the one for g_loss = 1; bg_policy_loss_bwd does it over
+// when the loss was scaled after all.  Rows too long for the registers take policy_rows_kernel (forward) and policy_grad_kernel
+// (backward), one more reading of the logits.
 #include "common.h"
 
 namespace bg {
 
-constexpr int PT = 256;      // threads per row
+constexpr int PT = 256;      // threads per row of the streaming kernels
+
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+  static constexpr int N = 4;
+  typedef f32x4 type;
+};
+template <> struct Vec<bf16_t> {
+  static constexpr int N = 8;
+  typedef bf16x8 type;
+};
 
 struct PolicyArgs {
   const void* logits;
@@ -26,163 +39,386 @@ struct PolicyArgs {
   float c_hi, c_lo, inv_t32;
   float* out_logp;
   float* out_kl;
-  float* stats;              // per row: m, 1 / s, w dloss_row/dlogp, w kl_coef, (lse_x - x0) - (lse_y - y0), kl, w loss_row (a double);  then 1 / N
+  float* stats;              // per row: m, 1 / s, w dloss_row/dlogp, w kl_coef, log s - log s' + kl, m', w loss_row (a double);  then 1 / N
 };
 
-__device__ __forceinline__ float policy_exp(float d, float c_hi, float c_lo) {        // 2^(d c), d <= 0
+// 2^(d c), d <= 0.  c_hi < c, so that c_lo > 0 and d = -inf gives 0, not a NaN.
+__device__ __forceinline__ float policy_exp(float d, float c_hi, float c_lo) {
   return __builtin_amdgcn_exp2f(__builtin_fmaf(d, c_hi, d * c_lo));
 }
 
-// running maximum, sum of exponentials and sum of exponentials times the difference to the reference
-struct RowSum {
-  float m, s, t;
-  __device__ __forceinline__ void rescale(float mn, float c_hi, float c_lo) {
-    if (mn > m) {
-      const float f = m == -INFINITY ? 0.f : policy_exp(m - mn, c_hi, c_lo);
-      s *= f;
-      t *= f;
-      m = mn;
-    }
-  }
-  __device__ __forceinline__ void join(const RowSum& o, float c_hi, float c_lo) {
-    const float mn = fmaxf(m, o.m);
-    rescale(mn, c_hi, c_lo);
-    const float f = o.m == -INFINITY ? (o.s == 0.f ? 0.f : 1.f) : policy_exp(o.m - mn, c_hi, c_lo);
-    s += f * o.s;
-    t += f * o.t;
-  }
-};
+// a row's vectors lie on the 16-byte grid: vector i holds the elements [i N - mis, i N - mis + N), the first and last in part
+template <typename T> __device__ __forceinline__ int misalignment(const void* p) { return (int)(((uintptr_t)p & 15) / sizeof(T)); }
 
-__device__ __forceinline__ RowSum row_join(RowSum r, RowSum* red, float c_hi, float c_lo) {
+// vector at element e0 of a row; elements outside [0, V) are -inf.  aligned: p + e0 is on the grid.
+template <typename T> __device__ __forceinline__ typename Vec<T>::type row_vector(const T* p, int64_t e0, int64_t V, bool aligned) {
+  typename Vec<T>::type r;
+  if (aligned && e0 >= 0 && e0 + Vec<T>::N <= V) return *(const typename Vec<T>::type*)(p + e0);
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    RowSum b;
-    b.m = __shfl_xor(r.m, o); b.s = __shfl_xor(r.s, o); b.t = __shfl_xor(r.t, o);
-    r.join(b, c_hi, c_lo);
-  }
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = r;
-  __syncthreads();
-  r = red[0];
-  for (int w = 1; w < PT / 64; ++w) r.join(red[w], c_hi, c_lo);
+  for (int k = 0; k < Vec<T>::N; ++k) r[k] = e0 + k >= 0 && e0 + k < V ? p[e0 + k] : from_f32<T>(-INFINITY);
   return r;
 }
-
-// what the logits of a row are taken against in differences: the sampled token's (0 if that one is masked or broken)
-template <typename T> __device__ __forceinline__ float row_origin(const T* x, int64_t id) {
-  const float v = to_f32(x[id]);
-  return __builtin_fabsf(v) <= 3.0e38f ? v : 0.f;
+template <typename T> __device__ __forceinline__ void store_row_vector(T* p, int64_t e0, int64_t V, bool aligned, const float (&x)[Vec<T>::N]) {
+  if (aligned && e0 >= 0 && e0 + Vec<T>::N <= V) {
+    typename Vec<T>::type r;
+#pragma unroll
+    for (int k = 0; k < Vec<T>::N; ++k) r[k] = from_f32<T>(x[k]);
+    *(typename Vec<T>::type*)(p + e0) = r;
+  } else {
+#pragma unroll
+    for (int k = 0; k < Vec<T>::N; ++k)
+      if (e0 + k >= 0 && e0 + k < V) p[e0 + k] = from_f32<T>(x[k]);
+  }
 }
+
+// over the workgroup's NW waves, the result in every thread
+template <int NW> __device__ __forceinline__ float block_max(float v, float* red) {
+  v = wave_max(v);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = red[0];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) v = fmaxf(v, red[w]);
+  return v;
+}
+
+// Ends the compiler's knowledge of a register's value: the row is kept as it was read and unpacked anew by each pass over it (left to
+// itself the compiler keeps the unpacked floats of bf16 rows from one pass to the next, twice the registers).
+template <typename V> __device__ __forceinline__ void forget(V& v) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  u32x4 u = __builtin_bit_cast(u32x4, v);
+  asm volatile("" : "+v"(u));
+  v = __builtin_bit_cast(V, u);
+}
+
+struct RowResult {          // what the gradient of a row needs
+  float m, inv_s, slope, w_kl, off, my;
+};
 
 __device__ __forceinline__ float row_weight(const PolicyArgs& a, int64_t row) {
   const int64_t id = a.ids[row];
   return id >= 0 && id < a.V ? (a.weights ? a.weights[row] : 1.f) : 0.f;
 }
 
-template <typename T, bool REF>
-__global__ __launch_bounds__(PT) void policy_rows_kernel(PolicyArgs a) {
-  __shared__ RowSum red[PT / 64];
+// log of a sum to ~1e-11, in few registers (the row sits in them meanwhile): s = 2^e f with f in [0.7, 1.42), log f = 2 atanh(z),
+// z = (f - 1) / (f + 1), by its series (|z| < 0.176: the first term left out is below 2 z^17 / 17 < 2e-14).
+__device__ __forceinline__ double log_sum(double s) {
+  if (!(s > 0.0 && s < 1e300)) return s == 0.0 ? -(double)INFINITY : s;          // an empty row; a broken one stays NaN
+  int e;
+  double f = frexp(s, &e);
+  if (f < 0.7071067811865476) { f += f; e -= 1; }
+  const double z = (f - 1.0) / (f + 1.0), z2 = z * z;
+  double q = 1.0 / 15.0;
+  q = fma(q, z2, 1.0 / 13.0); q = fma(q, z2, 1.0 / 11.0); q = fma(q, z2, 1.0 / 9.0);
+  q = fma(q, z2, 1.0 / 7.0); q = fma(q, z2, 1.0 / 5.0); q = fma(q, z2, 1.0 / 3.0);
+  return fma((double)e, 0.6931471805599453, 2.0 * fma(z * z2, q, z));
+}
+
+// One thread: the row's statistics to its log-prob, KL, loss term and gradient factors.
+template <bool REF>
+__device__ RowResult finish_row(const PolicyArgs& a, int64_t row, float w, float m, double s, float my, double sy, double t, float x_id) {
+  const double ls = log_sum(s);
+  const double logp = ((double)x_id - m) * a.inv_t - ls;
+  const float ratio = expf((float)(logp - a.old_logp[row])), A = a.adv[row];
+  const float lo = (float)(1.0 - a.clip_low), hi = (float)(1.0 + a.clip_high);
+  const float plain = -A * ratio, clipped = -A * fminf(fmaxf(ratio, lo), hi);
+  const float pg = plain != plain ? plain : fmaxf(plain, clipped);
+  RowResult r;
+  r.m = m;
+  r.inv_s = 1.f / (float)s;
+  float slope = plain >= clipped || plain != plain ? plain : 0.f;
+  double gap = 0.0;
+  float kl = 0.f;
+  if constexpr (REF) {
+    gap = ls - log_sum(sy);
+    kl = (float)(t / s * a.inv_t - gap);
+  } else if (a.ref_logp) {
+    const float d = (float)((double)a.ref_logp[row] - logp);
+    float e1;                                                        // exp(d) - 1
+    if (__builtin_fabsf(d) < 0.5f) {                                 // exp(d) - 1 - d by its series: d^11 / 11! < 2^-24 of it
+      float q = 1.f / 10.f;
+#pragma unroll
+      for (int i = 9; i >= 3; --i) q = __builtin_fmaf(d, q, 1.f) / (float)i;
+      kl = 0.5f * d * d * __builtin_fmaf(d, q, 1.f);
+      e1 = kl + d;
+    } else {
+      e1 = expf(d) - 1.f;                                           // |d| >= 1/2: no digits to lose
+      kl = e1 - d;
+    }
+    slope -= (float)a.kl_coef * e1;
+  }
+  r.slope = w * slope;
+  r.w_kl = (float)(w * a.kl_coef);
+  r.off = (float)gap + kl;
+  r.my = my;
+  a.out_logp[row] = (float)logp;
+  a.out_kl[row] = kl;
+  float* st = a.stats + row * BG_POLICY_STATS;
+  st[0] = r.m; st[1] = r.inv_s; st[2] = r.slope; st[3] = r.w_kl; st[4] = r.off; st[5] = r.my;
+  *(double*)(st + 6) = (double)w * (pg + a.kl_coef * kl);
+  return r;
+}
+
+__device__ __forceinline__ void skip_row(const PolicyArgs& a, int64_t row) {     // it does not count
+  if (threadIdx.x < BG_POLICY_STATS) a.stats[row * BG_POLICY_STATS + threadIdx.x] = 0.f;
+  if (threadIdx.x == 0) { a.out_logp[row] = 0.f; a.out_kl[row] = 0.f; }
+}
+
+// d loss / d logit of one element from its p and, with a reference, the difference of the two logits
+template <bool REF>
+__device__ __forceinline__ float grad_of(float p, float diff, float slope, float w_kl, float off, float inv_t) {
+  float d = -slope * p;
+  if constexpr (REF) {
+    const float k = w_kl * p * __builtin_fmaf(diff, inv_t, -off);
+    d += p != 0.f ? k : 0.f;                                         // a masked entry: its difference may be infinite
+  }
+  return d;
+}
+
+// 1 / N, N = sum of the weights that count (or the denominator) -> stats[rows * BG_POLICY_STATS]
+__global__ __launch_bounds__(1024) void policy_norm_kernel(PolicyArgs a, const float* denominator) {
+  __shared__ double red[16];
+  double n = 0.0;
+  if (denominator) {
+    n = denominator[0];
+  } else {
+    for (int64_t r = threadIdx.x; r < a.rows; r += 1024) n += row_weight(a, r);
+    n = wave_sum(n);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = n;
+    __syncthreads();
+    n = 0.0;
+    for (int i = 0; i < 16; ++i) n += red[i];
+  }
+  if (threadIdx.x == 0) a.stats[a.rows * BG_POLICY_STATS] = n == 0.0 ? 0.f : (float)(1.0 / n);
+}
+
+// loss = sum of the rows' terms / N, in a fixed order, fp64
+__global__ __launch_bounds__(1024) void policy_total_kernel(PolicyArgs a, float* out_loss) {
+  __shared__ double red[16];
+  double sum = 0.0;
+  for (int64_t r = threadIdx.x; r < a.rows; r += 1024) sum += *(const double*)(a.stats + r * BG_POLICY_STATS + 6);
+  sum = wave_sum(sum);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    sum = 0.0;
+    for (int i = 0; i < 16; ++i) sum += red[i];
+    const float inv_n = a.stats[a.rows * BG_POLICY_STATS];
+    out_loss[0] = inv_n == 0.f ? 0.f : (float)(sum * inv_n);
+  }
+}
+
+// Value and (dlogits != NULL) gradient of a row of at most NT * NV whole vectors, read once.  Its interior - the vectors that lie
+// wholly inside - is loaded without branches (indices clamped, what is outside set to -inf), so that all loads of a thread are under
+// way together; the fewer than 2 N elements before and after it go one each to the first threads.  Sums: fp32 per thread, fp64
+// across them.
+template <typename T, bool REF, int NT, int NV>
+__global__ __launch_bounds__(NT, 4) void policy_row_kernel(PolicyArgs a, T* dlogits) {
+  constexpr int N = Vec<T>::N, NW = NT / 64;
+  typedef typename Vec<T>::type V_t;
+  __shared__ float red_m[2][NW];
+  __shared__ double red[NW][3];
+  __shared__ RowResult sh_row;
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x;
-  float* st = a.stats + row * BG_POLICY_STATS;
+  const T* x = (const T*)a.logits + row * a.x_stride;
+  const T* y = REF ? (const T*)a.ref + row * a.ref_stride : nullptr;
+  T* dx = dlogits ? dlogits + row * a.V : nullptr;
+  const int V = (int)a.V, mis = misalignment<T>(x);
   const float w = row_weight(a, row);
   if (w == 0.f) {
-    if (tid < BG_POLICY_STATS) st[tid] = 0.f;
-    if (tid == 0) { a.out_logp[row] = 0.f; a.out_kl[row] = 0.f; }
+    skip_row(a, row);
+    const float zero[N] = {};
+    if (dlogits)
+      for (int i = tid; i * N - mis < V; i += NT) store_row_vector<T>(dx, i * N - mis, V, true, zero);
     return;
   }
-  const T* x = (const T*)a.logits + row * a.x_stride;
-  const T* y = REF ? (const T*)a.ref + row * a.ref_stride : nullptr;
-  const int64_t id = a.ids[row];
-  const float x0 = REF ? row_origin(x, id) : 0.f, y0 = REF ? row_origin(y, id) : 0.f;
-  RowSum rx = {-INFINITY, 0.f, 0.f}, ry = rx;
-  for (int64_t j = tid; j < a.V; j += PT) {
-    const float v = to_f32(x[j]);
-    rx.rescale(v, a.c_hi, a.c_lo);
-    const float e = v == -INFINITY ? 0.f : policy_exp(v - rx.m, a.c_hi, a.c_lo);
-    rx.s += e;
-    if constexpr (REF) {
-      const float u = to_f32(y[j]);
-      ry.rescale(u, a.c_hi, a.c_lo);
-      ry.s += u == -INFINITY ? 0.f : policy_exp(u - ry.m, a.c_hi, a.c_lo);
-      if (e != 0.f) rx.t += e * ((v - x0) - (u - y0));
+  const int lo = mis ? 1 : 0, hi = (V + mis) / N;                      // interior vectors (at least one: V >= 2 N)
+  const int head = lo * N - mis > 0 ? lo * N - mis : 0, tail = hi * N - mis;
+  const int extra = tid < head ? tid : tail + tid - head;              // the single element of this thread, if below V
+  const bool has_extra = extra < V;
+  V_t vx[NV], vy[REF ? NV : 1];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int i = min(max(tid + k * NT, lo), hi - 1);
+    vx[k] = *(const V_t*)(x + (i * N - mis));
+    if constexpr (REF) vy[k] = *(const V_t*)(y + (i * N - mis));
+  }
+  const float ex = has_extra ? to_f32(x[extra]) : -INFINITY, ey = REF && has_extra ? to_f32(y[extra]) : -INFINITY;
+  const int id = (int)a.ids[row];
+  const float x_id = to_f32(x[id]);
+  const float inv_n = a.stats[a.rows * BG_POLICY_STATS];
+  V_t none;
+#pragma unroll
+  for (int j = 0; j < N; ++j) none[j] = from_f32<T>(-INFINITY);
+  float m = ex, my = ey;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int i = tid + k * NT;
+    if (k == 0 || (k + 1) * NT > hi) {
+      const bool in = i >= lo && i < hi;
+      vx[k] = in ? vx[k] : none;
+      if constexpr (REF) vy[k] = in ? vy[k] : none;
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      m = fmaxf(m, (float)vx[k][j]);
+      if constexpr (REF) my = fmaxf(my, (float)vy[k][j]);
     }
   }
-  rx = row_join(rx, red, a.c_hi, a.c_lo);
-  if constexpr (REF) ry = row_join(ry, red, a.c_hi, a.c_lo);
-  if (tid != 0) return;
-  const double ls = log((double)rx.s);
-  const double logp = ((double)to_f32(x[id]) - rx.m) * a.inv_t - ls;
-  const double ratio = exp(logp - a.old_logp[row]), A = a.adv[row];
-  const double plain = -A * ratio;
-  const double clipped = -A * fmin(fmax(ratio, 1.0 - a.clip_low), 1.0 + a.clip_high);
-  double slope = plain >= clipped || plain != plain ? plain : 0.0;
-  double kl = 0.0, gap = 0.0;
-  if constexpr (REF) {
-    gap = (((double)rx.m - x0) - ((double)ry.m - y0)) * a.inv_t + (ls - log((double)ry.s));
-    kl = (double)rx.t / (double)rx.s * a.inv_t - gap;
-  } else if (a.ref_logp) {
-    const double d = a.ref_logp[row] - logp, e1 = expm1(d);
-    kl = e1 - d;
-    slope -= a.kl_coef * e1;
+  m = block_max<NW>(m, red_m[0]);
+  if constexpr (REF) my = block_max<NW>(my, red_m[1]);
+  const float ms = m == -INFINITY ? 0.f : m, mys = my == -INFINITY ? 0.f : my;
+  float s = 0.f, sy = 0.f, t = 0.f;
+  auto add = [&](float v, float u) __attribute__((always_inline)) {
+    const float dv = v - ms, e = policy_exp(dv, a.c_hi, a.c_lo);
+    s += e;
+    if constexpr (REF) {
+      const float du = u - mys, d = e * (dv - du);
+      sy += policy_exp(du, a.c_hi, a.c_lo);
+      t += e != 0.f ? d : 0.f;                                         // a masked entry: its difference may be infinite
+    }
+  };
+  add(ex, ey);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    forget(vx[k]);
+    if constexpr (REF) forget(vy[k]);
+#pragma unroll
+    for (int j = 0; j < N; ++j) add((float)vx[k][j], REF ? (float)vy[REF ? k : 0][j] : 0.f);
   }
-  const double pg = plain != plain ? plain : fmax(plain, clipped);
-  a.out_logp[row] = (float)logp;
-  a.out_kl[row] = (float)kl;
-  st[0] = rx.m;
-  st[1] = (float)(1.0 / rx.s);
-  st[2] = (float)(w * slope);
-  st[3] = (float)(w * a.kl_coef);
-  st[4] = (float)gap;
-  st[5] = (float)kl;
-  *(double*)(st + 6) = w * (pg + a.kl_coef * kl);
-}
-
-// loss = sum_r w_r (pg + kl_coef kl) / N in a fixed order, fp64; stats[rows * BG_POLICY_STATS] = 1 / N
-__global__ __launch_bounds__(1024) void policy_total_kernel(PolicyArgs a, const float* denominator, float* out_loss) {
-  __shared__ double red[2][16];
-  const int tid = threadIdx.x;
-  double sum = 0.0, wsum = 0.0;
-  for (int64_t r = tid; r < a.rows; r += 1024) {
-    sum += *(const double*)(a.stats + r * BG_POLICY_STATS + 6);
-    wsum += row_weight(a, r);
-  }
-  sum = wave_sum(sum);
-  wsum = wave_sum(wsum);
-  if ((tid & 63) == 0) { red[0][tid >> 6] = sum; red[1][tid >> 6] = wsum; }
+  const double s64 = wave_sum((double)s), t64 = REF ? wave_sum((double)t) : 0.0, sy64 = REF ? wave_sum((double)sy) : 0.0;
+  if ((tid & 63) == 0) { red[tid >> 6][0] = s64; red[tid >> 6][1] = t64; red[tid >> 6][2] = sy64; }
   __syncthreads();
   if (tid == 0) {
-    sum = wsum = 0.0;
-    for (int i = 0; i < 16; ++i) { sum += red[0][i]; wsum += red[1][i]; }
-    const double n = denominator ? (double)denominator[0] : wsum;
-    out_loss[0] = n == 0.0 ? 0.f : (float)(sum / n);
-    a.stats[a.rows * BG_POLICY_STATS] = n == 0.0 ? 0.f : (float)(1.0 / n);
+    double S = 0.0, Tt = 0.0, Sy = 0.0;
+    for (int i = 0; i < NW; ++i) { S += red[i][0]; Tt += red[i][1]; Sy += red[i][2]; }
+    sh_row = finish_row<REF>(a, row, w, ms, S, mys, Sy, Tt, x_id);
+  }
+  if (!dlogits) return;
+  __syncthreads();
+  const RowResult r = sh_row;
+  const float f = inv_n * a.inv_t32, slope = f * r.slope, w_kl = f * r.w_kl, off = r.off;
+  auto grad = [&](float v, float u) __attribute__((always_inline)) {
+    const float dv = v - ms, p = policy_exp(dv, a.c_hi, a.c_lo) * r.inv_s;
+    return grad_of<REF>(p, REF ? dv - (u - mys) : 0.f, slope, w_kl, off, a.inv_t32);
+  };
+  if (has_extra) dx[extra] = from_f32<T>(grad(ex, ey) + (extra == id ? slope : 0.f));
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int i = tid + k * NT;
+    if (i >= lo && i < hi) {
+      forget(vx[k]);
+      if constexpr (REF) forget(vy[k]);
+      float d[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) d[j] = grad((float)vx[k][j], REF ? (float)vy[REF ? k : 0][j] : 0.f);
+      const int hit = id - (i * N - mis);
+      if (hit >= 0 && hit < N) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) d[j] += hit == j ? slope : 0.f;
+      }
+      V_t o;
+#pragma unroll
+      for (int j = 0; j < N; ++j) o[j] = from_f32<T>(d[j]);
+      *(V_t*)(dx + (i * N - mis)) = o;
+    }
   }
 }
 
+// Streaming forward for rows of any length: the maximum in one reading, the sums in a second.
 template <typename T, bool REF>
-__global__ __launch_bounds__(PT) void policy_grad_kernel(PolicyArgs a, const float* g_loss, T* dlogits) {
+__global__ __launch_bounds__(PT) void policy_rows_kernel(PolicyArgs a) {
+  constexpr int N = Vec<T>::N, NW = PT / 64;
+  __shared__ float red_m[2][NW];
+  __shared__ double red[NW][3];
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x;
-  T* dx = dlogits + row * a.V;
-  const float* st = a.stats + row * BG_POLICY_STATS;
-  if (st[1] == 0.f) {                       // does not count (a row that does has s >= 1)
-    for (int64_t j = tid; j < a.V; j += PT) dx[j] = from_f32<T>(0.f);
+  const float w = row_weight(a, row);
+  if (w == 0.f) {
+    skip_row(a, row);
     return;
   }
   const T* x = (const T*)a.logits + row * a.x_stride;
   const T* y = REF ? (const T*)a.ref + row * a.ref_stride : nullptr;
-  const float f = g_loss[0] * a.stats[a.rows * BG_POLICY_STATS] * a.inv_t32;
-  const float m = st[0], inv_s = st[1], cA = f * st[2], cK = f * st[3], off = st[4] + st[5];
+  const int mis = misalignment<T>(x);
+  const bool y_on = !REF || misalignment<T>(y) == mis;
   const int64_t id = a.ids[row];
-  const float x0 = REF ? row_origin(x, id) : 0.f, y0 = REF ? row_origin(y, id) : 0.f;
-  for (int64_t j = tid; j < a.V; j += PT) {
-    const float v = to_f32(x[j]);
-    const float p = v == -INFINITY ? 0.f : policy_exp(v - m, a.c_hi, a.c_lo) * inv_s;
-    float d = cA * ((j == id ? 1.f : 0.f) - p);
-    if constexpr (REF)
-      if (p != 0.f) d += cK * p * (((v - x0) - (to_f32(y[j]) - y0)) * a.inv_t32 - off);
-    dx[j] = from_f32<T>(d);
+  float m = -INFINITY, my = -INFINITY;
+  for (int64_t e0 = (int64_t)tid * N - mis; e0 < a.V; e0 += PT * N) {
+    const typename Vec<T>::type vx = row_vector<T>(x, e0, a.V, true);
+    typename Vec<T>::type vy;
+    if constexpr (REF) vy = row_vector<T>(y, e0, a.V, y_on);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      m = fmaxf(m, (float)vx[j]);
+      if constexpr (REF) my = fmaxf(my, (float)vy[j]);
+    }
+  }
+  m = block_max<NW>(m, red_m[0]);
+  if constexpr (REF) my = block_max<NW>(my, red_m[1]);
+  const float ms = m == -INFINITY ? 0.f : m, mys = my == -INFINITY ? 0.f : my;
+  double s64 = 0.0, sy64 = 0.0, t64 = 0.0;
+  for (int64_t e0 = (int64_t)tid * N - mis; e0 < a.V; e0 += PT * N) {
+    const typename Vec<T>::type vx = row_vector<T>(x, e0, a.V, true);
+    typename Vec<T>::type vy;
+    if constexpr (REF) vy = row_vector<T>(y, e0, a.V, y_on);
+    float s = 0.f, sy = 0.f, t = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float dv = (float)vx[j] - ms, e = policy_exp(dv, a.c_hi, a.c_lo);
+      s += e;
+      if constexpr (REF) {
+        const float du = (float)vy[j] - mys, d = e * (dv - du);
+        sy += policy_exp(du, a.c_hi, a.c_lo);
+        t += e != 0.f ? d : 0.f;
+      }
+    }
+    s64 += s; sy64 += sy; t64 += t;
+  }
+  s64 = wave_sum(s64); t64 = wave_sum(t64); sy64 = wave_sum(sy64);
+  if ((tid & 63) == 0) { red[tid >> 6][0] = s64; red[tid >> 6][1] = t64; red[tid >> 6][2] = sy64; }
+  __syncthreads();
+  if (tid == 0) {
+    double S = 0.0, Tt = 0.0, Sy = 0.0;
+    for (int i = 0; i < NW; ++i) { S += red[i][0]; Tt += red[i][1]; Sy += red[i][2]; }
+    finish_row<REF>(a, row, w, ms, S, mys, Sy, Tt, to_f32(x[id]));
+  }
+}
+
+// Streaming gradient from the rows' statistics.  unless_one: dlogits holds the gradient for g_loss = 1 already, so that value ends it.
+template <typename T, bool REF>
+__global__ __launch_bounds__(PT) void policy_grad_kernel(PolicyArgs a, const float* g_loss, T* dlogits, int unless_one) {
+  constexpr int N = Vec<T>::N;
+  const float g = g_loss[0];
+  if (unless_one && g == 1.f) return;
+  const int tid = threadIdx.x;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    T* dx = dlogits + row * a.V;
+    const T* x = (const T*)a.logits + row * a.x_stride;
+    const T* y = REF ? (const T*)a.ref + row * a.ref_stride : nullptr;
+    const int mis = misalignment<T>(x);
+    const bool y_on = !REF || misalignment<T>(y) == mis, d_on = misalignment<T>(dx) == mis;
+    const float* st = a.stats + row * BG_POLICY_STATS;
+    const float ms = st[0], inv_s = st[1], off = st[4], mys = st[5];
+    const bool counts = inv_s != 0.f;                                  // a row that counts has a finite (or NaN) sum
+    const float f = g * a.stats[a.rows * BG_POLICY_STATS] * a.inv_t32, slope = f * st[2], w_kl = f * st[3];
+    const int64_t id = a.ids[row];
+    for (int64_t e0 = (int64_t)tid * N - mis; e0 < a.V; e0 += PT * N) {
+      float d[N] = {};
+      if (counts) {
+        const typename Vec<T>::type vx = row_vector<T>(x, e0, a.V, true);
+        typename Vec<T>::type vy;
+        if constexpr (REF) vy = row_vector<T>(y, e0, a.V, y_on);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const float dv = (float)vx[j] - ms, p = policy_exp(dv, a.c_hi, a.c_lo) * inv_s;
+          d[j] = grad_of<REF>(p, REF ? dv - ((float)vy[j] - mys) : 0.f, slope, w_kl, off, a.inv_t32);
+          if (e0 + j == id) d[j] += slope;
+        }
+      }
+      store_row_vector<T>(dx, e0, a.V, d_on, d);
+    }
   }
 }
 
@@ -208,48 +444,78 @@ static PolicyArgs policy_args(const bg_policy_shape* sh, const void* logits, con
   a.inv_t = 1.0 / sh->temperature;
   a.clip_low = sh->clip_low; a.clip_high = sh->clip_high; a.kl_coef = sh->kl_coef;
   const double c = 1.4426950408889634 / sh->temperature;
-  a.c_hi = (float)c;
+  a.c_hi = __builtin_nextafterf((float)c, 0.f);
   a.c_lo = (float)(c - (double)a.c_hi);
   a.inv_t32 = (float)a.inv_t;
   return a;
 }
 
+// Rows of at most NT * NV vectors.  Few threads for short rows; for the usual vocabularies
+// 512, so that two rows share a CU and one's loads cover the other's exponentials.
+template <typename T, bool REF> static bool policy_row_launch(const PolicyArgs& a, T* dlogits, hipStream_t st) {
+  const int64_t nvec = a.V / Vec<T>::N + 1;
+  if (a.V < 2 * Vec<T>::N) return false;
+  // reference or gradient rows that lie elsewhere on the 16-byte grid than the logits': the streaming kernels
+  const auto same_grid = [&](const void* p, int64_t stride) {
+    return (((uintptr_t)a.logits ^ (uintptr_t)p) & 15) == 0 && (a.x_stride - stride) * (int64_t)sizeof(T) % 16 == 0;
+  };
+  if (REF && !same_grid(a.ref, a.ref_stride)) return false;
+  if (dlogits && !same_grid(dlogits, a.V)) return false;
+  const dim3 grid((unsigned)a.rows);
+  if (nvec <= 256 * 2) hipLaunchKernelGGL((policy_row_kernel<T, REF, 256, 2>), grid, dim3(256), 0, st, a, dlogits);
+  else if (nvec <= 256 * 8) hipLaunchKernelGGL((policy_row_kernel<T, REF, 256, 8>), grid, dim3(256), 0, st, a, dlogits);
+  else if (nvec <= 512 * 13) hipLaunchKernelGGL((policy_row_kernel<T, REF, 512, 13>), grid, dim3(512), 0, st, a, dlogits);
+  else if (nvec <= 1024 * 13) hipLaunchKernelGGL((policy_row_kernel<T, REF, 1024, 13>), grid, dim3(1024), 0, st, a, dlogits);
+  else return false;
+  return true;
+}
+
+template <typename T, bool REF>
+static void policy_grad_launch(const PolicyArgs& a, const float* g_loss, T* dlogits, int unless_one, hipStream_t st) {
+  const int64_t most = unless_one ? 2048 : a.rows;                     // a launch that may have nothing to do: few workgroups
+  hipLaunchKernelGGL((policy_grad_kernel<T, REF>), dim3((unsigned)(a.rows < most ? a.rows : most)), dim3(PT), 0, st, a, g_loss, dlogits, unless_one);
+}
+
+template <typename T, bool REF> static int policy_fwd(const PolicyArgs& a, T* dlogits, hipStream_t st) {
+  if (policy_row_launch<T, REF>(a, dlogits, st)) return dlogits ? 1 : 0;
+  hipLaunchKernelGGL((policy_rows_kernel<T, REF>), dim3((unsigned)a.rows), dim3(PT), 0, st, a);
+  return 0;
+}
+
 extern "C" int bg_policy_loss_fwd(const bg_policy_shape* sh, const void* logits, const void* ref_logits, const int64_t* ids,
                                   const float* old_logp, const float* ref_logp, const float* advantages, const float* weights,
-                                  const float* denominator, float* out_loss, float* out_logp, float* out_kl, float* stats, void* stream) {
+                                  const float* denominator, float* out_loss, float* out_logp, float* out_kl, float* stats, void* dlogits,
+                                  int* has_gradient, void* stream) {
   if (int rc = policy_check("bg_policy_loss_fwd", sh, logits, ref_logits, ids, stats)) return rc;
   BG_REQUIRE(old_logp && advantages && out_loss && out_logp && out_kl, "bg_policy_loss_fwd: null argument");
   BG_REQUIRE(!(ref_logits && ref_logp), "bg_policy_loss_fwd: ref_logits and ref_logp exclude each other");
+  BG_REQUIRE(!dlogits || has_gradient, "bg_policy_loss_fwd: dlogits without has_gradient");
   PolicyArgs a = policy_args(sh, logits, ref_logits, ids, stats);
   a.old_logp = old_logp; a.ref_logp = ref_logp; a.adv = advantages; a.weights = weights;
   a.out_logp = out_logp; a.out_kl = out_kl;
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)sh->rows), block(PT);
-  if (sh->dtype == BG_F32) {
-    if (ref_logits) hipLaunchKernelGGL((policy_rows_kernel<float, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((policy_rows_kernel<float, false>), grid, block, 0, st, a);
-  } else {
-    if (ref_logits) hipLaunchKernelGGL((policy_rows_kernel<bf16_t, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((policy_rows_kernel<bf16_t, false>), grid, block, 0, st, a);
-  }
-  hipLaunchKernelGGL(policy_total_kernel, dim3(1), dim3(1024), 0, st, a, denominator, out_loss);
+  hipLaunchKernelGGL(policy_norm_kernel, dim3(1), dim3(1024), 0, st, a, denominator);
+  int wrote;
+  if (sh->dtype == BG_F32) wrote = ref_logits ? policy_fwd<float, true>(a, (float*)dlogits, st) : policy_fwd<float, false>(a, (float*)dlogits, st);
+  else wrote = ref_logits ? policy_fwd<bf16_t, true>(a, (bf16_t*)dlogits, st) : policy_fwd<bf16_t, false>(a, (bf16_t*)dlogits, st);
+  if (has_gradient) *has_gradient = wrote;
+  hipLaunchKernelGGL(policy_total_kernel, dim3(1), dim3(1024), 0, st, a, out_loss);
   BG_CHECK_LAUNCH("bg_policy_loss_fwd");
   return BG_OK;
 }
 
 extern "C" int bg_policy_loss_bwd(const bg_policy_shape* sh, const void* logits, const void* ref_logits, const int64_t* ids,
-                                  const float* stats, const float* g_loss, void* dlogits, void* stream) {
+                                  const float* stats, const float* g_loss, void* dlogits, int has_gradient, void* stream) {
   if (int rc = policy_check("bg_policy_loss_bwd", sh, logits, ref_logits, ids, stats)) return rc;
   BG_REQUIRE(g_loss && dlogits, "bg_policy_loss_bwd: null argument");
   const PolicyArgs a = policy_args(sh, logits, ref_logits, ids, (float*)stats);
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)sh->rows), block(PT);
   if (sh->dtype == BG_F32) {
-    if (ref_logits) hipLaunchKernelGGL((policy_grad_kernel<float, true>), grid, block, 0, st, a, g_loss, (float*)dlogits);
-    else hipLaunchKernelGGL((policy_grad_kernel<float, false>), grid, block, 0, st, a, g_loss, (float*)dlogits);
+    if (ref_logits) policy_grad_launch<float, true>(a, g_loss, (float*)dlogits, has_gradient, st);
+    else policy_grad_launch<float, false>(a, g_loss, (float*)dlogits, has_gradient, st);
   } else {
-    if (ref_logits) hipLaunchKernelGGL((policy_grad_kernel<bf16_t, true>), grid, block, 0, st, a, g_loss, (bf16_t*)dlogits);
-    else hipLaunchKernelGGL((policy_grad_kernel<bf16_t, false>), grid, block, 0, st, a, g_loss, (bf16_t*)dlogits);
+    if (ref_logits) policy_grad_launch<bf16_t, true>(a, g_loss, (bf16_t*)dlogits, has_gradient, st);
+    else policy_grad_launch<bf16_t, false>(a, g_loss, (bf16_t*)dlogits, has_gradient, st);
   }
   BG_CHECK_LAUNCH("bg_policy_loss_bwd");
   return BG_OK;

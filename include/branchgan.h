@@ -538,6 +538,9 @@ int bg_kv_cache_attn_fwd(const bg_kv_cache* cache, const void* data, const void*
  * kl are 0, its gradient is 0.  A logit of -inf (or the type's lowest value) has probability 0 and adds nothing to the KL.
  * _fwd writes out_loss (1 float), out_logp / out_kl (rows) and stats (rows x BG_POLICY_STATS + 1 floats on
  * an 8-byte boundary: what _bwd needs);  _bwd writes dlogits ([rows][V], dtype of logits) = *g_loss * dloss / dlogits.
+ * _fwd takes dlogits too (NULL: value only): rows that fit a workgroup's registers (V up to 106480 in bf16, 53240 in fp32) leave their
+ * gradient for g_loss = 1 there on the same reading of the logits, and *has_gradient (host) is 1.  Handed on to _bwd with that
+ * buffer it makes _bwd end at once when *g_loss is 1; any other value computes the gradient from the logits again.
  */
 #define BG_POLICY_STATS 8
 typedef struct {
@@ -547,9 +550,9 @@ typedef struct {
 } bg_policy_shape;
 int bg_policy_loss_fwd(const bg_policy_shape* sh, const void* logits, const void* ref_logits, const int64_t* ids, const float* old_logp,
                        const float* ref_logp, const float* advantages, const float* weights, const float* denominator,
-                       float* out_loss, float* out_logp, float* out_kl, float* stats, void* stream);
+                       float* out_loss, float* out_logp, float* out_kl, float* stats, void* dlogits, int* has_gradient, void* stream);
 int bg_policy_loss_bwd(const bg_policy_shape* sh, const void* logits, const void* ref_logits, const int64_t* ids, const float* stats,
-                       const float* g_loss, void* dlogits, void* stream);
+                       const float* g_loss, void* dlogits, int has_gradient, void* stream);
 
 #ifdef __cplusplus
 }

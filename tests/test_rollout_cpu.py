@@ -66,9 +66,9 @@ def test_policy_calls_refuse_before_any_launch():
             setattr(s, k, v)
         return s
     def fwd(s, logits=p, ref=None, ref_logp=None, stats=p):
-        return lib.bg_policy_loss_fwd(ctypes.byref(s), logits, ref, p, p, ref_logp, p, None, None, p, p, p, stats, None)
+        return lib.bg_policy_loss_fwd(ctypes.byref(s), logits, ref, p, p, ref_logp, p, None, None, p, p, p, stats, None, None, None)
     def bwd(s, logits=p, ref=None, stats=p):
-        return lib.bg_policy_loss_bwd(ctypes.byref(s), logits, ref, p, stats, p, p, None)
+        return lib.bg_policy_loss_bwd(ctypes.byref(s), logits, ref, p, stats, p, p, 0, None)
     for f in (fwd, bwd):
         for bad, word in ((dict(dtype=3), b"dtype 3"), (dict(rows=0), b"rows=0"), (dict(V=0), b"V=0"), (dict(x_stride=49), b"stride=49"),
                           (dict(temperature=0.0), b"temperature"), (dict(temperature=math.nan), b"temperature"), (dict(clip_low=-1.0), b"clip range"),
