@@ -190,8 +190,16 @@ def ptr(t):
     return None if t is None else c_vp(t.data_ptr())
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # the handle without a Stream object (a tenth of the time)
+
+
+def raw_stream(device_index):
+    """The current HIP stream of a device, as an integer."""
+    return _raw_stream(device_index) if _raw_stream is not None else torch.cuda.current_stream(device_index).cuda_stream
+
+
 def stream_ptr():
-    return c_vp(torch.cuda.current_stream().cuda_stream)
+    return c_vp(raw_stream(torch.cuda.current_device()))
 
 
 def dtype_code(t):

@@ -23,9 +23,10 @@ class QuantizedKVCache:
         self.bits, self.head_dim, self.capacity = int(bits), int(head_dim), int(capacity)
         tiles = -(-int(capacity) // ops.KV_TILE)
         self.data = torch.zeros((n_layers, batch, heads, tiles * tile), dtype=torch.uint8, device=device)
+        self._layers = [ops.KVCacheLayer(d, self.bits, self.head_dim, self.capacity) for d in self.data]
 
     def layer(self, i):
-        return ops.KVCacheLayer(self.data[i], self.bits, self.head_dim, self.capacity)
+        return self._layers[i]
 
     def __len__(self):
         return self.data.shape[0]

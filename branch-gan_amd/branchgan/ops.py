@@ -820,21 +820,21 @@ class KVCacheLayer:
         if data.dtype != torch.uint8 or data.dim() != 3 or data.stride(-1) != 1 or data.shape[-1] != -(-int(capacity) // KV_TILE) * tile:
             raise ValueError(f"cache data must be uint8 (batch, heads, {-(-int(capacity) // KV_TILE) * tile}) with a dense last dimension")
         self.data, self.bits, self.head_dim, self.capacity = data, int(bits), int(head_dim), int(capacity)
-
-    def _struct(self):
+        self.batch, self.heads, self.device = data.shape[0], data.shape[1], data.device
         sh = C.KvCache()
-        sh.bits, sh.B, sh.H, sh.Dh, sh.capacity = self.bits, self.data.shape[0], self.data.shape[1], self.head_dim, self.capacity
-        sh.c_sb, sh.c_sh = self.data.stride(0), self.data.stride(1)
-        return sh
+        sh.bits, sh.B, sh.H, sh.Dh, sh.capacity = self.bits, self.batch, self.heads, self.head_dim, self.capacity
+        sh.c_sb, sh.c_sh = data.stride(0), data.stride(1)
+        self._struct = ctypes.byref(sh)
 
 
-def _kv_rows(name, t, B, dev):
-    """start / counts of the cache calls: int32 (B,) on the cache's device, or None."""
+def _kv_rows(name, t, layer):
+    """start / counts of the cache calls: int32 (B,) on the cache's device, or None.  -> a dense tensor, its address"""
     if t is None:
-        return None
-    if t.dtype != torch.int32 or t.shape != (B,) or t.device != dev:
-        raise ValueError(f"{name} must be int32 of shape ({B},) on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.contiguous()
+        return None, None
+    if t.dtype != torch.int32 or t.shape != (layer.batch,) or t.device != layer.device:
+        raise ValueError(f"{name} must be int32 of shape ({layer.batch},) on {layer.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    t = t.contiguous()
+    return t, t.data_ptr()
 
 
 def _no_grad_wanted(what, *tensors):
@@ -842,45 +842,52 @@ def _no_grad_wanted(what, *tensors):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
 
 
+def _on_device(device, call):
+    """call(raw current stream of the device), made on that device."""
+    if torch.cuda.current_device() == device.index:
+        return call(C.raw_stream(device.index))
+    with torch.cuda.device(device):
+        return call(C.raw_stream(device.index))
+
+
 def kv_cache_append(layer, k, v, start=None, counts=None):
     """bg_kv_cache_append: quantises k, v (B, H, T, Dh) - fp32 or bf16, any strides - into the cache at positions start[b] .. .
     start int32 (B,) or None (= 0): tokens each sequence holds already; counts int32 (B,) or None (= T): how many of the T are
     the sequence's own, the rest is padding.  Positions outside the cache and padding are not written."""
     C.require_cuda(layer.data, k, v, start, counts)
-    B, H = layer.data.shape[:2]
-    if k.dim() != 4 or k.shape != v.shape or k.shape[0] != B or k.shape[1] != H or k.shape[3] != layer.head_dim:
-        raise ValueError(f"k and v must be ({B}, {H}, T, {layer.head_dim}), got {tuple(k.shape)} and {tuple(v.shape)}")
-    if k.dtype != v.dtype or k.device != layer.data.device or v.device != layer.data.device:
+    B, H, Dh = layer.batch, layer.heads, layer.head_dim
+    if k.dim() != 4 or k.shape != v.shape or k.shape[0] != B or k.shape[1] != H or k.shape[3] != Dh:
+        raise ValueError(f"k and v must be ({B}, {H}, T, {Dh}), got {tuple(k.shape)} and {tuple(v.shape)}")
+    if k.dtype != v.dtype or k.device != layer.device or v.device != layer.device:
         raise ValueError(f"k and v must share one dtype and the cache's device, got {k.dtype} on {k.device}, {v.dtype} on {v.device}")
     _no_grad_wanted("kv_cache_append", k, v)
-    start, counts = _kv_rows("start", start, B, k.device), _kv_rows("counts", counts, B, k.device)
+    (start, p_start), (counts, p_counts) = _kv_rows("start", start, layer), _kv_rows("counts", counts, layer)
     code, T = C.dtype_code(k), k.shape[2]
-    if T == 0 or B == 0 or H == 0:
+    if k.numel() == 0:
         return
     k, v = _unit_last(k), _unit_last(v)
-    sh = layer._struct()
-    with torch.cuda.device(k.device), _timed("kv_cache_append"):
-        C.check(C.lib().bg_kv_cache_append(ctypes.byref(sh), C.ptr(layer.data), C.ptr(k), C.ptr(v), code, T, *k.stride()[:3], *v.stride()[:3],
-                                           C.ptr(start), C.ptr(counts), C.stream_ptr()), "bg_kv_cache_append")
+    with _timed("kv_cache_append"):
+        C.check(_on_device(layer.device, lambda stream: C.lib().bg_kv_cache_append(
+            layer._struct, layer.data.data_ptr(), k.data_ptr(), v.data_ptr(), code, T, *k.stride()[:3], *v.stride()[:3], p_start, p_counts, stream)),
+            "bg_kv_cache_append")
 
 
 def kv_cache_read(layer, n, start=None, counts=None, dtype=torch.bfloat16):
     """bg_kv_cache_read -> k, v (B, H, n, Dh) in dtype: the values held at positions start[b] .. start[b] + n - 1; zeros for rows
     t >= counts[b] and outside the cache."""
     C.require_cuda(layer.data, start, counts)
-    B, H = layer.data.shape[:2]
-    dev = layer.data.device
-    start, counts = _kv_rows("start", start, B, dev), _kv_rows("counts", counts, B, dev)
-    if int(n) < 0:
+    (start, p_start), (counts, p_counts) = _kv_rows("start", start, layer), _kv_rows("counts", counts, layer)
+    n = int(n)
+    if n < 0:
         raise ValueError(f"kv_cache_read: n = {n}")
-    k, v = [torch.empty((B, H, int(n), layer.head_dim), dtype=dtype, device=dev) for _ in range(2)]
+    k = torch.empty((layer.batch, layer.heads, n, layer.head_dim), dtype=dtype, device=layer.device)
+    v = torch.empty_like(k)
     code = C.dtype_code(k)
     if k.numel() == 0:
         return k, v
-    sh = layer._struct()
-    with torch.cuda.device(dev), _timed("kv_cache_read"):
-        C.check(C.lib().bg_kv_cache_read(ctypes.byref(sh), C.ptr(layer.data), C.ptr(k), C.ptr(v), code, int(n), *k.stride()[:3], C.ptr(start),
-                                         C.ptr(counts), C.stream_ptr()), "bg_kv_cache_read")
+    with _timed("kv_cache_read"):
+        C.check(_on_device(layer.device, lambda stream: C.lib().bg_kv_cache_read(
+            layer._struct, layer.data.data_ptr(), k.data_ptr(), v.data_ptr(), code, n, *k.stride()[:3], p_start, p_counts, stream)), "bg_kv_cache_read")
     return k, v
 
 
@@ -890,84 +897,86 @@ def kv_cache_attention(q, layer, start=None, counts=None, scale=None, max_keys=N
     see nothing (padding) are zeros.  max_keys: the most keys any sequence holds after the append, if the host knows it (default:
     the capacity); keys past it are not read.  -> (out like q [a (B, T, Hq, Dh)-contiguous view], lse fp32 (B, Hq, T))."""
     C.require_cuda(q, layer.data, start, counts)
-    B, H = layer.data.shape[:2]
+    B, H = layer.batch, layer.heads
     if q.dim() != 4 or q.shape[0] != B or q.shape[3] != layer.head_dim or q.shape[1] == 0 or q.shape[1] % max(H, 1):
         raise ValueError(f"q must be ({B}, a multiple of {H} heads, T, {layer.head_dim}), got {tuple(q.shape)}")
-    if q.device != layer.data.device:
-        raise ValueError(f"q is on {q.device}, the cache on {layer.data.device}")
+    if q.device != layer.device:
+        raise ValueError(f"q is on {q.device}, the cache on {layer.device}")
     _no_grad_wanted("kv_cache_attention", q)
-    start, counts = _kv_rows("start", start, B, q.device), _kv_rows("counts", counts, B, q.device)
+    (start, p_start), (counts, p_counts) = _kv_rows("start", start, layer), _kv_rows("counts", counts, layer)
     max_keys = layer.capacity if max_keys is None else int(max_keys)
     if not 0 < max_keys <= layer.capacity:
         raise ValueError(f"max_keys {max_keys} is not in 1 .. {layer.capacity} (the capacity)")
     code, (_, Hq, T, Dh) = C.dtype_code(q), q.shape
-    out = torch.empty((B, T, Hq, Dh), dtype=q.dtype, device=q.device).permute(0, 2, 1, 3)
+    out = torch.empty((B, T, Hq, Dh), dtype=q.dtype, device=q.device).transpose(1, 2)
     lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device)
-    if out.numel() == 0:
+    if q.numel() == 0:
         return out, lse
     q = _unit_last(q)
     if scale is None:
         scale = 1.0 / math.sqrt(Dh)
-    sh = layer._struct()
-    with torch.cuda.device(q.device), _timed("kv_cache_attention"):
-        # a workspace of the call's own (the caching allocator's, so a captured graph keeps its own too): calls on several streams
-        # and graphs replayed side by side must not share one
-        ws_bytes = C.lib().bg_kv_cache_attn_workspace_bytes(ctypes.byref(sh), Hq, T, max_keys)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-        C.check(C.lib().bg_kv_cache_attn_fwd(ctypes.byref(sh), C.ptr(layer.data), C.ptr(q), code, Hq, T, *q.stride()[:3], C.ptr(start), C.ptr(counts),
-                                             max_keys, float(scale), C.ptr(out), *out.stride()[:3], C.ptr(lse), C.ptr(ws), ws_bytes,
-                                             C.stream_ptr()), "bg_kv_cache_attn_fwd")
+    lib = C.lib()
+    # a workspace of the call's own (the caching allocator's, so a captured graph keeps its own too): calls on several streams
+    # and graphs replayed side by side must not share one
+    ws_bytes = lib.bg_kv_cache_attn_workspace_bytes(layer._struct, Hq, T, max_keys)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    with _timed("kv_cache_attention"):
+        C.check(_on_device(layer.device, lambda stream: lib.bg_kv_cache_attn_fwd(
+            layer._struct, layer.data.data_ptr(), q.data_ptr(), code, Hq, T, *q.stride()[:3], p_start, p_counts, max_keys, float(scale),
+            out.data_ptr(), *out.stride()[:3], lse.data_ptr(), ws.data_ptr() if ws_bytes else None, ws_bytes, stream)), "bg_kv_cache_attn_fwd")
     return out, lse
 
 
 # ---------------------------------------------------------------------------------------------------
 # Clipped policy loss with a KL term
 # ---------------------------------------------------------------------------------------------------
+def _policy_launch(name, device, call):
+    with _timed(name):
+        C.check(_on_device(device, call), name)
+
+
 class _PolicyLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, ids, old_logp, advantages, weights, ref_logp, ref_logits, denominator, clip_low, clip_high, kl_coef, temperature):
+    def forward(ctx, logits, ids, rows_f32, ref_logits, denominator, shape):
         V = logits.shape[-1]
         dense = lambda t: t if t.stride(0) >= V or t.shape[0] == 1 else t.contiguous()       # expanded rows
-        x = dense(_rows_2d(logits.detach()))
-        y = dense(_rows_2d(ref_logits.detach())) if ref_logits is not None else None
+        x = dense(_rows_2d(logits))
+        y = dense(_rows_2d(ref_logits)) if ref_logits is not None else None
         rows, dev = x.shape[0], x.device
         ids = ids.reshape(rows).to(torch.int64).contiguous()
-        flat = lambda t: None if t is None else _f32c(t.detach().reshape(rows))
+        flat = [None if t is None else _f32c(t.reshape(rows)) for t in rows_f32]
         sh = C.PolicyShape()
         sh.dtype, sh.rows, sh.V = C.dtype_code(x), rows, V
         sh.x_stride, sh.ref_stride = max(x.stride(0), V), (max(y.stride(0), V) if y is not None else 0)
-        sh.temperature, sh.clip_low, sh.clip_high, sh.kl_coef = temperature, clip_low, clip_high, kl_coef
-        out = torch.empty(1, dtype=torch.float32, device=dev)
-        logp, kl = [torch.empty(rows, dtype=torch.float32, device=dev) for _ in range(2)]
+        sh.temperature, sh.clip_low, sh.clip_high, sh.kl_coef = shape
+        loss, lead = torch.empty((), dtype=torch.float32, device=dev), logits.shape[:-1]
+        logp, kl = torch.empty(lead, dtype=torch.float32, device=dev), torch.empty(lead, dtype=torch.float32, device=dev)
         stats = torch.empty(rows * C.POLICY_STATS + 1, dtype=torch.float32, device=dev)
-        args = [flat(t) for t in (old_logp, ref_logp, advantages, weights)] + [denominator]
         # the gradient for an incoming gradient of 1 comes out of the same reading of the logits; backward hands this buffer out
         dx = torch.empty((rows, V), dtype=x.dtype, device=dev) if ctx.needs_input_grad[0] else None
         has = C.c_i32(0)
-        with torch.cuda.device(dev), _timed(f"policy_loss_fwd[{rows}]"):
-            C.check(C.lib().bg_policy_loss_fwd(ctypes.byref(sh), C.ptr(x), C.ptr(y), C.ptr(ids), *[C.ptr(t) for t in args], C.ptr(out), C.ptr(logp),
-                                               C.ptr(kl), C.ptr(stats), C.ptr(dx), ctypes.byref(has), C.stream_ptr()), "bg_policy_loss_fwd")
-        ctx.save_for_backward(x, ids, stats, *(() if y is None else (y,)))
-        ctx.dx = dx if has.value else None
-        ctx.sh, ctx.in_shape = sh, logits.shape
-        loss, logp, kl = out.view(()), logp.view(logits.shape[:-1]), kl.view(logits.shape[:-1])
+        ptr = lambda t: None if t is None else t.data_ptr()
+        _policy_launch("bg_policy_loss_fwd", dev, lambda stream: C.lib().bg_policy_loss_fwd(
+            ctypes.byref(sh), x.data_ptr(), ptr(y), ids.data_ptr(), *[ptr(t) for t in flat], ptr(denominator), loss.data_ptr(), logp.data_ptr(),
+            kl.data_ptr(), stats.data_ptr(), ptr(dx), ctypes.byref(has), stream))
+        ctx.save_for_backward(x, ids, stats, y)
+        ctx.dx, ctx.sh, ctx.in_shape = dx if has.value else None, sh, logits.shape
         ctx.mark_non_differentiable(logp, kl)
         return loss, logp, kl
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_loss, _g_logp, _g_kl):
-        x, ids, stats = ctx.saved_tensors[:3]
-        y = ctx.saved_tensors[3] if len(ctx.saved_tensors) > 3 else None
-        g = g_loss.reshape(1).contiguous().float()
+        x, ids, stats, y = ctx.saved_tensors
+        g = g_loss if g_loss.dtype == torch.float32 else g_loss.float()
         dx, ctx.dx = ctx.dx, None                     # the buffer is handed out once: a second backward computes its own
         has = dx is not None
         if not has:
             dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        with torch.cuda.device(x.device), _timed(f"policy_loss_bwd[{x.shape[0]}]"):
-            C.check(C.lib().bg_policy_loss_bwd(ctypes.byref(ctx.sh), C.ptr(x), C.ptr(y), C.ptr(ids), C.ptr(stats), C.ptr(g), C.ptr(dx),
-                                               int(has), C.stream_ptr()), "bg_policy_loss_bwd")
-        return (dx.view(ctx.in_shape),) + (None,) * 11
+        _policy_launch("bg_policy_loss_bwd", x.device, lambda stream: C.lib().bg_policy_loss_bwd(
+            ctypes.byref(ctx.sh), x.data_ptr(), None if y is None else y.data_ptr(), ids.data_ptr(), stats.data_ptr(), g.data_ptr(), dx.data_ptr(),
+            int(has), stream))
+        return dx.view(ctx.in_shape), None, None, None, None, None
 
 
 def policy_loss(logits, ids, old_logp, advantages, weights=None, ref_logp=None, ref_logits=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0,
@@ -999,5 +1008,6 @@ def policy_loss(logits, ids, old_logp, advantages, weights=None, ref_logp=None, 
             denominator = _f32c(denominator.detach().reshape(1))
         else:
             denominator = torch.full((1,), float(denominator), dtype=torch.float32, device=logits.device)
-    return _PolicyLoss.apply(logits, ids, old_logp, advantages, weights, ref_logp, ref_logits, denominator, float(clip_low), float(clip_high),
-                             float(kl_coef), float(temperature))
+    rows_f32 = tuple(None if t is None else t.detach() for t in (old_logp, ref_logp, advantages, weights))
+    return _PolicyLoss.apply(logits, ids, rows_f32, None if ref_logits is None else ref_logits.detach(), denominator,
+                             (float(temperature), float(clip_low), float(clip_high), float(kl_coef)))
