@@ -962,11 +962,14 @@ class _PolicyLoss(torch.autograd.Function):
         ctx.save_for_backward(x, ids, stats, y)
         ctx.dx, ctx.sh, ctx.in_shape = dx if has.value else None, sh, logits.shape
         ctx.mark_non_differentiable(logp, kl)
+        ctx.set_materialize_grads(False)              # no zeros for the outputs without a gradient
         return loss, logp, kl
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_loss, _g_logp, _g_kl):
+        if g_loss is None:
+            return (None,) * 6
         x, ids, stats, y = ctx.saved_tensors
         g = g_loss if g_loss.dtype == torch.float32 else g_loss.float()
         dx, ctx.dx = ctx.dx, None                     # the buffer is handed out once: a second backward computes its own

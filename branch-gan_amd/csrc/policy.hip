@@ -26,6 +26,8 @@ template <> struct Vec<bf16_t> {
   typedef bf16x8 type;
 };
 
+constexpr int64_t NORM_ROWS = 1024;      // up to here the workgroups of short rows sum the weights themselves (12 KB from L2): a launch less
+
 struct PolicyArgs {
   const void* logits;
   const void* ref;
@@ -94,6 +96,8 @@ template <typename V> __device__ __forceinline__ void forget(V& v) {
 struct RowResult {          // what the gradient of a row needs
   float m, inv_s, slope, w_kl, off, my;
 };
+
+__device__ __forceinline__ float inverse(double n) { return n == 0.0 ? 0.f : (float)(1.0 / n); }
 
 __device__ __forceinline__ float row_weight(const PolicyArgs& a, int64_t row) {
   const int64_t id = a.ids[row];
@@ -175,36 +179,37 @@ __device__ __forceinline__ float grad_of(float p, float diff, float slope, float
   return d;
 }
 
-// 1 / N, N = sum of the weights that count (or the denominator) -> stats[rows * BG_POLICY_STATS]
-__global__ __launch_bounds__(1024) void policy_norm_kernel(PolicyArgs a, const float* denominator) {
+// N = the sum of the weights that count; 1 / N -> stats[rows * BG_POLICY_STATS], before the rows' gradients need it (many rows)
+__global__ __launch_bounds__(1024) void policy_norm_kernel(PolicyArgs a) {
   __shared__ double red[16];
   double n = 0.0;
-  if (denominator) {
-    n = denominator[0];
-  } else {
-    for (int64_t r = threadIdx.x; r < a.rows; r += 1024) n += row_weight(a, r);
-    n = wave_sum(n);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = n;
-    __syncthreads();
-    n = 0.0;
-    for (int i = 0; i < 16; ++i) n += red[i];
-  }
-  if (threadIdx.x == 0) a.stats[a.rows * BG_POLICY_STATS] = n == 0.0 ? 0.f : (float)(1.0 / n);
+  for (int64_t r = threadIdx.x; r < a.rows; r += 1024) n += row_weight(a, r);
+  n = wave_sum(n);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = n;
+  __syncthreads();
+  n = 0.0;
+  for (int i = 0; i < 16; ++i) n += red[i];
+  if (threadIdx.x == 0) a.stats[a.rows * BG_POLICY_STATS] = inverse(n);
 }
 
-// loss = sum of the rows' terms / N, in a fixed order, fp64
-__global__ __launch_bounds__(1024) void policy_total_kernel(PolicyArgs a, float* out_loss) {
-  __shared__ double red[16];
-  double sum = 0.0;
-  for (int64_t r = threadIdx.x; r < a.rows; r += 1024) sum += *(const double*)(a.stats + r * BG_POLICY_STATS + 6);
+// loss = sum of the rows' terms / N, in a fixed order, fp64; leaves 1 / N for the backward call
+__global__ __launch_bounds__(1024) void policy_total_kernel(PolicyArgs a, const float* denominator, float* out_loss) {
+  __shared__ double red[2][16];
+  double sum = 0.0, n = 0.0;
+  for (int64_t r = threadIdx.x; r < a.rows; r += 1024) {
+    sum += *(const double*)(a.stats + r * BG_POLICY_STATS + 6);
+    if (!denominator) n += row_weight(a, r);
+  }
   sum = wave_sum(sum);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
+  n = wave_sum(n);
+  if ((threadIdx.x & 63) == 0) { red[0][threadIdx.x >> 6] = sum; red[1][threadIdx.x >> 6] = n; }
   __syncthreads();
   if (threadIdx.x == 0) {
-    sum = 0.0;
-    for (int i = 0; i < 16; ++i) sum += red[i];
-    const float inv_n = a.stats[a.rows * BG_POLICY_STATS];
-    out_loss[0] = inv_n == 0.f ? 0.f : (float)(sum * inv_n);
+    sum = n = 0.0;
+    for (int i = 0; i < 16; ++i) { sum += red[0][i]; n += red[1][i]; }
+    if (denominator) n = denominator[0];
+    a.stats[a.rows * BG_POLICY_STATS] = inverse(n);
+    out_loss[0] = n == 0.0 ? 0.f : (float)(sum / n);
   }
 }
 
@@ -213,12 +218,13 @@ __global__ __launch_bounds__(1024) void policy_total_kernel(PolicyArgs a, float*
 // way together; the fewer than 2 N elements before and after it go one each to the first threads.  Sums: fp32 per thread, fp64
 // across them.
 template <typename T, bool REF, int NT, int NV>
-__global__ __launch_bounds__(NT, 4) void policy_row_kernel(PolicyArgs a, T* dlogits) {
+__global__ __launch_bounds__(NT, 4) void policy_row_kernel(PolicyArgs a, const float* denominator, T* dlogits) {
   constexpr int N = Vec<T>::N, NW = NT / 64;
   typedef typename Vec<T>::type V_t;
   __shared__ float red_m[2][NW];
-  __shared__ double red[NW][3];
+  __shared__ double red[NW][4];
   __shared__ RowResult sh_row;
+  __shared__ float sh_inv_n;
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x;
   const T* x = (const T*)a.logits + row * a.x_stride;
@@ -247,7 +253,9 @@ __global__ __launch_bounds__(NT, 4) void policy_row_kernel(PolicyArgs a, T* dlog
   const float ex = has_extra ? to_f32(x[extra]) : -INFINITY, ey = REF && has_extra ? to_f32(y[extra]) : -INFINITY;
   const int id = (int)a.ids[row];
   const float x_id = to_f32(x[id]);
-  const float inv_n = a.stats[a.rows * BG_POLICY_STATS];
+  double n64 = 0.0;
+  if (NT == 256 && a.rows <= NORM_ROWS && !denominator)
+    for (int64_t r = tid; r < a.rows; r += NT) n64 += row_weight(a, r);
   V_t none;
 #pragma unroll
   for (int j = 0; j < N; ++j) none[j] = from_f32<T>(-INFINITY);
@@ -288,17 +296,20 @@ __global__ __launch_bounds__(NT, 4) void policy_row_kernel(PolicyArgs a, T* dlog
     for (int j = 0; j < N; ++j) add((float)vx[k][j], REF ? (float)vy[REF ? k : 0][j] : 0.f);
   }
   const double s64 = wave_sum((double)s), t64 = REF ? wave_sum((double)t) : 0.0, sy64 = REF ? wave_sum((double)sy) : 0.0;
-  if ((tid & 63) == 0) { red[tid >> 6][0] = s64; red[tid >> 6][1] = t64; red[tid >> 6][2] = sy64; }
+  if constexpr (NT == 256) n64 = wave_sum(n64);
+  if ((tid & 63) == 0) { red[tid >> 6][0] = s64; red[tid >> 6][1] = t64; red[tid >> 6][2] = sy64; red[tid >> 6][3] = n64; }
   __syncthreads();
   if (tid == 0) {
-    double S = 0.0, Tt = 0.0, Sy = 0.0;
-    for (int i = 0; i < NW; ++i) { S += red[i][0]; Tt += red[i][1]; Sy += red[i][2]; }
+    double S = 0.0, Tt = 0.0, Sy = 0.0, Nw = 0.0;
+    for (int i = 0; i < NW; ++i) { S += red[i][0]; Tt += red[i][1]; Sy += red[i][2]; Nw += red[i][3]; }
+    sh_inv_n = denominator ? inverse(denominator[0])
+               : NT == 256 && a.rows <= NORM_ROWS ? inverse(Nw) : a.stats[a.rows * BG_POLICY_STATS];
     sh_row = finish_row<REF>(a, row, w, ms, S, mys, Sy, Tt, x_id);
   }
   if (!dlogits) return;
   __syncthreads();
   const RowResult r = sh_row;
-  const float f = inv_n * a.inv_t32, slope = f * r.slope, w_kl = f * r.w_kl, off = r.off;
+  const float f = sh_inv_n * a.inv_t32, slope = f * r.slope, w_kl = f * r.w_kl, off = r.off;
   auto grad = [&](float v, float u) __attribute__((always_inline)) {
     const float dv = v - ms, p = policy_exp(dv, a.c_hi, a.c_lo) * r.inv_s;
     return grad_of<REF>(p, REF ? dv - (u - mys) : 0.f, slope, w_kl, off, a.inv_t32);
@@ -452,7 +463,7 @@ static PolicyArgs policy_args(const bg_policy_shape* sh, const void* logits, con
 
 // Rows of at most NT * NV vectors.  Few threads for short rows; for the usual vocabularies
 // 512, so that two rows share a CU and one's loads cover the other's exponentials.
-template <typename T, bool REF> static bool policy_row_launch(const PolicyArgs& a, T* dlogits, hipStream_t st) {
+template <typename T, bool REF> static bool policy_row_launch(const PolicyArgs& a, const float* denominator, T* dlogits, hipStream_t st) {
   const int64_t nvec = a.V / Vec<T>::N + 1;
   if (a.V < 2 * Vec<T>::N) return false;
   // reference or gradient rows that lie elsewhere on the 16-byte grid than the logits': the streaming kernels
@@ -462,10 +473,10 @@ template <typename T, bool REF> static bool policy_row_launch(const PolicyArgs& 
   if (REF && !same_grid(a.ref, a.ref_stride)) return false;
   if (dlogits && !same_grid(dlogits, a.V)) return false;
   const dim3 grid((unsigned)a.rows);
-  if (nvec <= 256 * 2) hipLaunchKernelGGL((policy_row_kernel<T, REF, 256, 2>), grid, dim3(256), 0, st, a, dlogits);
-  else if (nvec <= 256 * 8) hipLaunchKernelGGL((policy_row_kernel<T, REF, 256, 8>), grid, dim3(256), 0, st, a, dlogits);
-  else if (nvec <= 512 * 13) hipLaunchKernelGGL((policy_row_kernel<T, REF, 512, 13>), grid, dim3(512), 0, st, a, dlogits);
-  else if (nvec <= 1024 * 13) hipLaunchKernelGGL((policy_row_kernel<T, REF, 1024, 13>), grid, dim3(1024), 0, st, a, dlogits);
+  if (nvec <= 256 * 2) hipLaunchKernelGGL((policy_row_kernel<T, REF, 256, 2>), grid, dim3(256), 0, st, a, denominator, dlogits);
+  else if (nvec <= 256 * 8) hipLaunchKernelGGL((policy_row_kernel<T, REF, 256, 8>), grid, dim3(256), 0, st, a, denominator, dlogits);
+  else if (nvec <= 512 * 13) hipLaunchKernelGGL((policy_row_kernel<T, REF, 512, 13>), grid, dim3(512), 0, st, a, denominator, dlogits);
+  else if (nvec <= 1024 * 13) hipLaunchKernelGGL((policy_row_kernel<T, REF, 1024, 13>), grid, dim3(1024), 0, st, a, denominator, dlogits);
   else return false;
   return true;
 }
@@ -476,8 +487,9 @@ static void policy_grad_launch(const PolicyArgs& a, const float* g_loss, T* dlog
   hipLaunchKernelGGL((policy_grad_kernel<T, REF>), dim3((unsigned)(a.rows < most ? a.rows : most)), dim3(PT), 0, st, a, g_loss, dlogits, unless_one);
 }
 
-template <typename T, bool REF> static int policy_fwd(const PolicyArgs& a, T* dlogits, hipStream_t st) {
-  if (policy_row_launch<T, REF>(a, dlogits, st)) return dlogits ? 1 : 0;
+template <typename T, bool REF> static int policy_fwd(const PolicyArgs& a, const float* denominator, T* dlogits, hipStream_t st) {
+  if (dlogits && !denominator && (a.rows > NORM_ROWS || a.V / Vec<T>::N + 1 > 256 * 8)) hipLaunchKernelGGL(policy_norm_kernel, dim3(1), dim3(1024), 0, st, a);
+  if (policy_row_launch<T, REF>(a, denominator, dlogits, st)) return dlogits ? 1 : 0;
   hipLaunchKernelGGL((policy_rows_kernel<T, REF>), dim3((unsigned)a.rows), dim3(PT), 0, st, a);
   return 0;
 }
@@ -494,12 +506,13 @@ extern "C" int bg_policy_loss_fwd(const bg_policy_shape* sh, const void* logits,
   a.old_logp = old_logp; a.ref_logp = ref_logp; a.adv = advantages; a.weights = weights;
   a.out_logp = out_logp; a.out_kl = out_kl;
   hipStream_t st = (hipStream_t)stream;
-  hipLaunchKernelGGL(policy_norm_kernel, dim3(1), dim3(1024), 0, st, a, denominator);
   int wrote;
-  if (sh->dtype == BG_F32) wrote = ref_logits ? policy_fwd<float, true>(a, (float*)dlogits, st) : policy_fwd<float, false>(a, (float*)dlogits, st);
-  else wrote = ref_logits ? policy_fwd<bf16_t, true>(a, (bf16_t*)dlogits, st) : policy_fwd<bf16_t, false>(a, (bf16_t*)dlogits, st);
+  if (sh->dtype == BG_F32)
+    wrote = ref_logits ? policy_fwd<float, true>(a, denominator, (float*)dlogits, st) : policy_fwd<float, false>(a, denominator, (float*)dlogits, st);
+  else
+    wrote = ref_logits ? policy_fwd<bf16_t, true>(a, denominator, (bf16_t*)dlogits, st) : policy_fwd<bf16_t, false>(a, denominator, (bf16_t*)dlogits, st);
   if (has_gradient) *has_gradient = wrote;
-  hipLaunchKernelGGL(policy_total_kernel, dim3(1), dim3(1024), 0, st, a, out_loss);
+  hipLaunchKernelGGL(policy_total_kernel, dim3(1), dim3(1024), 0, st, a, denominator, out_loss);
   BG_CHECK_LAUNCH("bg_policy_loss_fwd");
   return BG_OK;
 }
