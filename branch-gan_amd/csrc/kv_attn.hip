@@ -30,8 +30,11 @@ constexpr int KW = 4;                       // waves per workgroup
 constexpr int KV_TURN = 4 * KV_TILE;        // keys a wave takes per turn
 
 // Turn of a wave in steps of TS rows of four keys per tile, so that the codes in flight fit the registers beside the accumulators
-template <int BITS, int DH, bool PACKED> constexpr int kv_steps() {
-  return PACKED ? (DH * BITS <= 512 ? 8 : DH * BITS <= 1024 ? 4 : 2) : (DH * BITS <= 512 ? 4 : 2);
+template <typename T, int BITS, int DH, bool PACKED> constexpr int kv_steps() {
+  if (!PACKED) return DH * BITS <= 512 ? 4 : 2;
+  if (DH * BITS <= 256) return 4;
+  if (DH * BITS <= 512) return sizeof(T) == 4 && DH == 128 ? 4 : 8;
+  return DH * BITS <= 1024 && !(sizeof(T) == 4 && DH == 256) ? 4 : 2;
 }
 
 struct KvAttnArgs {
@@ -69,13 +72,18 @@ union Frag {
 // 8 codes -> 8 bf16 numbers code + OFFT.  4 bits: the nibble as bits 3..6 of a bf16 in [16, 32) is 16 + stored code; 8 bits: converted
 // (a conversion that takes its byte from the word, and half a pack).
 template <int BITS> constexpr float kv_offset() { return BITS == 4 ? 24.f : 0.f; }
-template <int BITS> __device__ __forceinline__ bf16x8 unpack_codes(const uint32_t* w) {
+// The two constants sit in a vector and a scalar register: as literals they would make the mask-or two instructions.
+struct Nibbles {
+  uint32_t mask, base;
+  __device__ __forceinline__ Nibbles() : mask(0x00780078u), base(0x41804180u) { asm volatile("" : "+v"(mask), "+s"(base)); }
+};
+template <int BITS> __device__ __forceinline__ bf16x8 unpack_codes(const uint32_t* w, const Nibbles& nb) {
   Frag f;
   if constexpr (BITS == 4) {
-    f.u[0] = ((w[0] << 3) & 0x00780078u) | 0x41804180u;
-    f.u[1] = ((w[0] >> 1) & 0x00780078u) | 0x41804180u;
-    f.u[2] = ((w[0] >> 5) & 0x00780078u) | 0x41804180u;
-    f.u[3] = ((w[0] >> 9) & 0x00780078u) | 0x41804180u;
+    f.u[0] = ((w[0] << 3) & nb.mask) | nb.base;
+    f.u[1] = ((w[0] >> 1) & nb.mask) | nb.base;
+    f.u[2] = ((w[0] >> 5) & nb.mask) | nb.base;
+    f.u[3] = ((w[0] >> 9) & nb.mask) | nb.base;
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) f.v[i] = (bf16_t)(float)(int8_t)(w[i / 4] >> (8 * (i % 4)));
@@ -83,23 +91,33 @@ template <int BITS> __device__ __forceinline__ bf16x8 unpack_codes(const uint32_
   return f.v;
 }
 
+__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+
 // x -> N bf16 pieces that add up to it (8 bits each)
 template <int N> __device__ __forceinline__ void split_bf16(const float (&x)[8], bf16x8 (&piece)[N]) {
-  float rest[8];
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 #pragma unroll
-  for (int e = 0; e < 8; ++e) rest[e] = x[e];
+  for (int h = 0; h < 4; ++h) {
+    f32x2 rest = {x[2 * h], x[2 * h + 1]};
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      piece[i][e] = (bf16_t)rest[e];
-      if (i + 1 < N) rest[e] -= (float)piece[i][e];
+    for (int i = 0; i < N; ++i) {
+      const bf16x2 p = __builtin_convertvector(rest, bf16x2);
+      piece[i][2 * h] = p[0];
+      piece[i][2 * h + 1] = p[1];
+      if (i + 1 < N) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, p);
+        rest[0] -= bf16_lo(u);
+        rest[1] -= bf16_hi(u);
+      }
     }
   }
 }
 
 template <int CTRL> __device__ __forceinline__ float dpp_add(float x) {
-  return x + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xF, 0xF, true));
+#pragma clang fp contract(off)          // a fused multiply-add would need the moved value in a register of its own
+  return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, true));
 }
 template <int NG> __device__ __forceinline__ float group_sum(float x) {      // over NG adjacent lanes
   if constexpr (NG >= 2) x = dpp_add<0xB1>(x);                              // quad_perm 1,0,3,2
@@ -108,89 +126,47 @@ template <int NG> __device__ __forceinline__ float group_sum(float x) {      // 
   return x;
 }
 
-__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
-
-// waves per SIMD the kernel is built for: two, but one (512 registers) where two would spill
+// Waves per SIMD the kernel is built for: four for small heads, whose turns are short and bound by vector work as much as by
+// memory; else two; one (512 registers) where two would spill.
 template <typename T, int BITS, int DH, bool PACKED> constexpr int kv_waves() {
-  return DH == 256 && (!PACKED || sizeof(T) == 4) ? 1 : DH == 128 && BITS == 4 && (!PACKED || sizeof(T) == 4) ? 1 : 2;
+  if (PACKED) return DH * BITS <= 256 ? (sizeof(T) == 4 && DH == 64 ? 3 : 4) : sizeof(T) == 4 && DH * BITS > 1024 ? 1 : 2;
+  return DH == 256 || (DH == 128 && BITS == 4) ? 1 : 2;
 }
 
 template <typename T, int BITS, int DH, bool PACKED>
 __global__ __launch_bounds__(64 * KW, (kv_waves<T, BITS, DH, PACKED>())) void kv_attn_kernel(KvAttnArgs a) {
   using L = KvTile<BITS, DH>;
-  constexpr int NG = L::NG, TS = kv_steps<BITS, DH, PACKED>(), NO = TS / 2, CB = DH / 16;
+  constexpr int NG = L::NG, TS = kv_steps<T, BITS, DH, PACKED>(), NO = TS / 2, CB = DH / 16;
   constexpr int ROWS = PACKED ? 16 / NG : 16, GL = PACKED ? 1 : NG;         // rows per tile; groups whose scales a lane needs
   constexpr int NQ = sizeof(T) == 4 ? 3 : 1, NP = sizeof(T) == 4 ? 3 : 2;   // bf16 pieces of queries / probabilities
   constexpr float OFFT = kv_offset<BITS>();
+  constexpr bool OWN_Q = PACKED && NG * NQ > 4;     // keep a lane's one group only, and the zeros of the others as a select per use
+  constexpr bool LDS_Q = !PACKED && NG * NQ > 8;    // the pieces of long fp32 rows live in LDS
+  constexpr int NQF = OWN_Q || LDS_Q ? 1 : NG;
   constexpr int KWORDS = NG * L::WORD / 4, VWORDS = NO * L::WORD / 4;
   __shared__ float sh_o[KW][ROWS][DH];
   __shared__ float sh_m[KW][16], sh_l[KW][16];
+  __shared__ bf16x8 sh_q[LDS_Q ? NG : 1][NQ][LDS_Q ? 64 : 1];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, j = lane >> 4;
-  const int64_t blk = blockIdx.x;
-  const int split = (int)(blk % a.splits), rt = (int)(blk / a.splits % a.row_tiles);
-  const int64_t bh = blk / a.splits / a.row_tiles;
-  const int b = (int)(bh / a.kv.H), h = (int)(bh % a.kv.H);
+  const int b = blockIdx.z, h = blockIdx.y;
+  const int rt = (int)(blockIdx.x / (uint32_t)a.splits), split = (int)blockIdx.x - rt * a.splits;
   const int R = a.kv.T * a.G, row0 = rt * ROWS;                             // rows (t, g) of this cache head: rho = t G + g
-
-  // this lane's column: its row, and what that row sees
-  const int rho = row0 + (PACKED ? n / NG : n), my_g = PACKED ? n % NG : 0;
-  const bool real = rho < R;
-  const int vis = real ? min(a.kv.visible(b, rho / a.G), a.max_keys) : 0x7FFFFFFF;
-  int n_max = real ? vis : 0, n_min = vis;
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) {
-    n_max = max(n_max, __shfl_xor(n_max, o));
-    n_min = min(n_min, __shfl_xor(n_min, o));
-  }
-  n_max = __builtin_amdgcn_readfirstlane(n_max);
-  n_min = __builtin_amdgcn_readfirstlane(n_min);
-
-  // queries: B operand of step g = channels 32 g + 8 j + 0..7 of column n's row
-  bf16x8 qf[NG][NQ];
-  float q0[GL];                                                              // what the offset of the codes adds to a score
-  {
-    const T* q = (const T*)a.q + b * a.q_sb + (int64_t)(h * a.G + rho % a.G) * a.q_sh + (int64_t)(rho / a.G) * a.q_st;
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      float x[8], sum = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float v = real && (!PACKED || g == my_g) ? to_f32(q[32 * g + 8 * j + e]) : 0.f;
-        x[e] = a.negate ? -v : v;
-        sum += x[e];
-      }
-      split_bf16<NQ>(x, qf[g]);
-      sum += __shfl_xor(sum, 16);
-      sum += __shfl_xor(sum, 32);
-      if constexpr (PACKED) q0[0] = g == 0 ? sum : q0[0] + sum;              // one group is not zero
-      else q0[g] = sum;
-    }
-#pragma unroll
-    for (int g = 0; g < GL; ++g) q0[g] *= -OFFT;
-  }
-
-  f32x4 acc[CB], off = {0.f, 0.f, 0.f, 0.f};                                 // PACKED: one offset sum; else one per group
-  f32x4 offg[PACKED ? 1 : NG];
-#pragma unroll
-  for (int c = 0; c < CB; ++c) acc[c] = off;
-#pragma unroll
-  for (int g = 0; g < (PACKED ? 1 : NG); ++g) offg[g] = off;
-  float mc = -INFINITY, l = 0.f;                                             // maximum in log2 units, this lane's share of the sum
-  Frag ones;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) ones.v[i] = (bf16_t)OFFT;
-
   const uint8_t* base = a.kv.data + b * a.kv.c_sb + h * a.kv.c_sh;
   const int last_tile = (a.kv.capacity - 1) / KV_TILE;
-  const int turns = (n_max + KV_TURN - 1) / KV_TURN;
-  const int t_begin = (int)((int64_t)turns * split / a.splits), t_end = (int)((int64_t)turns * (split + 1) / a.splits);
   constexpr int SUB = 8 / TS;                                                // steps of a turn
-  const int my_turns = t_end - t_begin > wave ? (t_end - t_begin - wave + KW - 1) / KW : 0;
-  const int steps = my_turns * SUB;
+
+  // this lane's column: its row
+  const int rho = row0 + (PACKED ? n / NG : n), my_g = PACKED ? n % NG : 0;
+  const bool real = rho < R;
+  int t_row = 0, g_row = rho;                                                // rho = t_row G + g_row
+  if (a.kv.T > 1) {
+    t_row = (int)((uint32_t)rho / (uint32_t)a.G);
+    g_row = rho - t_row * a.G;
+  }
 
   uint32_t kw[TS][KWORDS], ks[GL][TS * 2], vw[CB][VWORDS], vs[GL][TS * 2];
+  int t_begin = 0;
   auto key_base = [&](int step, int tile_in_turn) __attribute__((always_inline)) -> const uint8_t* {
     const int tile = (t_begin + wave + KW * (step / SUB)) * 4 + tile_in_turn;
     return base + (int64_t)min(tile, last_tile) * L::BYTES;
@@ -212,36 +188,108 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<T, BITS, DH, PACKED>())) void kv
 #pragma unroll
     for (int g = 0; g < GL; ++g) load_words<TS * 2>(vt + L::VS + s * TS * 8 + (PACKED ? my_g : g) * KV_TILE * 2, vs[g]);
   };
+  // with the whole key range in this workgroup the first turn's place is known before the sequence's length is
+  if (a.splits == 1) load_k(0);
 
-  if (steps > 0) load_k(0);
+  // queries: B operand of step g = channels 32 g + 8 j + 0..7 of column n's row
+  bf16x8 qf[NQF][NQ];
+  float q0[GL];                                                              // what the offset of the codes adds to a score
+  {
+    const T* q = (const T*)a.q + b * a.q_sb + (int64_t)(h * a.G + g_row) * a.q_sh + (int64_t)t_row * a.q_st + 8 * j;
+#pragma unroll
+    for (int g = 0; g < (PACKED ? 1 : NG); ++g) {
+      float x[8], sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float v = real ? to_f32(q[32 * (PACKED ? my_g : g) + e]) : 0.f;
+        x[e] = a.negate ? -v : v;
+        sum += x[e];
+      }
+      bf16x8 piece[NQ];
+      split_bf16<NQ>(x, piece);
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+        if constexpr (LDS_Q) sh_q[g][i][lane] = piece[i];                    // the four waves write the same values
+        else qf[g][i] = piece[i];
+      }
+      sum += __shfl_xor(sum, 16);
+      sum += __shfl_xor(sum, 32);
+      q0[g] = -OFFT * sum;
+    }
+    if constexpr (PACKED && !OWN_Q) {
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+        const Frag own = {.v = qf[0][i]};
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          Frag f;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) f.u[w] = g == my_g ? own.u[w] : 0u;
+          qf[g][i] = f.v;
+        }
+      }
+    }
+  }
+  if constexpr (LDS_Q) __syncthreads();
+  auto query = [&](int g, int i) __attribute__((always_inline)) -> bf16x8 {
+    if constexpr (LDS_Q) return sh_q[g][i][lane];
+    if constexpr (!OWN_Q) return qf[g][i];
+    const Frag own = {.v = qf[0][i]};
+    Frag f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) f.u[w] = g == my_g ? own.u[w] : 0u;
+    return f.v;
+  };
+
+  // what the rows of this tile see: all of them at least n_min keys, none more than n_max
+  const int count = a.kv.count(b), t_lo = a.kv.T > 1 ? row0 / a.G : 0, t_hi = a.kv.T > 1 ? (min(row0 + ROWS, R) - 1) / a.G : 0;
+  const int n_max = t_lo < count ? min(a.kv.visible(b, min(t_hi, count - 1)), a.max_keys) : 0;
+  const int n_min = t_hi < count ? min(a.kv.visible(b, t_lo), a.max_keys) : 0;
+  const int vis = real ? min(a.kv.visible(b, t_row), a.max_keys) : 0x7FFFFFFF;
+
+  f32x4 acc[CB], off = {0.f, 0.f, 0.f, 0.f};                                 // PACKED: one offset sum; else one per group
+  f32x4 offg[PACKED ? 1 : NG];
+#pragma unroll
+  for (int c = 0; c < CB; ++c) acc[c] = off;
+#pragma unroll
+  for (int g = 0; g < (PACKED ? 1 : NG); ++g) offg[g] = off;
+  float mc = -INFINITY, l = 0.f;                                             // maximum in log2 units, this lane's share of the sum
+  Frag ones;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ones.v[i] = (bf16_t)OFFT;
+
+  const Nibbles nb;
+  const int turns = (n_max + KV_TURN - 1) / KV_TURN;
+  int t_end = turns;
+  if (a.splits > 1) {
+    const int each = (int)((uint32_t)turns / (uint32_t)a.splits), more = turns - each * a.splits;      // the first `more` splits take one more
+    t_begin = split * each + min(split, more);
+    t_end = t_begin + each + (split < more ? 1 : 0);
+  }
+  const int my_turns = t_end - t_begin > wave ? (t_end - t_begin - wave + KW - 1) / KW : 0;
+  const int steps = my_turns * SUB;
+  if (a.splits > 1 && steps > 0) load_k(0);
   for (int step = 0; step < steps; ++step) {
     load_v(step);
     // scores
-    float sc[TS][4];
+    f32x4 sc[TS];
 #pragma unroll
-    for (int t = 0; t < TS; ++t) {
-      if constexpr (PACKED) {
-        f32x4 d = {q0[0], q0[0], q0[0], q0[0]};
+    for (int t = 0; t < TS; ++t) sc[t] = PACKED ? f32x4{q0[0], q0[0], q0[0], q0[0]} : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          const bf16x8 kf = unpack_codes<BITS>(&kw[t][g * L::WORD / 4]);
+    for (int g = 0; g < NG; ++g) {
+      bf16x8 qg[NQ];
 #pragma unroll
-          for (int i = 0; i < NQ; ++i) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[g][i], d, 0, 0, 0);
-        }
+      for (int i = 0; i < NQ; ++i) qg[i] = query(g, i);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float k_scale = r & 1 ? bf16_hi(ks[0][2 * t + r / 2]) : bf16_lo(ks[0][2 * t + r / 2]);
-          sc[t][r] = group_sum<NG>(d[r] * k_scale);
-        }
-      } else {
+      for (int t = 0; t < TS; ++t) {
+        const bf16x8 kf = unpack_codes<BITS>(&kw[t][g * L::WORD / 4], nb);
+        if constexpr (PACKED) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sc[t][r] = 0.f;
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          const bf16x8 kf = unpack_codes<BITS>(&kw[t][g * L::WORD / 4]);
+          for (int i = 0; i < NQ; ++i) sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qg[i], sc[t], 0, 0, 0);
+        } else {
           f32x4 d = {q0[g], q0[g], q0[g], q0[g]};
 #pragma unroll
-          for (int i = 0; i < NQ; ++i) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[g][i], d, 0, 0, 0);
+          for (int i = 0; i < NQ; ++i) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qg[i], d, 0, 0, 0);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const float k_scale = r & 1 ? bf16_hi(ks[g][2 * t + r / 2]) : bf16_lo(ks[g][2 * t + r / 2]);
@@ -250,6 +298,24 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<T, BITS, DH, PACKED>())) void kv
         }
       }
     }
+    if constexpr (PACKED) {
+#pragma unroll
+      for (int t = 0; t < TS; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float k_scale = r & 1 ? bf16_hi(ks[0][2 * t + r / 2]) : bf16_lo(ks[0][2 * t + r / 2]);
+          sc[t][r] = group_sum<NG>(sc[t][r] * k_scale);
+        }
+    }
+    // (the sums stay in this block: moved behind the branch below, an add and the lane exchange that feeds it are two instructions)
+#pragma unroll
+    for (int t = 0; t < TS; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float v = sc[t][r];
+        asm volatile("" : "+v"(v));
+        sc[t][r] = v;
+      }
     if (step + 1 < steps) load_k(step + 1);
     // keys of this lane: key0 + 4 t + r
     const int turn0 = (t_begin + wave + KW * (step / SUB)) * KV_TURN;
@@ -327,7 +393,7 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<T, BITS, DH, PACKED>())) void kv
       }
 #pragma unroll
       for (int c = 0; c < CB; ++c) {
-        const bf16x8 vf = unpack_codes<BITS>(&vw[c][o * L::WORD / 4]);
+        const bf16x8 vf = unpack_codes<BITS>(&vw[c][o * L::WORD / 4], nb);
 #pragma unroll
         for (int i = 0; i < NP; ++i) acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf[PACKED ? 0 : c / 2][i], vf, acc[c], 0, 0, 0);
       }
@@ -367,7 +433,7 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<T, BITS, DH, PACKED>())) void kv
       ((T*)a.out)[b * a.o_sb + hq * a.o_sh + t * a.o_st + ch] = from_f32<T>(any ? o / S : 0.f);
       if (a.lse && ch == 0) a.lse[((int64_t)b * a.kv.H * a.G + hq) * a.kv.T + t] = any ? (M + __log2f(S)) * 0.6931471805599453f : -INFINITY;
     } else {
-      float* part = a.part + ((bh * R + rr) * a.splits + split) * (DH + 2);
+      float* part = a.part + ((((int64_t)b * a.kv.H + h) * R + rr) * a.splits + split) * (DH + 2);
       part[ch] = o;
       if (ch == 0) { part[DH] = M; part[DH + 1] = S; }
     }
@@ -432,9 +498,10 @@ extern "C" size_t bg_kv_cache_attn_workspace_bytes(const bg_kv_cache* cache, int
 }
 
 template <typename T, int BITS, int DH>
-static void kv_attn_launch(const KvAttnArgs& a, const KvPlan& p, int64_t blocks, hipStream_t st) {
-  if (p.packed) hipLaunchKernelGGL((kv_attn_kernel<T, BITS, DH, true>), dim3((unsigned)blocks), dim3(64 * KW), 0, st, a);
-  else hipLaunchKernelGGL((kv_attn_kernel<T, BITS, DH, false>), dim3((unsigned)blocks), dim3(64 * KW), 0, st, a);
+static void kv_attn_launch(const KvAttnArgs& a, const KvPlan& p, hipStream_t st) {
+  const dim3 grid((unsigned)(p.row_tiles * p.splits), (unsigned)a.kv.H, (unsigned)a.kv.B);
+  if (p.packed) hipLaunchKernelGGL((kv_attn_kernel<T, BITS, DH, true>), grid, dim3(64 * KW), 0, st, a);
+  else hipLaunchKernelGGL((kv_attn_kernel<T, BITS, DH, false>), grid, dim3(64 * KW), 0, st, a);
   if (p.splits > 1) {
     const int64_t rows = (int64_t)a.kv.B * a.kv.H * a.kv.T * a.G;
     hipLaunchKernelGGL((kv_attn_join_kernel<T, DH>), dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, st, a, rows);
@@ -451,8 +518,9 @@ extern "C" int bg_kv_cache_attn_fwd(const bg_kv_cache* cache, const void* data, 
   BG_REQUIRE(max_keys > 0 && max_keys <= cache->capacity, "bg_kv_cache_attn_fwd: max_keys=%d of capacity %d", max_keys, cache->capacity);
   BG_REQUIRE((int64_t)T * Hq < (1ll << 30), "bg_kv_cache_attn_fwd: T=%d Hq=%d", T, Hq);
   const KvPlan p = kv_attn_plan(cache, Hq, T, max_keys);
-  const int64_t blocks = (int64_t)cache->B * cache->H * p.row_tiles * p.splits, rows = (int64_t)cache->B * Hq * T;
-  BG_REQUIRE(blocks < (1ll << 31) && rows < (1ll << 31), "bg_kv_cache_attn_fwd: %lld blocks, %lld rows", (long long)blocks, (long long)rows);
+  const int64_t rows = (int64_t)cache->B * Hq * T;
+  BG_REQUIRE(cache->B <= 65535 && cache->H <= 65535 && (int64_t)p.row_tiles * p.splits < (1ll << 31) && rows < (1ll << 31),
+             "bg_kv_cache_attn_fwd: B=%d H=%d, %lld rows", cache->B, cache->H, (long long)rows);
   const size_t need = bg_kv_cache_attn_workspace_bytes(cache, Hq, T, max_keys);
   if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 3))) {
     set_error("bg_kv_cache_attn_fwd: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, need);
@@ -470,9 +538,9 @@ extern "C" int bg_kv_cache_attn_fwd(const bg_kv_cache* cache, const void* data, 
   a.negate = scale < 0.f;
   a.scale_log2 = (float)((scale < 0.f ? -(double)scale : (double)scale) * 1.4426950408889634);
   hipStream_t st = (hipStream_t)stream;
-#define BG_GO(BITS, DH)                                                \
-  if (dtype == BG_F32) kv_attn_launch<float, BITS, DH>(a, p, blocks, st); \
-  else kv_attn_launch<bf16_t, BITS, DH>(a, p, blocks, st)
+#define BG_GO(BITS, DH)                                           \
+  if (dtype == BG_F32) kv_attn_launch<float, BITS, DH>(a, p, st); \
+  else kv_attn_launch<bf16_t, BITS, DH>(a, p, st)
   BG_KV_DISPATCH(cache->bits, cache->Dh, BG_GO)
 #undef BG_GO
   BG_CHECK_LAUNCH("bg_kv_cache_attn_fwd");
