@@ -45,9 +45,17 @@ struct KvAttnArgs {
   int64_t o_sb, o_sh, o_st;
   float* lse;
   float* part;                              // [row][split][Dh + 2]: unnormalised output, maximum (log2), sum
-  int G, max_keys, splits, row_tiles, negate;
+  int G, max_keys, splits, each, rows_per_tile, negate;      // each: turns per split
   float scale_log2;                         // |scale| log2(e)
 };
+
+// Most (returned) and fewest keys that the rows of the tile at row0 see.
+__device__ __forceinline__ int tile_keys(const KvAttnArgs& a, int b, int row0, int& fewest) {
+  const int count = a.kv.count(b), last = min(row0 + a.rows_per_tile, a.kv.T * a.G) - 1;
+  const int t_lo = a.kv.T > 1 ? row0 / a.G : 0, t_hi = a.kv.T > 1 ? last / a.G : 0;
+  fewest = t_hi < count ? min(a.kv.visible(b, t_lo), a.max_keys) : 0;
+  return t_lo < count ? min(a.kv.visible(b, min(t_hi, count - 1)), a.max_keys) : 0;
+}
 
 template <int N> __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
   if constexpr (N % 4 == 0) {
@@ -231,20 +239,19 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<T, BITS, DH, PACKED>())) void kv
     }
   }
   if constexpr (LDS_Q) __syncthreads();
-  auto query = [&](int g, int i) __attribute__((always_inline)) -> bf16x8 {
+  auto query = [&](int g, int i, int own_g) __attribute__((always_inline)) -> bf16x8 {
     if constexpr (LDS_Q) return sh_q[g][i][lane];
     if constexpr (!OWN_Q) return qf[g][i];
     const Frag own = {.v = qf[0][i]};
     Frag f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) f.u[w] = g == my_g ? own.u[w] : 0u;
+    for (int w = 0; w < 4; ++w) f.u[w] = g == own_g ? own.u[w] : 0u;
     return f.v;
   };
 
   // what the rows of this tile see: all of them at least n_min keys, none more than n_max
-  const int count = a.kv.count(b), t_lo = a.kv.T > 1 ? row0 / a.G : 0, t_hi = a.kv.T > 1 ? (min(row0 + ROWS, R) - 1) / a.G : 0;
-  const int n_max = t_lo < count ? min(a.kv.visible(b, min(t_hi, count - 1)), a.max_keys) : 0;
-  const int n_min = t_hi < count ? min(a.kv.visible(b, t_lo), a.max_keys) : 0;
+  int n_min;
+  const int n_max = tile_keys(a, b, row0, n_min);
   const int vis = real ? min(a.kv.visible(b, t_row), a.max_keys) : 0x7FFFFFFF;
 
   f32x4 acc[CB], off = {0.f, 0.f, 0.f, 0.f};                                 // PACKED: one offset sum; else one per group
@@ -260,12 +267,9 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<T, BITS, DH, PACKED>())) void kv
 
   const Nibbles nb;
   const int turns = (n_max + KV_TURN - 1) / KV_TURN;
-  int t_end = turns;
-  if (a.splits > 1) {
-    const int each = (int)((uint32_t)turns / (uint32_t)a.splits), more = turns - each * a.splits;      // the first `more` splits take one more
-    t_begin = split * each + min(split, more);
-    t_end = t_begin + each + (split < more ? 1 : 0);
-  }
+  t_begin = split * a.each;
+  const int t_end = min(turns, t_begin + a.each);
+  if (split > 0 && t_begin >= turns) return;                                 // nothing here: the joining kernel counts the same way
   const int my_turns = t_end - t_begin > wave ? (t_end - t_begin - wave + KW - 1) / KW : 0;
   const int steps = my_turns * SUB;
   if (a.splits > 1 && steps > 0) load_k(0);
@@ -273,13 +277,15 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<T, BITS, DH, PACKED>())) void kv
     load_v(step);
     // scores
     f32x4 sc[TS];
+    int own_g = my_g;
+    if constexpr (OWN_Q) asm volatile("" : "+v"(own_g));      // the selects stay in the loop: ahead of it they would take NG times the registers
 #pragma unroll
     for (int t = 0; t < TS; ++t) sc[t] = PACKED ? f32x4{q0[0], q0[0], q0[0], q0[0]} : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       bf16x8 qg[NQ];
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) qg[i] = query(g, i);
+      for (int i = 0; i < NQ; ++i) qg[i] = query(g, i, own_g);
 #pragma unroll
       for (int t = 0; t < TS; ++t) {
         const bf16x8 kf = unpack_codes<BITS>(&kw[t][g * L::WORD / 4], nb);
@@ -340,19 +346,17 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<T, BITS, DH, PACKED>())) void kv
       const float keep = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mc - m_new);
       mc = m_new;
       l *= keep;
-      if (step != 0) {
-        float f[4];                                                          // of the accumulators' rows 4 j + r: lane 4 j + r has it
+      float f[4];                                                            // of the accumulators' rows 4 j + r: lane 4 j + r has it
 #pragma unroll
-        for (int r = 0; r < 4; ++r) f[r] = __shfl(keep, 4 * j + r);
+      for (int r = 0; r < 4; ++r) f[r] = __shfl(keep, 4 * j + r);
 #pragma unroll
-        for (int c = 0; c < CB; ++c)
+      for (int c = 0; c < CB; ++c)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[c][r] *= f[r];
+        for (int r = 0; r < 4; ++r) acc[c][r] *= f[r];
 #pragma unroll
-        for (int g = 0; g < (PACKED ? 1 : NG); ++g)
+      for (int g = 0; g < (PACKED ? 1 : NG); ++g)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) offg[g][r] *= f[r];
-      }
+        for (int r = 0; r < 4; ++r) offg[g][r] *= f[r];
     }
     const float ms = mc == -INFINITY ? 0.f : mc;
     float p[TS][4];
@@ -440,40 +444,60 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<T, BITS, DH, PACKED>())) void kv
   }
 }
 
-// Joins the splits of a row: one wave per row.
+// Joins the splits of a row: one wave per row, the states of eight splits under way together.
 template <typename T, int DH>
-__global__ __launch_bounds__(256) void kv_attn_join_kernel(KvAttnArgs a, int64_t rows) {
+__global__ __launch_bounds__(256) void kv_attn_join_kernel(KvAttnArgs a, uint32_t rows) {
+  constexpr int PER = (DH + 63) / 64, U = 8;
   const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const uint32_t row = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= rows) return;
-  const int R = a.kv.T * a.G;
-  const int64_t bh = row / R;
-  const int rr = (int)(row % R), b = (int)(bh / a.kv.H), h = (int)(bh % a.kv.H), t = rr / a.G, hq = h * a.G + rr % a.G;
-  const float* part = a.part + row * a.splits * (DH + 2);
-  float M = -INFINITY;
-  for (int s = lane; s < a.splits; s += 64) M = fmaxf(M, part[(int64_t)s * (DH + 2) + DH]);
-  M = wave_max(M);
-  const float Ms = M == -INFINITY ? 0.f : M;
-  float S = 0.f, o[(DH + 63) / 64] = {};
-  for (int s = 0; s < a.splits; ++s) {
-    const float* ps = part + (int64_t)s * (DH + 2);
-    const float f = __builtin_amdgcn_exp2f(ps[DH] - Ms);
-    S += f * ps[DH + 1];
+  const uint32_t R = (uint32_t)(a.kv.T * a.G), bh = row / R;
+  const int rr = (int)(row - bh * R), b = (int)(bh / (uint32_t)a.kv.H), h = (int)(bh - b * (uint32_t)a.kv.H);
+  const int t = rr / a.G, hq = h * a.G + rr % a.G;
+  int fewest;
+  const int turns = (tile_keys(a, b, rr - rr % a.rows_per_tile, fewest) + KV_TURN - 1) / KV_TURN;
+  const int splits = max(1, (turns + a.each - 1) / a.each);
+  const float* part = a.part + (int64_t)row * a.splits * (DH + 2);
+  float M = -INFINITY, S = 0.f, o[PER] = {};
+  for (int s0 = 0; s0 < splits; s0 += U) {
+    float m[U], l[U], v[U][PER];
 #pragma unroll
-    for (int i = 0; i < (DH + 63) / 64; ++i)
-      if (lane + 64 * i < DH) o[i] += f * ps[lane + 64 * i];
+    for (int u = 0; u < U; ++u) {
+      const float* ps = part + (int64_t)min(s0 + u, splits - 1) * (DH + 2);
+      m[u] = s0 + u < splits ? ps[DH] : -INFINITY;
+      l[u] = ps[DH + 1];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) v[u][i] = ps[min(lane + 64 * i, DH - 1)];
+    }
+    float top = M;
+#pragma unroll
+    for (int u = 0; u < U; ++u) top = fmaxf(top, m[u]);
+    const float ms = top == -INFINITY ? 0.f : top, keep = __builtin_amdgcn_exp2f(M - ms);
+    M = top;
+    S *= keep;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) o[i] *= keep;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float f = s0 + u < splits ? __builtin_amdgcn_exp2f(m[u] - ms) : 0.f;
+      const bool in = s0 + u < splits;
+      S += in ? f * l[u] : 0.f;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) o[i] += in ? f * v[u][i] : 0.f;
+    }
   }
   const bool any = a.kv.visible(b, t) > 0;
 #pragma unroll
-  for (int i = 0; i < (DH + 63) / 64; ++i)
+  for (int i = 0; i < PER; ++i)
     if (lane + 64 * i < DH) ((T*)a.out)[b * a.o_sb + hq * a.o_sh + t * a.o_st + lane + 64 * i] = from_f32<T>(any ? o[i] / S : 0.f);
   if (a.lse && lane == 0) a.lse[((int64_t)b * a.kv.H * a.G + hq) * a.kv.T + t] = any ? (M + __log2f(S)) * 0.6931471805599453f : -INFINITY;
 }
 
 // How many workgroups share a row tile's key range: enough to give every CU two (512), none with less than one turn for each wave.
+// A split is a fixed number of turns, so shorter sequences have fewer splits and all workgroups the same work.
 struct KvPlan {
   bool packed;
-  int row_tiles, splits;
+  int row_tiles, splits, each;
 };
 static KvPlan kv_attn_plan(const bg_kv_cache* c, int Hq, int T, int max_keys) {
   KvPlan p;
@@ -481,9 +505,10 @@ static KvPlan kv_attn_plan(const bg_kv_cache* c, int Hq, int T, int max_keys) {
   const int ng = c->Dh / KV_GROUP;
   p.packed = R <= 16 / ng;
   p.row_tiles = (int)cdiv(R, p.packed ? 16 / ng : 16);
-  const int64_t base = (int64_t)c->B * c->H * p.row_tiles;
-  const int64_t most = cdiv(max_keys, KV_TURN * KW), want = cdiv(512, base);
-  p.splits = (int)(want < most ? want : most);
+  const int64_t base = (int64_t)c->B * c->H * p.row_tiles, turns = cdiv(max_keys, KV_TURN);
+  const int64_t most = cdiv(turns, KW), want = cdiv(512, base);
+  p.each = (int)cdiv(turns, want < most ? want : most);
+  p.splits = (int)cdiv(turns, p.each);
   return p;
 }
 
@@ -503,7 +528,7 @@ static void kv_attn_launch(const KvAttnArgs& a, const KvPlan& p, hipStream_t st)
   if (p.packed) hipLaunchKernelGGL((kv_attn_kernel<T, BITS, DH, true>), grid, dim3(64 * KW), 0, st, a);
   else hipLaunchKernelGGL((kv_attn_kernel<T, BITS, DH, false>), grid, dim3(64 * KW), 0, st, a);
   if (p.splits > 1) {
-    const int64_t rows = (int64_t)a.kv.B * a.kv.H * a.kv.T * a.G;
+    const uint32_t rows = (uint32_t)(a.kv.B * a.kv.H) * (uint32_t)(a.kv.T * a.G);
     hipLaunchKernelGGL((kv_attn_join_kernel<T, DH>), dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, st, a, rows);
   }
 }
@@ -534,7 +559,8 @@ extern "C" int bg_kv_cache_attn_fwd(const bg_kv_cache* cache, const void* data, 
   a.q = q; a.q_sb = q_sb; a.q_sh = q_sh; a.q_st = q_st;
   a.out = out; a.o_sb = o_sb; a.o_sh = o_sh; a.o_st = o_st;
   a.lse = lse; a.part = (float*)workspace;
-  a.G = Hq / cache->H; a.max_keys = max_keys; a.splits = p.splits; a.row_tiles = p.row_tiles;
+  a.G = Hq / cache->H; a.max_keys = max_keys; a.splits = p.splits; a.each = p.each;
+  a.rows_per_tile = p.packed ? 16 / (cache->Dh / KV_GROUP) : 16;
   a.negate = scale < 0.f;
   a.scale_log2 = (float)((scale < 0.f ? -(double)scale : (double)scale) * 1.4426950408889634);
   hipStream_t st = (hipStream_t)stream;

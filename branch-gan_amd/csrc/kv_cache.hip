@@ -6,7 +6,8 @@
 // s = NaN and reads as NaN, so a broken activation shows instead of turning into a large finite number.
 // The code is that of the REAL quotient x / s, not of a rounded one: with r = 1 / s correctly rounded, q0 = x r, q = q0 + (x - q0 s) r
 // is the correctly rounded quotient (Markstein).  For bf16 x it lands on k + 1/2 only if the real quotient does (both have 8
-// significant bits); for fp32 x the sign of x - q s decides there.
+// significant bits); for fp32 x the sign of x - q s decides there.  No code needs clamping: s is within 2^-9 of a / L, so |x / s| <
+// L + 1/2.  Adding 1.5 * 2^23 + offset rounds q to an integer, half to even, in the float's low bits, where packing takes it from.
 //
 // Bound by HBM for prompts (bytes in + 0.56 or 1.06 bytes per value out), by latency for one token.
 #include "kv_cache.h"
@@ -18,30 +19,39 @@ __device__ __forceinline__ uint16_t f32_to_bf16_bits(float x) {          // roun
   return (uint16_t)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
 }
 
-// scale bits of a group from the bits of its largest magnitude (ordered as integers: finite < inf < NaN); rs = 1 / s or 0
-template <int TOP> __device__ __forceinline__ uint16_t group_scale(uint32_t amax_bits, float& s, float& rs) {
-  if (amax_bits > 0x7F000000u) { s = 0.f; rs = 0.f; return 0x7FC0; }
-  uint16_t b = f32_to_bf16_bits(__uint_as_float(amax_bits) / (float)TOP);
-  if (b < 0x0080) b = 0;
-  s = bf16_bits_to_f32(b);
-  rs = b ? 1.0f / s : 0.f;
-  return b;
+template <int CTRL> __device__ __forceinline__ uint32_t dpp_max(uint32_t x) {
+  return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, true));
 }
 
-template <typename T, int TOP> __device__ __forceinline__ int code_of(float x, float s, float rs) {
+// Scale bits of a group from the bits of its largest magnitude (ordered as integers: finite < inf < NaN); rs = 1 / s or 0.
+template <typename T, int TOP> __device__ __forceinline__ uint16_t group_scale(uint32_t amax_bits, float& s, float& rs) {
+  const float a = __uint_as_float(amax_bits);
+  // a bf16 a is at least 2^-16 away from where a / L rounds the other way, so a product will do for it
+  uint32_t b = f32_to_bf16_bits(sizeof(T) == 2 ? a * (1.0f / TOP) : a / (float)TOP);
+  if (b < 0x0080u) b = 0;
+  const bool broken = amax_bits > 0x7F000000u;
+  s = broken ? 0.f : bf16_bits_to_f32(b);
+  const float r0 = __builtin_amdgcn_rcpf(s);                    // one step makes it the rounded reciprocal: 1 / s of an 8-bit s stays
+  const float r = __builtin_fmaf(__builtin_fmaf(-s, r0, 1.f), r0, r0);      // 2^-33 clear of a tie
+  rs = b == 0 || broken ? 0.f : r;
+  return broken ? 0x7FC0 : (uint16_t)b;
+}
+
+constexpr float KV_MAGIC = 12582912.f;          // 1.5 * 2^23
+
+// The code of x plus OFFSET (0 when rs is 0: x may be anything) in the low bits of KV_MAGIC's integer part: the rest are KV_MAGIC's own bits.
+template <typename T, int OFFSET> __device__ __forceinline__ uint32_t code_bits(float x, float s, float rs) {
   const float q0 = x * rs;
   const float e0 = __builtin_fmaf(-q0, s, x);
-  const float q = __builtin_fmaf(e0, rs, q0);
-  float c = __builtin_rintf(q);
+  float q = __builtin_fmaf(e0, rs, q0);
   if constexpr (sizeof(T) == 4) {
-    const float h = q - c;
-    if (__builtin_fabsf(h) == 0.5f) {
+    const float half = q - __builtin_rintf(q);
+    if (__builtin_fabsf(half) == 0.5f) {                         // is x on, below or above the border q s ?
       const float e = __builtin_fmaf(-q, s, x);
-      if (e != 0.f) c = e > 0.f ? q + 0.5f : q - 0.5f;
+      if (e != 0.f) q += e > 0.f ? 0.25f : -0.25f;
     }
   }
-  c = __builtin_fminf(__builtin_fmaxf(c, (float)-TOP), (float)TOP);        // s = 0 (zeros, NaN groups): rs = 0 and c = 0 or NaN -> below
-  return rs == 0.f ? 0 : (int)c;
+  return __float_as_uint(q + (KV_MAGIC + (float)OFFSET));
 }
 
 // One token per sequence: a thread per (K or V, batch, head, channel).  The 32 lanes of a group share its scale through shuffles;
@@ -60,11 +70,14 @@ __global__ __launch_bounds__(256) void kv_append_token_kernel(KvArgs a, const T*
   if (a.count(b) < 1 || pos < 0 || pos >= a.capacity) return;
   const float x = to_f32(is_v ? v[b * v_sb + h * v_sh + c] : k[b * k_sb + h * k_sh + c]);
   uint32_t m = __float_as_uint(x) & 0x7FFFFFFFu;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
+  m = dpp_max<0xB1>(m);                                        // 1, 2, 4, 8: quad_perm, half row, row mirrors
+  m = dpp_max<0x4E>(m);
+  m = dpp_max<0x141>(m);
+  m = dpp_max<0x140>(m);
+  m = max(m, (uint32_t)__shfl_xor((int)m, 16));
   float s, rs;
-  const uint16_t sb = group_scale<L::TOP>(m, s, rs);
-  const uint32_t code = (uint32_t)(code_of<T, L::TOP>(x, s, rs) + L::OFF) & 255u;
+  const uint16_t sb = group_scale<T, L::TOP>(m, s, rs);
+  const uint32_t code = rs == 0.f ? (uint32_t)L::OFF : code_bits<T, L::OFF>(x, s, rs) & (BITS == 4 ? 15u : 255u);
   uint8_t* tile = a.data + b * a.c_sb + h * a.c_sh + (int64_t)(pos / KV_TILE) * L::BYTES;
   const int key = pos % KV_TILE, g = c / KV_GROUP, kg = (c / 8) % 4;
   if ((c & 31) == 0) *(uint16_t*)(tile + (is_v ? L::VS : L::KS) + L::scale_at(key, g)) = sb;
@@ -167,36 +180,48 @@ __global__ __launch_bounds__(128) void kv_append_tiles_kernel(KvArgs a, const T*
           for (int j = 0; j < 8; ++j) x[e][j] = 0.f;
         }
       }
-      uint32_t vw[8][BITS == 4 ? 1 : 2] = {};
+      // words as sums of shifted code bits: what KV_MAGIC's bits add up to is taken off beforehand; 8-bit codes run through an offset
+      // of 128, so that no byte borrows from the next, and lose it to a flip of every top bit
+      constexpr int OFFSET = BITS == 4 ? L::OFF : 128;
+      constexpr uint32_t START = 0u - (BITS == 4 ? 0x4B400000u * 0x11111111u : 0x4B400000u * 0x01010101u);
+      uint32_t vw[8][BITS / 4];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int w = 0; w < BITS / 4; ++w) vw[j][w] = START;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const bool in = key0 + e >= lo && key0 + e < hi;
         uint32_t m = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[e][j]) & 0x7FFFFFFFu);
-        m = max(m, (uint32_t)__shfl_xor((int)m, 1));
-        m = max(m, (uint32_t)__shfl_xor((int)m, 2));
+        m = dpp_max<0xB1>(m);                                  // the 4 lanes of a group are adjacent
+        m = dpp_max<0x4E>(m);
         float s, rs;
-        const uint16_t sb = group_scale<L::TOP>(m, s, rs);
+        const uint16_t sb = group_scale<T, L::TOP>(m, s, rs);
         const int key = 8 * oct + e;
         if (in && kg == 0) *(uint16_t*)(img + (kv ? L::VS : L::KS) + L::scale_at(key, g)) = sb;
-        uint32_t kw[2] = {0, 0};
+        uint32_t kw[BITS / 4];
+#pragma unroll
+        for (int w = 0; w < BITS / 4; ++w) kw[w] = START;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const uint32_t code = (uint32_t)(code_of<T, L::TOP>(x[e][j], s, rs) + L::OFF) & 255u;
-          if constexpr (BITS == 4) {
-            if (kv == 0) kw[0] |= code << (4 * kv_nibble(j));
-            else vw[j][0] |= code << (4 * kv_nibble(e));
-          } else {
-            if (kv == 0) kw[j / 4] |= code << (8 * (j % 4));
-            else vw[j][e / 4] |= code << (8 * (e % 4));
-          }
+          // a group of zeros or a broken one: rs = 0, and 0 (or NaN) times it must not reach the code
+          const uint32_t code = code_bits<T, OFFSET>(rs == 0.f ? 0.f : x[e][j], s, rs);
+          uint32_t& w = kv == 0 ? kw[BITS == 4 ? 0 : j / 4] : vw[j][BITS == 4 ? 0 : e / 4];
+          w += code << (BITS == 4 ? 4 * kv_nibble(kv == 0 ? j : e) : 8 * ((kv == 0 ? j : e) % 4));
         }
         if (kv == 0 && in) {
           uint32_t* p = (uint32_t*)(img + key * L::KROW + (kg * L::NG + g) * L::WORD);
-          p[0] = kw[0];
-          if constexpr (BITS == 8) p[1] = kw[1];
+#pragma unroll
+          for (int w = 0; w < BITS / 4; ++w) p[w] = BITS == 4 ? kw[w] : kw[w] ^ 0x80808080u;
         }
+      }
+      if constexpr (BITS == 8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int w = 0; w < 2; ++w) vw[j][w] ^= 0x80808080u;
       }
       if (kv == 1) {
         uint32_t mask[2] = {0, 0};
