@@ -104,19 +104,48 @@ __global__ __launch_bounds__(256) void kv_append_token_kernel(KvArgs a, const T*
   }
 }
 
-template <typename T, bool VEC> __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-  if constexpr (!VEC) {
+// Bits of the largest magnitude among 8 numbers; bf16 pairs are compared as packed 16-bit integers.
+__device__ __forceinline__ uint32_t max_magnitude(const float (&x)[8]) {
+  uint32_t m = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = to_f32(p[j]);
-  } else if constexpr (sizeof(T) == 2) {
-    const bf16x8 r = *(const bf16x8*)p;
+  for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[j]) & 0x7FFFFFFFu);
+  return m;
+}
+__device__ __forceinline__ uint32_t max_magnitude(const bf16x8& x) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  const u32x4 u = __builtin_bit_cast(u32x4, x) & 0x7FFF7FFFu;
+  // (the casts: a bit cast of a vector element itself reads the first one)
+  const u16x2 a = __builtin_elementwise_max(__builtin_bit_cast(u16x2, (uint32_t)u[0]), __builtin_bit_cast(u16x2, (uint32_t)u[1]));
+  const u16x2 b = __builtin_elementwise_max(__builtin_bit_cast(u16x2, (uint32_t)u[2]), __builtin_bit_cast(u16x2, (uint32_t)u[3]));
+  const uint32_t m = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(a, b));
+  return max(m << 16, m & 0xFFFF0000u);
+}
+
+// 8 neighbouring channels as they come from memory: bf16x8, or float[8]
+template <typename T> struct Octet { typedef bf16x8 type; };
+template <> struct Octet<float> { struct type { float x[8]; __device__ __forceinline__ float operator[](int i) const { return x[i]; } }; };
+__device__ __forceinline__ uint32_t max_magnitude(const Octet<float>::type& x) { return max_magnitude(x.x); }
+template <typename T, bool VEC> __device__ __forceinline__ typename Octet<T>::type load_octet(const T* p) {
+  typename Octet<T>::type r;
+  if constexpr (sizeof(T) == 2) {
+    if constexpr (VEC) {
+      r = *(const bf16x8*)p;
+    } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = (float)r[j];
+      for (int j = 0; j < 8; ++j) r[j] = p[j];
+    }
   } else {
-    const f32x4 r0 = *(const f32x4*)p, r1 = *(const f32x4*)(p + 4);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) { x[j] = r0[j]; x[4 + j] = r1[j]; }
+    for (int h = 0; h < 2; ++h) {
+      f32x4 v;
+      if constexpr (VEC) v = *(const f32x4*)(p + 4 * h);
+      else v = f32x4{p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3]};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r.x[4 * h + j] = v[j];
+    }
   }
+  return r;
 }
 
 template <typename T, bool VEC> __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
@@ -137,172 +166,171 @@ template <typename T, bool VEC> __device__ __forceinline__ void store8(T* p, con
   }
 }
 
-// Several tokens: 128 threads take 256 / DH tiles, a thread the 8 keys x 8 channels of one word column of K and of V (so that the
-// transposition of V stays in its registers).  The tile is put together in LDS and leaves as whole 16-byte rows; a tile that the
-// new tokens cover only in part is read first, and the codes and scales of its other keys go back as they were.
-template <typename T, int BITS, int DH, bool VEC>
-__global__ __launch_bounds__(128) void kv_append_tiles_kernel(KvArgs a, const T* k, const T* v, int64_t k_sb, int64_t k_sh, int64_t k_st,
-                                                              int64_t v_sb, int64_t v_sh, int64_t v_st, int blocks_per_head) {
+// Several tokens: 128 threads take the keys, or (the other half of the grid) the values, of 256 / DH tiles; a thread the 8 keys x 8
+// channels of one word column (so that the transposition of V stays in its registers).  A tile's part is put together in LDS and
+// leaves as whole 16-byte rows; a tile that the new tokens cover only in part is read first, and the codes and scales of its other
+// keys go back as they were.  (Keys and values apart: twice the workgroups of half the registers; 8 x 777 tokens of 12 heads of 64
+// in fp32 17.9 -> 15.8 us.)
+template <typename T, int BITS, int DH, bool VEC, int KV>
+__device__ __forceinline__ void append_tiles(const KvArgs& a, const T* src0, int64_t sb, int64_t sh, int64_t st, int blk, int blocks_per_head,
+                                             uint8_t* image) {
   using L = KvTile<BITS, DH>;
   constexpr int TPW = 256 / DH, NTH = DH / 2, U = DH / 8;
-  __shared__ __attribute__((aligned(16))) uint8_t image[TPW * L::BYTES];
+  constexpr int CODES = KV ? L::V : 0, CODE_BYTES = KV ? DH * L::VROW : L::V, SCALES = KV ? L::VS : L::KS, SCALE_BYTES = L::VS - L::KS;
+  constexpr int PART = CODE_BYTES + SCALE_BYTES;                // this part of a tile, codes then scales
   const int tid = threadIdx.x, lt = tid / NTH, ti = tid % NTH, u = ti % U, oct = ti / U;
-  const int64_t bh = blockIdx.x / blocks_per_head;
-  const int b = (int)(bh / a.H), h = (int)(bh % a.H);
+  const int bh = blk / blocks_per_head, b = bh / a.H, h = bh % a.H;
   const int start = a.first(b), count = a.count(b);
   // new tokens that fit: positions lo .. hi - 1
   const int64_t hi64 = (int64_t)start + count;
   const int lo = start < 0 ? 0 : min(start, a.capacity), hi = (int)(hi64 < 0 ? 0 : (hi64 > a.capacity ? a.capacity : hi64));
-  const int tile = lo / KV_TILE + (int)(blockIdx.x % blocks_per_head) * TPW + lt;
-  const int k0 = tile * KV_TILE;                               // (a capacity below 2^31 - 4096 is required)
+  const int tile = lo / KV_TILE + (blk % blocks_per_head) * TPW + lt;
+  const int k0 = tile * KV_TILE;                               // (a capacity below 2^30 is required)
   const bool any = k0 < hi && lo < hi;                         // tiles past the last token: nothing to do
   const bool whole = k0 >= lo && k0 + KV_TILE <= hi;
   uint8_t* out = a.data + b * a.c_sb + h * a.c_sh + (int64_t)tile * L::BYTES;
-  uint8_t* img = image + lt * L::BYTES;
+  uint8_t* img = image + lt * PART;
+  const auto at = [](int i) { return 16 * i < CODE_BYTES ? CODES + 16 * i : SCALES + 16 * i - CODE_BYTES; };
   if (any && !whole)
-    for (int i = ti; i < L::BYTES / 16; i += NTH) *(uint4*)(img + 16 * i) = *(const uint4*)(out + 16 * i);
+    for (int i = ti; i < PART / 16; i += NTH) *(uint4*)(img + 16 * i) = *(const uint4*)(out + at(i));
   __syncthreads();
   if (any) {
     const int g = u / 4, kg = u % 4;
     const int key0 = k0 + 8 * oct;
-    const T* src[2] = {k + b * k_sb + h * k_sh + 8 * u, v + b * v_sb + h * v_sh + 8 * u};
-    const int64_t st[2] = {k_st, v_st};
+    const T* src = src0 + b * sb + h * sh + 8 * u;
+    // rows outside the new tokens are read as the nearest one inside, and what comes of them is not stored
+    typename Octet<T>::type x[8];
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-      float x[8][8];
+    for (int e = 0; e < 8; ++e) x[e] = load_octet<T, VEC>(src + (int64_t)(min(max(key0 + e, lo), hi - 1) - start) * st);
+    // words as sums of shifted code bits: what KV_MAGIC's bits add up to is taken off beforehand; 8-bit codes run through an offset
+    // of 128, so that no byte borrows from the next, and lose it to a flip of every top bit
+    constexpr int OFFSET = BITS == 4 ? L::OFF : 128;
+    constexpr uint32_t START = 0u - (BITS == 4 ? 0x4B400000u * 0x11111111u : 0x4B400000u * 0x01010101u);
+    constexpr uint32_t FLIP = BITS == 4 ? 0u : 0x80808080u;
+    uint32_t vw[8][BITS / 4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int pos = key0 + e;
-        if (pos >= lo && pos < hi) {
-          load8<T, VEC>(src[kv] + (int64_t)(pos - start) * st[kv], x[e]);
-        } else {
+    for (int j = 0; j < 8; ++j)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) x[e][j] = 0.f;
-        }
+      for (int w = 0; w < BITS / 4; ++w) vw[j][w] = START;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const bool in = key0 + e >= lo && key0 + e < hi;
+      uint32_t m = max_magnitude(x[e]);
+      m = dpp_max<0xB1>(m);                                    // the 4 lanes of a group are adjacent
+      m = dpp_max<0x4E>(m);
+      float s, rs;
+      const uint16_t scale = group_scale<T, L::TOP>(m, s, rs);
+      const int key = 8 * oct + e;
+      if (in && kg == 0) *(uint16_t*)(img + CODE_BYTES + L::scale_at(key, g)) = scale;
+      uint32_t kw[BITS / 4];
+#pragma unroll
+      for (int w = 0; w < BITS / 4; ++w) kw[w] = START;
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = (float)x[e][j];
+      if (__any(scale == 0x7FC0)) {                            // a broken group in this wave: its NaNs must not reach the sums
+        asm volatile("");                                      // (a branch, not selects on every element of every call)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = scale == 0x7FC0 ? 0.f : f[j];
       }
-      // words as sums of shifted code bits: what KV_MAGIC's bits add up to is taken off beforehand; 8-bit codes run through an offset
-      // of 128, so that no byte borrows from the next, and lose it to a flip of every top bit
-      constexpr int OFFSET = BITS == 4 ? L::OFF : 128;
-      constexpr uint32_t START = 0u - (BITS == 4 ? 0x4B400000u * 0x11111111u : 0x4B400000u * 0x01010101u);
-      uint32_t vw[8][BITS / 4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t code = code_bits<T, OFFSET>(f[j], s, rs);
+        uint32_t& w = KV == 0 ? kw[BITS == 4 ? 0 : j / 4] : vw[j][BITS == 4 ? 0 : e / 4];
+        w += code << (BITS == 4 ? 4 * kv_nibble(KV == 0 ? j : e) : 8 * ((KV == 0 ? j : e) % 4));
+      }
+      if (KV == 0 && in) {
+        uint32_t* p = (uint32_t*)(img + key * L::KROW + (kg * L::NG + g) * L::WORD);
 #pragma unroll
-        for (int w = 0; w < BITS / 4; ++w) vw[j][w] = START;
+        for (int w = 0; w < BITS / 4; ++w) p[w] = kw[w] ^ FLIP;
+      }
+    }
+    if constexpr (KV == 1) {
+      uint32_t mask[2] = {0, 0};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const bool in = key0 + e >= lo && key0 + e < hi;
-        uint32_t m = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[e][j]) & 0x7FFFFFFFu);
-        m = dpp_max<0xB1>(m);                                  // the 4 lanes of a group are adjacent
-        m = dpp_max<0x4E>(m);
-        float s, rs;
-        const uint16_t sb = group_scale<T, L::TOP>(m, s, rs);
-        const int key = 8 * oct + e;
-        if (in && kg == 0) *(uint16_t*)(img + (kv ? L::VS : L::KS) + L::scale_at(key, g)) = sb;
-        uint32_t kw[BITS / 4];
-#pragma unroll
-        for (int w = 0; w < BITS / 4; ++w) kw[w] = START;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          // a group of zeros or a broken one: rs = 0, and 0 (or NaN) times it must not reach the code
-          const uint32_t code = code_bits<T, OFFSET>(rs == 0.f ? 0.f : x[e][j], s, rs);
-          uint32_t& w = kv == 0 ? kw[BITS == 4 ? 0 : j / 4] : vw[j][BITS == 4 ? 0 : e / 4];
-          w += code << (BITS == 4 ? 4 * kv_nibble(kv == 0 ? j : e) : 8 * ((kv == 0 ? j : e) % 4));
-        }
-        if (kv == 0 && in) {
-          uint32_t* p = (uint32_t*)(img + key * L::KROW + (kg * L::NG + g) * L::WORD);
-#pragma unroll
-          for (int w = 0; w < BITS / 4; ++w) p[w] = BITS == 4 ? kw[w] : kw[w] ^ 0x80808080u;
-        }
+        if constexpr (BITS == 4) mask[0] |= in ? 15u << (4 * kv_nibble(e)) : 0u;
+        else mask[e / 4] |= in ? 255u << (8 * (e % 4)) : 0u;
       }
-      if constexpr (BITS == 8) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+      for (int j = 0; j < 8; ++j) {
+        uint32_t* p = (uint32_t*)(img + (8 * u + j) * L::VROW + oct * L::WORD);
 #pragma unroll
-          for (int w = 0; w < 2; ++w) vw[j][w] ^= 0x80808080u;
-      }
-      if (kv == 1) {
-        uint32_t mask[2] = {0, 0};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const bool in = key0 + e >= lo && key0 + e < hi;
-          if constexpr (BITS == 4) mask[0] |= in ? 15u << (4 * kv_nibble(e)) : 0u;
-          else mask[e / 4] |= in ? 255u << (8 * (e % 4)) : 0u;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          uint32_t* p = (uint32_t*)(img + L::V + (8 * u + j) * L::VROW + oct * L::WORD);
-#pragma unroll
-          for (int w = 0; w < BITS / 4; ++w) p[w] = whole ? vw[j][w] : ((p[w] & ~mask[w]) | (vw[j][w] & mask[w]));
+        for (int w = 0; w < BITS / 4; ++w) {
+          const uint32_t c = vw[j][w] ^ FLIP;
+          p[w] = whole ? c : ((p[w] & ~mask[w]) | (c & mask[w]));
         }
       }
     }
   }
   __syncthreads();
   if (any)
-    for (int i = ti; i < L::BYTES / 16; i += NTH) *(uint4*)(out + 16 * i) = *(const uint4*)(img + 16 * i);
+    for (int i = ti; i < PART / 16; i += NTH) *(uint4*)(out + at(i)) = *(const uint4*)(img + 16 * i);
+}
+
+template <typename T, int BITS, int DH, bool VEC>
+__global__ __launch_bounds__(128) void kv_append_tiles_kernel(KvArgs a, const T* k, const T* v, int64_t k_sb, int64_t k_sh, int64_t k_st,
+                                                              int64_t v_sb, int64_t v_sh, int64_t v_st, int blocks_per_head) {
+  __shared__ __attribute__((aligned(16))) uint8_t image[256 / DH * KvTile<BITS, DH>::BYTES / 2];
+  const int half = (int)(gridDim.x / 2);
+  if ((int)blockIdx.x < half) append_tiles<T, BITS, DH, VEC, 0>(a, k, k_sb, k_sh, k_st, blockIdx.x, blocks_per_head, image);
+  else append_tiles<T, BITS, DH, VEC, 1>(a, v, v_sb, v_sh, v_st, blockIdx.x - half, blocks_per_head, image);
 }
 
 // Values back: the same 8 x 8 blocks, codes straight from memory.  Row t of the output is position start + t; rows at or past the
 // sequence's count, and positions outside the cache, are zeros.
-template <typename T, int BITS, int DH, bool VEC>
-__global__ __launch_bounds__(128) void kv_read_kernel(KvArgs a, T* k, T* v, int64_t o_sb, int64_t o_sh, int64_t o_st, int blocks_per_head) {
+template <typename T, int BITS, int DH, bool VEC, int KV>
+__device__ __forceinline__ void read_tiles(const KvArgs& a, T* out0, int64_t o_sb, int64_t o_sh, int64_t o_st, int blk, int blocks_per_head) {
   using L = KvTile<BITS, DH>;
   constexpr int TPW = 256 / DH, NTH = DH / 2, U = DH / 8;
   const int tid = threadIdx.x, lt = tid / NTH, ti = tid % NTH, u = ti % U, oct = ti / U;
-  const int64_t bh = blockIdx.x / blocks_per_head;
-  const int b = (int)(bh / a.H), h = (int)(bh % a.H);
+  const int bh = blk / blocks_per_head, b = bh / a.H, h = bh % a.H;
   const int64_t start = a.first(b);
   const int count = a.count(b);
   const int64_t floor_tile = start >= 0 ? start / KV_TILE : -((KV_TILE - 1 - start) / KV_TILE);
-  const int64_t tile = floor_tile + (int64_t)(blockIdx.x % blocks_per_head) * TPW + lt;
+  const int64_t tile = floor_tile + (int64_t)(blk % blocks_per_head) * TPW + lt;
   const int64_t pos0 = tile * KV_TILE + 8 * oct;               // this thread's 8 positions
   if (pos0 + 8 <= start || pos0 >= start + a.T) return;
   const int g = u / 4, kg = u % 4;
   const uint8_t* t = a.data + b * a.c_sb + h * a.c_sh + tile * L::BYTES;
-  bool held[8];
+  uint32_t w[8][BITS / 4] = {};
+  uint16_t sc[8] = {};
+  if (tile >= 0 && tile * KV_TILE < a.capacity && pos0 < start + count) {      // the tile exists and holds rows that are asked for
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t* p = KV == 0 ? (const uint32_t*)(t + (8 * oct + i) * L::KROW + (kg * L::NG + g) * L::WORD)
+                                  : (const uint32_t*)(t + L::V + (8 * u + i) * L::VROW + oct * L::WORD);
+#pragma unroll
+      for (int q = 0; q < BITS / 4; ++q) w[i][q] = p[q];
+      sc[i] = *(const uint16_t*)(t + (KV ? L::VS : L::KS) + L::scale_at(8 * oct + i, g));
+    }
+  }
+  T* out = out0 + b * o_sb + h * o_sh + 8 * u;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const int64_t pos = pos0 + e;
-    held[e] = pos >= start && pos < start + count && pos >= 0 && pos < a.capacity;
+    const bool held = pos >= start && pos < start + count && pos >= 0 && pos < a.capacity;
+    const float s = bf16_bits_to_f32(sc[e]);
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int row = KV == 0 ? e : j, el = KV == 0 ? j : e;   // K words run along the channels, V words along the keys
+      int code;
+      if constexpr (BITS == 4) code = (int)((w[row][0] >> (4 * kv_nibble(el))) & 15u) - L::OFF;
+      else code = (int8_t)(w[row][el / 4] >> (8 * (el % 4)));
+      x[j] = held ? s * (float)code : 0.f;
+    }
+    const int64_t row = pos - start;
+    if (row >= 0 && row < a.T) store8<T, VEC>(out + row * o_st, x);
   }
-  const bool inside = tile >= 0 && tile * KV_TILE < a.capacity;      // the tile exists
-#pragma unroll
-  for (int kv = 0; kv < 2; ++kv) {
-    float x[8][8];
-    uint32_t w[8][BITS / 4] = {};
-    uint16_t sc[8] = {};
-    if (inside) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t* p = kv == 0 ? (const uint32_t*)(t + (8 * oct + i) * L::KROW + (kg * L::NG + g) * L::WORD)
-                                    : (const uint32_t*)(t + L::V + (8 * u + i) * L::VROW + oct * L::WORD);
-#pragma unroll
-        for (int q = 0; q < BITS / 4; ++q) w[i][q] = p[q];
-        sc[i] = *(const uint16_t*)(t + (kv ? L::VS : L::KS) + L::scale_at(8 * oct + i, g));
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float s = bf16_bits_to_f32(sc[e]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int row = kv == 0 ? e : j, el = kv == 0 ? j : e;      // K words run along the channels, V words along the keys
-        int code;
-        if constexpr (BITS == 4) code = (int)((w[row][0] >> (4 * kv_nibble(el))) & 15u) - L::OFF;
-        else code = (int8_t)(w[row][el / 4] >> (8 * (el % 4)));
-        x[e][j] = held[e] ? s * (float)code : 0.f;
-      }
-    }
-    T* out = (kv ? v : k) + b * o_sb + h * o_sh + 8 * u;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int64_t row = pos0 + e - start;
-      if (row >= 0 && row < a.T) store8<T, VEC>(out + row * o_st, x[e]);
-    }
-  }
+}
+
+template <typename T, int BITS, int DH, bool VEC>
+__global__ __launch_bounds__(128) void kv_read_kernel(KvArgs a, T* k, T* v, int64_t o_sb, int64_t o_sh, int64_t o_st, int blocks_per_head) {
+  const int half = (int)(gridDim.x / 2);
+  if ((int)blockIdx.x < half) read_tiles<T, BITS, DH, VEC, 0>(a, k, o_sb, o_sh, o_st, blockIdx.x, blocks_per_head);
+  else read_tiles<T, BITS, DH, VEC, 1>(a, v, o_sb, o_sh, o_st, blockIdx.x - half, blocks_per_head);
 }
 
 int kv_check(const char* who, const bg_kv_cache* c, const void* data, int dtype, int64_t T) {
@@ -367,7 +395,7 @@ extern "C" int bg_kv_cache_append(const bg_kv_cache* cache, void* data, const vo
     return BG_OK;
   }
   const int64_t tiles = cdiv((int64_t)T + KV_TILE - 1, KV_TILE);            // T tokens at any offset touch at most this many
-  const int64_t per_head = cdiv(tiles, 256 / cache->Dh), blocks = per_head * heads;
+  const int64_t per_head = cdiv(tiles, 256 / cache->Dh), blocks = 2 * per_head * heads;     // keys, values
   BG_REQUIRE(blocks < (1ll << 31), "bg_kv_cache_append: %lld blocks", (long long)blocks);
 #define BG_GO2(TT, BITS, DH, VEC)                                                                                                   \
   hipLaunchKernelGGL((kv_append_tiles_kernel<TT, BITS, DH, VEC>), dim3((unsigned)blocks), dim3(128), 0, st, a, (const TT*)k,        \
@@ -391,7 +419,7 @@ extern "C" int bg_kv_cache_read(const bg_kv_cache* cache, const void* data, void
   const int e = dtype == BG_F32 ? 4 : 2;
   const bool vec = aligned16(k, o_sb, o_sh, o_st, e) && aligned16(v, 0, 0, 0, e);
   const int64_t tiles = cdiv((int64_t)T + KV_TILE - 1, KV_TILE);
-  const int64_t per_head = cdiv(tiles, 256 / cache->Dh), blocks = per_head * cache->B * cache->H;
+  const int64_t per_head = cdiv(tiles, 256 / cache->Dh), blocks = 2 * per_head * cache->B * cache->H;
   BG_REQUIRE(blocks < (1ll << 31), "bg_kv_cache_read: %lld blocks", (long long)blocks);
 #define BG_GO2(TT, BITS, DH, VEC)                                                                                                 \
   hipLaunchKernelGGL((kv_read_kernel<TT, BITS, DH, VEC>), dim3((unsigned)blocks), dim3(128), 0, st, a, (TT*)k, (TT*)v, o_sb,      \
