@@ -45,7 +45,7 @@ struct KvAttnArgs {
   int64_t o_sb, o_sh, o_st;
   float* lse;
   float* part;                              // [row][split][Dh + 2]: unnormalised output, maximum (log2), sum
-  int G, max_keys, splits, each, rows_per_tile, negate;      // each: turns per split
+  int G, max_keys, splits, rows_per_tile, negate;
   float scale_log2;                         // |scale| log2(e)
 };
 
@@ -137,7 +137,7 @@ template <int NG> __device__ __forceinline__ float group_sum(float x) {      // 
 // Waves per SIMD the kernel is built for: four for small heads, whose turns are short and bound by vector work as much as by
 // memory; else two; one (512 registers) where two would spill.
 template <typename T, int BITS, int DH, bool PACKED> constexpr int kv_waves() {
-  if (PACKED) return DH * BITS <= 256 ? (sizeof(T) == 4 && DH == 64 ? 3 : 4) : sizeof(T) == 4 && DH * BITS > 1024 ? 1 : 2;
+  if (PACKED) return DH * BITS <= 256 ? (sizeof(T) == 4 && DH == 64 ? 3 : 4) : 2;
   return DH == 256 || (DH == 128 && BITS == 4) ? 1 : 2;
 }
 
@@ -151,7 +151,7 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<T, BITS, DH, PACKED>())) void kv
   constexpr bool OWN_Q = PACKED && NG * NQ > 4;     // keep a lane's one group only, and the zeros of the others as a select per use
   constexpr bool LDS_Q = !PACKED && NG * NQ > 8;    // the pieces of long fp32 rows live in LDS
   constexpr int NQF = OWN_Q || LDS_Q ? 1 : NG;
-  constexpr int KWORDS = NG * L::WORD / 4, VWORDS = NO * L::WORD / 4;
+  constexpr int KWORDS = NG * L::WORD / 4, VWORDS = CB * L::WORD / 4;
   __shared__ float sh_o[KW][ROWS][DH];
   __shared__ float sh_m[KW][16], sh_l[KW][16];
   __shared__ bf16x8 sh_q[LDS_Q ? NG : 1][NQ][LDS_Q ? 64 : 1];
@@ -173,7 +173,7 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<T, BITS, DH, PACKED>())) void kv
     g_row = rho - t_row * a.G;
   }
 
-  uint32_t kw[TS][KWORDS], ks[GL][TS * 2], vw[CB][VWORDS], vs[GL][TS * 2];
+  uint32_t kw[TS][KWORDS], ks[GL][TS * 2], vw[NO][VWORDS], vs[GL][TS * 2];
   int t_begin = 0;
   auto key_base = [&](int step, int tile_in_turn) __attribute__((always_inline)) -> const uint8_t* {
     const int tile = (t_begin + wave + KW * (step / SUB)) * 4 + tile_in_turn;
@@ -192,7 +192,7 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<T, BITS, DH, PACKED>())) void kv
     const int s = step % SUB;
     const uint8_t* vt = key_base(step, j);
 #pragma unroll
-    for (int c = 0; c < CB; ++c) load_words<VWORDS>(vt + L::V + (16 * c + n) * L::VROW + s * NO * L::WORD, vw[c]);
+    for (int o = 0; o < NO; ++o) load_words<VWORDS>(vt + L::V + ((s * NO + o) * 16 + n) * CB * L::WORD, vw[o]);
 #pragma unroll
     for (int g = 0; g < GL; ++g) load_words<TS * 2>(vt + L::VS + s * TS * 8 + (PACKED ? my_g : g) * KV_TILE * 2, vs[g]);
   };
@@ -267,9 +267,9 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<T, BITS, DH, PACKED>())) void kv
 
   const Nibbles nb;
   const int turns = (n_max + KV_TURN - 1) / KV_TURN;
-  t_begin = split * a.each;
-  const int t_end = min(turns, t_begin + a.each);
-  if (split > 0 && t_begin >= turns) return;                                 // nothing here: the joining kernel counts the same way
+  const int each = (int)((uint32_t)turns / (uint32_t)a.splits), more = turns - each * a.splits;        // the first `more` splits take one more
+  t_begin = split * each + min(split, more);
+  const int t_end = t_begin + each + (split < more ? 1 : 0);
   const int my_turns = t_end - t_begin > wave ? (t_end - t_begin - wave + KW - 1) / KW : 0;
   const int steps = my_turns * SUB;
   if (a.splits > 1 && steps > 0) load_k(0);
@@ -397,7 +397,7 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<T, BITS, DH, PACKED>())) void kv
       }
 #pragma unroll
       for (int c = 0; c < CB; ++c) {
-        const bf16x8 vf = unpack_codes<BITS>(&vw[c][o * L::WORD / 4], nb);
+        const bf16x8 vf = unpack_codes<BITS>(&vw[o][c * L::WORD / 4], nb);
 #pragma unroll
         for (int i = 0; i < NP; ++i) acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf[PACKED ? 0 : c / 2][i], vf, acc[c], 0, 0, 0);
       }
@@ -454,9 +454,7 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(KvAttnArgs a, uint32_
   const uint32_t R = (uint32_t)(a.kv.T * a.G), bh = row / R;
   const int rr = (int)(row - bh * R), b = (int)(bh / (uint32_t)a.kv.H), h = (int)(bh - b * (uint32_t)a.kv.H);
   const int t = rr / a.G, hq = h * a.G + rr % a.G;
-  int fewest;
-  const int turns = (tile_keys(a, b, rr - rr % a.rows_per_tile, fewest) + KV_TURN - 1) / KV_TURN;
-  const int splits = max(1, (turns + a.each - 1) / a.each);
+  const int splits = a.splits;
   const float* part = a.part + (int64_t)row * a.splits * (DH + 2);
   float M = -INFINITY, S = 0.f, o[PER] = {};
   for (int s0 = 0; s0 < splits; s0 += U) {
@@ -494,10 +492,11 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(KvAttnArgs a, uint32_
 }
 
 // How many workgroups share a row tile's key range: enough to give every CU two (512), none with less than one turn for each wave.
-// A split is a fixed number of turns, so shorter sequences have fewer splits and all workgroups the same work.
+// (Even splits of every sequence: splits of a fixed number of turns, fewer for short sequences, leave CUs idle - 16 uneven sequences
+// of 8 heads, 8 bits, 67 against 79 us.)
 struct KvPlan {
   bool packed;
-  int row_tiles, splits, each;
+  int row_tiles, splits;
 };
 static KvPlan kv_attn_plan(const bg_kv_cache* c, int Hq, int T, int max_keys) {
   KvPlan p;
@@ -505,10 +504,9 @@ static KvPlan kv_attn_plan(const bg_kv_cache* c, int Hq, int T, int max_keys) {
   const int ng = c->Dh / KV_GROUP;
   p.packed = R <= 16 / ng;
   p.row_tiles = (int)cdiv(R, p.packed ? 16 / ng : 16);
-  const int64_t base = (int64_t)c->B * c->H * p.row_tiles, turns = cdiv(max_keys, KV_TURN);
-  const int64_t most = cdiv(turns, KW), want = cdiv(512, base);
-  p.each = (int)cdiv(turns, want < most ? want : most);
-  p.splits = (int)cdiv(turns, p.each);
+  const int64_t base = (int64_t)c->B * c->H * p.row_tiles;
+  const int64_t most = cdiv(max_keys, KV_TURN * KW), want = cdiv(512, base);
+  p.splits = (int)(want < most ? want : most);
   return p;
 }
 
@@ -559,7 +557,7 @@ extern "C" int bg_kv_cache_attn_fwd(const bg_kv_cache* cache, const void* data, 
   a.q = q; a.q_sb = q_sb; a.q_sh = q_sh; a.q_st = q_st;
   a.out = out; a.o_sb = o_sb; a.o_sh = o_sh; a.o_st = o_st;
   a.lse = lse; a.part = (float*)workspace;
-  a.G = Hq / cache->H; a.max_keys = max_keys; a.splits = p.splits; a.each = p.each;
+  a.G = Hq / cache->H; a.max_keys = max_keys; a.splits = p.splits;
   a.rows_per_tile = p.packed ? 16 / (cache->Dh / KV_GROUP) : 16;
   a.negate = scale < 0.f;
   a.scale_log2 = (float)((scale < 0.f ? -(double)scale : (double)scale) * 1.4426950408889634);

@@ -2,7 +2,7 @@
 //
 // A (batch, head) holds tiles of 32 consecutive keys.  One tile of head size DH, NG = DH / 32 groups of 32 channels:
 //   K codes    [32 keys][4 kg][NG g] words of the channels 32 g + 8 kg + 0..7 (8 codes: 4 bytes at 4 bits, 8 bytes at 8 bits)
-//   V codes    [DH channels][4 octets] words of the keys 8 octet + 0..7
+//   V codes    [4 octets][16 n][DH / 16 c] words of the keys 8 octet + 0..7 of channel 16 c + n
 //   K scales   [NG g][32 keys] bf16
 //   V scales   the same
 // A word is what one lane feeds to a 32-deep matrix instruction (8 consecutive elements of its row), for K along the channels and
@@ -23,11 +23,11 @@ template <int BITS, int DH> struct KvTile {
   static constexpr int OFF = BITS == 4 ? 8 : 0;
   static constexpr int WORD = BITS;                      // bytes of 8 codes
   static constexpr int KROW = DH * BITS / 8;
-  static constexpr int VROW = KV_TILE * BITS / 8;
   static constexpr int V = KV_TILE * KROW;
-  static constexpr int KS = V + DH * VROW;
+  static constexpr int KS = V + KV_TILE * DH * BITS / 8;
   static constexpr int VS = KS + KV_TILE * NG * 2;
   static constexpr int BYTES = VS + KV_TILE * NG * 2;
+  static constexpr int v_word(int oct, int ch) { return V + ((oct * 16 + ch % 16) * (DH / 16) + ch / 16) * WORD; }
   static constexpr int scale_at(int key, int g) { return (g * KV_TILE + key) * 2; }
 };
 

@@ -92,14 +92,14 @@ __global__ __launch_bounds__(256) void kv_append_token_kernel(KvArgs a, const T*
       tile[key * L::KROW + (kg * L::NG + g) * 8 + (c & 7)] = (uint8_t)code;
     }
   } else {
-    uint8_t* row = tile + L::V + c * L::VROW;
+    uint8_t* word = tile + L::v_word(key >> 3, c);
     if constexpr (BITS == 4) {
       const int nib = kv_nibble(key & 7);
-      uint8_t* p = row + (key >> 3) * 4 + (nib >> 1);
+      uint8_t* p = word + (nib >> 1);
       const int sh = 4 * (nib & 1);
       *p = (uint8_t)((*p & ~(15u << sh)) | (code << sh));
     } else {
-      row[key] = (uint8_t)code;
+      word[key & 7] = (uint8_t)code;
     }
   }
 }
@@ -176,7 +176,7 @@ __device__ __forceinline__ void append_tiles(const KvArgs& a, const T* src0, int
                                              uint8_t* image) {
   using L = KvTile<BITS, DH>;
   constexpr int TPW = 256 / DH, NTH = DH / 2, U = DH / 8;
-  constexpr int CODES = KV ? L::V : 0, CODE_BYTES = KV ? DH * L::VROW : L::V, SCALES = KV ? L::VS : L::KS, SCALE_BYTES = L::VS - L::KS;
+  constexpr int CODES = KV ? L::V : 0, CODE_BYTES = L::V, SCALES = KV ? L::VS : L::KS, SCALE_BYTES = L::VS - L::KS;
   constexpr int PART = CODE_BYTES + SCALE_BYTES;                // this part of a tile, codes then scales
   const int tid = threadIdx.x, lt = tid / NTH, ti = tid % NTH, u = ti % U, oct = ti / U;
   const int bh = blk / blocks_per_head, b = bh / a.H, h = bh % a.H;
@@ -255,7 +255,7 @@ __device__ __forceinline__ void append_tiles(const KvArgs& a, const T* src0, int
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        uint32_t* p = (uint32_t*)(img + (8 * u + j) * L::VROW + oct * L::WORD);
+        uint32_t* p = (uint32_t*)(img + L::v_word(oct, 8 * u + j) - L::V);
 #pragma unroll
         for (int w = 0; w < BITS / 4; ++w) {
           const uint32_t c = vw[j][w] ^ FLIP;
@@ -300,7 +300,7 @@ __device__ __forceinline__ void read_tiles(const KvArgs& a, T* out0, int64_t o_s
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint32_t* p = KV == 0 ? (const uint32_t*)(t + (8 * oct + i) * L::KROW + (kg * L::NG + g) * L::WORD)
-                                  : (const uint32_t*)(t + L::V + (8 * u + i) * L::VROW + oct * L::WORD);
+                                  : (const uint32_t*)(t + L::v_word(oct, 8 * u + i));
 #pragma unroll
       for (int q = 0; q < BITS / 4; ++q) w[i][q] = p[q];
       sc[i] = *(const uint16_t*)(t + (KV ? L::VS : L::KS) + L::scale_at(8 * oct + i, g));
