@@ -6,19 +6,19 @@
 // bits: signed), the scales join in fp32 - on the scores after the product, on the probabilities before it.  Nothing held is rounded again.  bf16
 // queries are exact operands; fp32 queries go in as three bf16 pieces (24 bits), probabilities as two (16 bits, for bf16 outputs) or three.
 //
-// Layout.  One wave takes 4 tiles (128 keys) per turn with v_mfma_f32_16x16x32_bf16; lane = (n = lane % 16, j = lane / 16).
-//   scores   A = K codes: row rr of 16 is key 4 t + rr % 4 of tile rr / 4, B = queries: column n.  The result gives lane (n, j) the
-//            scores of column n against keys 4 t + r (r = 0..3) of tile j: over t, the 32 keys of ITS tile.
-//   output   A = probabilities: row n, lane group j holds 8 keys of tile j - what the lane already has -, B = V codes: lane (n, j) holds
-//            channel n's 8 keys of tile j.  Codes go from memory to operands with one shift and one mask-or per pair; P never
-//            leaves its lane; no LDS in the loop.
-// Columns.  PACKED (rows <= 16 / NG, decoding): column n = (row n / NG, channel group n % NG), its query zero outside its group: the
-//   NG partial scores of a row land in NG adjacent lanes, each with its own scale, and are summed by DPP; the output's A rows
-//   are (row, group) pairs, of which a column block uses the ones of its group.  One scale per key and lane instead of NG.
-//   Otherwise a column is a row and the groups are separate products.  (Which is faster depends on the rows only: a packed tile holds
-//   16 / NG of them at about half the vector work of a general one with 16.)
+// Layouts.  One wave takes 4 tiles (128 keys) per turn with v_mfma_f32_16x16x32_bf16 (rows of A x columns of B, 32 deep; lane = (n =
+// lane % 16, j = lane / 16) holds 8 elements of A's row n and of B's column n, and results (rows 4 j + r, column n)).
+//   Many rows (kv_attn_kernel: prompts, many query heads to a cache head).  Scores: A = K codes, row rr = key 4 t + rr % 4 of tile rr / 4;
+//     B = queries, column n = a row; the channel groups are separate products.  Lane (n, j) gets row n's scores against the 32 keys of
+//     tile j, which as probabilities are already the A operand of the output, whose B = V codes: P never leaves its lane, no LDS.
+//   Few rows (kv_decode_kernel: at most 16 pairs (row, channel group) - the groups' partial products are columns of their own, so
+//     that a group costs a lane, not an instruction).  Scores: A = queries, row of pair p zero outside its group; B = K codes, column
+//     n = key 8 n + t of the turn: lane (n, j) gets RR = 1, 2 or 4 pairs' scores for 8 keys, a quarter of the vector work of the layout
+//     above where RR is 1 (one query head per cache head up to heads of 128).  Sums over a row's pairs by lane swaps.  The
+//     probabilities go through LDS once (16 bytes per pair and octet of keys) to become A operands.
+//   In both the codes go from memory to operands with one shift and one mask-or per pair.
 // Softmax.  The running maximum of a row moves only when a score passes it by 2^8 (probabilities stay below 256), so that
-//   the usual turn needs no exchange between lanes.
+//   the usual turn needs no exchange between lanes for it.
 // Work.  Four waves per workgroup take turns round robin; the key range is split over workgroups when there are too few of
 //   them to fill 256 CUs (kv_attn_plan), the partial states joined by a second kernel.
 // Bound by HBM: 0.5625 or 1.0625 bytes per cached value.
@@ -28,14 +28,6 @@ namespace bg {
 
 constexpr int KW = 4;                       // waves per workgroup
 constexpr int KV_TURN = 4 * KV_TILE;        // keys a wave takes per turn
-
-// Turn of a wave in steps of TS rows of four keys per tile, so that the codes in flight fit the registers beside the accumulators
-template <typename T, int BITS, int DH, bool PACKED> constexpr int kv_steps() {
-  if (!PACKED) return DH * BITS <= 512 ? 4 : 2;
-  if (DH * BITS <= 256) return 4;
-  if (DH * BITS <= 512) return sizeof(T) == 4 && DH == 128 ? 4 : 8;
-  return DH * BITS <= 1024 && !(sizeof(T) == 4 && DH == 256) ? 4 : 2;
-}
 
 struct KvAttnArgs {
   KvArgs kv;
@@ -123,38 +115,385 @@ template <int N> __device__ __forceinline__ void split_bf16(const float (&x)[8],
   }
 }
 
-template <int CTRL> __device__ __forceinline__ float dpp_add(float x) {
-#pragma clang fp contract(off)          // a fused multiply-add would need the moved value in a register of its own
-  return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, true));
+template <int CTRL> __device__ __forceinline__ float dpp(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, true));
 }
-template <int NG> __device__ __forceinline__ float group_sum(float x) {      // over NG adjacent lanes
-  if constexpr (NG >= 2) x = dpp_add<0xB1>(x);                              // quad_perm 1,0,3,2
-  if constexpr (NG >= 4) x = dpp_add<0x4E>(x);                              // quad_perm 2,3,0,1
-  if constexpr (NG >= 8) x = dpp_add<0x141>(x);                             // row_half_mirror
-  return x;
+// over the 16 lanes n of a lane group, the result in all of them
+__device__ __forceinline__ float sum16(float x) {
+  x += dpp<0xB1>(x);                                     // quad_perm 1,0,3,2 and 2,3,0,1, mirrors of 8 and of 16 lanes
+  x += dpp<0x4E>(x);
+  x += dpp<0x141>(x);
+  return x + dpp<0x140>(x);
+}
+__device__ __forceinline__ float max16(float x) {
+  x = fmaxf(x, dpp<0xB1>(x));
+  x = fmaxf(x, dpp<0x4E>(x));
+  x = fmaxf(x, dpp<0x141>(x));
+  return fmaxf(x, dpp<0x140>(x));
+}
+// over lane groups j, j ^ 1 (and j ^ 2)
+__device__ __forceinline__ float sum_j1(float x) {
+  const auto v = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(v[0]) + __uint_as_float(v[1]);
+}
+__device__ __forceinline__ float sum_j2(float x) {
+  const auto v = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(v[0]) + __uint_as_float(v[1]);
+}
+__device__ __forceinline__ float bf16_at(const uint32_t* w, int i) { return i & 1 ? bf16_hi(w[i / 2]) : bf16_lo(w[i / 2]); }
+
+// Joins the states of the workgroup's waves and writes the rows row0 .. row0 + ROWS - 1, or the split's partial state.
+template <typename T, int DH, int ROWS, typename Shared>
+__device__ __forceinline__ void write_rows(const KvAttnArgs& a, Shared& sh, int b, int h, int row0, int split) {
+  const int R = a.kv.T * a.G;
+  for (int i = threadIdx.x; i < ROWS * DH; i += 64 * KW) {
+    const int row = i / DH, ch = i % DH, rr = row0 + row;
+    if (rr >= R) break;
+    float M = sh.m[0][row];
+#pragma unroll
+    for (int w = 1; w < KW; ++w) M = fmaxf(M, sh.m[w][row]);
+    const float Ms = M == -INFINITY ? 0.f : M;
+    float S = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < KW; ++w) {
+      const float f = __builtin_amdgcn_exp2f(sh.m[w][row] - Ms);
+      S += f * sh.l[w][row];
+      o += f * sh.o[w][row][ch];
+    }
+    if (a.splits == 1) {
+      const int t = rr / a.G, hq = h * a.G + rr - t * a.G;
+      const bool any = a.kv.visible(b, t) > 0;
+      ((T*)a.out)[b * a.o_sb + hq * a.o_sh + t * a.o_st + ch] = from_f32<T>(any ? o / S : 0.f);
+      if (a.lse && ch == 0) a.lse[((int64_t)b * a.kv.H * a.G + hq) * a.kv.T + t] = any ? (M + __log2f(S)) * 0.6931471805599453f : -INFINITY;
+    } else {
+      float* part = a.part + ((((int64_t)b * a.kv.H + h) * R + rr) * a.splits + split) * (DH + 2);
+      part[ch] = o;
+      if (ch == 0) { part[DH] = M; part[DH + 1] = S; }
+    }
+  }
 }
 
-// Waves per SIMD the kernel is built for: four for small heads, whose turns are short and bound by vector work as much as by
-// memory; else two; one (512 registers) where two would spill.
-template <typename T, int BITS, int DH, bool PACKED> constexpr int kv_waves() {
-  if (PACKED) return DH * BITS <= 256 ? (sizeof(T) == 4 && DH == 64 ? 3 : 4) : 2;
-  return DH == 256 || (DH == 128 && BITS == 4) ? 1 : 2;
+// The turns of a split: the first `more` of them take one more than the rest.
+__device__ __forceinline__ void split_turns(const KvAttnArgs& a, int split, int turns, int& begin, int& end) {
+  const int each = (int)((uint32_t)turns / (uint32_t)a.splits), more = turns - each * a.splits;
+  begin = split * each + min(split, more);
+  end = begin + each + (split < more ? 1 : 0);
 }
 
-template <typename T, int BITS, int DH, bool PACKED>
-__global__ __launch_bounds__(64 * KW, (kv_waves<T, BITS, DH, PACKED>())) void kv_attn_kernel(KvAttnArgs a) {
+// ---- few rows --------------------------------------------------------------------------------------------------------------------
+template <typename T, int BITS, int DH, int RR> struct DecodeShape {
+  static constexpr int NG = DH / KV_GROUP, ROWS = 4 * RR / NG, PAIRS = 4 * RR;
+  static constexpr int RL = RR > NG ? RR / NG : 1;                           // rows a lane holds scores of
+  // a turn's codes in flight, K and V: whole (32 registers each at most), halves or quarters
+  static constexpr int KT = DH * BITS <= 512 ? 8 : DH * BITS <= 1024 ? 4 : 2, VT = KT / 2;
+  // waves per SIMD: small heads are bound by vector work and latency as much as by memory
+  static constexpr int WAVES = DH * BITS > 256 || RR == 4 ? 2 : DH * BITS == 256 && sizeof(T) == 4 ? 3 : 4;
+};
+
+template <typename T, int BITS, int DH, int RR>
+__global__ __launch_bounds__(64 * KW, (DecodeShape<T, BITS, DH, RR>::WAVES)) void kv_decode_kernel(KvAttnArgs a) {
   using L = KvTile<BITS, DH>;
-  constexpr int NG = L::NG, TS = kv_steps<T, BITS, DH, PACKED>(), NO = TS / 2, CB = DH / 16;
-  constexpr int ROWS = PACKED ? 16 / NG : 16, GL = PACKED ? 1 : NG;         // rows per tile; groups whose scales a lane needs
+  using D = DecodeShape<T, BITS, DH, RR>;
+  constexpr int NG = L::NG, CB = DH / 16, RL = D::RL, KT = D::KT, VT = D::VT, KP = 8 / KT, VP = 4 / VT;
   constexpr int NQ = sizeof(T) == 4 ? 3 : 1, NP = sizeof(T) == 4 ? 3 : 2;   // bf16 pieces of queries / probabilities
   constexpr float OFFT = kv_offset<BITS>();
-  constexpr bool OWN_Q = PACKED && NG * NQ > 4;     // keep a lane's one group only, and the zeros of the others as a select per use
-  constexpr bool LDS_Q = !PACKED && NG * NQ > 8;    // the pieces of long fp32 rows live in LDS
-  constexpr int NQF = OWN_Q || LDS_Q ? 1 : NG;
+  constexpr bool OWN_Q = NG * NQ > 4;               // keep a lane's one group only, and the zeros of the others as a select per use
   constexpr int KWORDS = NG * L::WORD / 4, VWORDS = CB * L::WORD / 4;
-  __shared__ float sh_o[KW][ROWS][DH];
-  __shared__ float sh_m[KW][16], sh_l[KW][16];
-  __shared__ bf16x8 sh_q[LDS_Q ? NG : 1][NQ][LDS_Q ? 64 : 1];
+  struct Shared {
+    float o[KW][D::ROWS][DH];
+    float m[KW][D::ROWS], l[KW][D::ROWS];
+    bf16x8 p[KW][NP][D::PAIRS][16];
+  };
+  __shared__ Shared sh;
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, j = lane >> 4;
+  const int b = blockIdx.z, h = blockIdx.y, split = blockIdx.x;
+  const int R = a.kv.T * a.G;
+  const uint8_t* base = a.kv.data + b * a.kv.c_sb + h * a.kv.c_sh;
+  const int last_tile = (a.kv.capacity - 1) / KV_TILE;
+
+  // pairs p = row NG + group.  As a query operand lane n's row holds pair n / 4 RR + n % 4 (none for n % 4 >= RR): the scores of that
+  // matrix row, 4 j + r, come out in register r of lane group j, which so gets the pairs j RR + r.
+  const int q_pair = (n >> 2) * RR + (n & 3), q_row = q_pair / NG, q_g = q_pair % NG;
+  const bool q_real = (n & 3) < RR && q_row < R;
+  int pair_g[RR], row_vis[RL];
+#pragma unroll
+  for (int r = 0; r < RR; ++r) pair_g[r] = (j * RR + r) % NG;
+
+  uint32_t kw[KT][KWORDS], ks[RR][4], vw[VT][VWORDS], vs[RR][4];
+  int t_begin = 0;
+  const auto tile_at = [&](int turn, int i) __attribute__((always_inline)) -> const uint8_t* {
+    return base + (int64_t)min(4 * turn + i, last_tile) * L::BYTES;
+  };
+  const auto load_k = [&](int turn, int piece) __attribute__((always_inline)) {
+    const uint8_t* t = tile_at(turn, n >> 2);
+#pragma unroll
+    for (int i = 0; i < KT; ++i) load_words<KWORDS>(t + (8 * (n & 3) + piece * KT + i) * L::KROW + j * NG * L::WORD, kw[i]);
+    if (piece == 0) {
+#pragma unroll
+      for (int r = 0; r < RR; ++r) load_words<4>(t + L::KS + L::scale_at(8 * (n & 3), pair_g[r]), ks[r]);
+    }
+  };
+  const auto load_v = [&](int turn, int piece) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < VT; ++i) load_words<VWORDS>(tile_at(turn, piece * VT + i) + L::V + (j * 16 + n) * CB * L::WORD, vw[i]);
+    if (piece == 0) {
+#pragma unroll
+      for (int r = 0; r < RR; ++r) load_words<4>(tile_at(turn, n >> 2) + L::VS + L::scale_at(8 * (n & 3), pair_g[r]), vs[r]);
+    }
+  };
+  // with the whole key range in this workgroup the first turn's place is known before the sequence's length is
+  if (a.splits == 1) load_k(wave, 0);
+
+  bf16x8 qf[OWN_Q ? 1 : NG][NQ];
+  float q0[RR];                                                              // what the offset of the codes adds to a score
+  {
+    const int t_row = a.kv.T > 1 ? (int)((uint32_t)q_row / (uint32_t)a.G) : 0, g_row = q_row - t_row * a.G;
+    const T* q = (const T*)a.q + b * a.q_sb + (int64_t)(h * a.G + g_row) * a.q_sh + (int64_t)t_row * a.q_st + 32 * q_g + 8 * j;
+    float x[8], sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float v = q_real ? to_f32(q[e]) : 0.f;
+      x[e] = a.negate ? -v : v;
+      sum += x[e];
+    }
+    bf16x8 piece[NQ];
+    split_bf16<NQ>(x, piece);
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      if constexpr (OWN_Q) {
+        qf[0][i] = piece[i];
+      } else {
+        const Frag own = {.v = piece[i]};
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          Frag f;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) f.u[w] = g == q_g ? own.u[w] : 0u;
+          qf[g][i] = f.v;
+        }
+      }
+    }
+    sum = -OFFT * sum_j2(sum_j1(sum));
+#pragma unroll
+    for (int r = 0; r < RR; ++r) q0[r] = __shfl(sum, 4 * j + r);
+  }
+
+  int n_min;
+  const int n_max = tile_keys(a, b, 0, n_min);
+#pragma unroll
+  for (int i = 0; i < RL; ++i) {
+    const int row = j * RR / NG + i;
+    row_vis[i] = row < R ? min(a.kv.visible(b, a.kv.T > 1 ? row / a.G : 0), a.max_keys) : 0x7FFFFFFF;
+  }
+  const int turns = (n_max + KV_TURN - 1) / KV_TURN;
+  int t_end;
+  split_turns(a, split, turns, t_begin, t_end);
+  if (a.splits > 1 && t_begin + wave < t_end) load_k(t_begin + wave, 0);
+
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  f32x4 acc[CB], off = zero;
+#pragma unroll
+  for (int c = 0; c < CB; ++c) acc[c] = zero;
+  float mc[RL], l[RL];                                                       // maximum in log2 units, this lane's share of the sum
+#pragma unroll
+  for (int i = 0; i < RL; ++i) { mc[i] = -INFINITY; l[i] = 0.f; }
+  Frag ones;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ones.v[i] = (bf16_t)OFFT;
+  const Nibbles nb;
+
+  for (int turn = t_begin + wave; turn < t_end; turn += KW) {
+    const bool more = turn + KW < t_end;
+    load_v(turn, 0);
+    // scores of this lane's rows against keys 8 n + t
+    float s[8][RL];
+#pragma unroll
+    for (int kp = 0; kp < KP; ++kp) {
+      f32x4 d[KT];
+#pragma unroll
+      for (int i = 0; i < KT; ++i) {
+        d[i] = zero;
+#pragma unroll
+        for (int r = 0; r < RR; ++r) d[i][r] = q0[r];
+      }
+      int own_g = q_g;
+      if constexpr (OWN_Q) asm volatile("" : "+v"(own_g));    // the selects stay in the loop: ahead of it they would take NG times the registers
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        bf16x8 qg[NQ];
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+          if constexpr (OWN_Q) {
+            const Frag own = {.v = qf[0][i]};
+            Frag f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) f.u[w] = g == own_g ? own.u[w] : 0u;
+            qg[i] = f.v;
+          } else {
+            qg[i] = qf[g][i];
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < KT; ++i) {
+          const bf16x8 kf = unpack_codes<BITS>(&kw[i][g * L::WORD / 4], nb);
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) d[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qg[q], kf, d[i], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < KT; ++i) {
+        const int t = kp * KT + i;
+        float v[RR];
+#pragma unroll
+        for (int r = 0; r < RR; ++r) v[r] = d[i][r] * bf16_at(ks[r], t);
+#pragma unroll
+        for (int rl = 0; rl < RL; ++rl) {
+          float x = v[rl * NG < RR ? rl * NG : 0];
+#pragma unroll
+          for (int g = 1; g < (NG < RR ? NG : RR); ++g) x += v[rl * NG + g];
+          if constexpr (NG >= 2 * RR) x = sum_j1(x);
+          if constexpr (NG >= 4 * RR) x = sum_j2(x);
+          s[t][rl] = x;
+        }
+      }
+      if (kp + 1 < KP) load_k(turn, kp + 1);
+    }
+    if (more) load_k(turn + KW, 0);
+
+    const int key0 = turn * KV_TURN + 8 * n;
+    const bool partial = turn * KV_TURN + KV_TURN > n_min;                   // some row does not see all of this turn
+    if (partial) {
+#pragma unroll
+      for (int t = 0; t < 8; ++t)
+#pragma unroll
+        for (int rl = 0; rl < RL; ++rl) s[t][rl] = key0 + t < row_vis[rl] ? s[t][rl] : -INFINITY;
+    }
+    float top[RL];
+    bool past = turn == t_begin + wave;
+#pragma unroll
+    for (int rl = 0; rl < RL; ++rl) {
+      top[rl] = s[0][rl];
+#pragma unroll
+      for (int t = 1; t < 8; ++t) top[rl] = fmaxf(top[rl], s[t][rl]);
+      top[rl] *= a.scale_log2;
+      past = past || top[rl] > mc[rl] + 8.f;
+    }
+    if (__any(past)) {
+      float keep[RL];
+#pragma unroll
+      for (int rl = 0; rl < RL; ++rl) {
+        const float m_new = fmaxf(mc[rl], max16(top[rl]));
+        keep[rl] = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mc[rl] - m_new);
+        mc[rl] = m_new;
+        l[rl] *= keep[rl];
+      }
+      float f[4];                                                            // of the accumulators' rows, pairs 4 j + r
+#pragma unroll
+      for (int r = 0; r < 4; ++r) f[r] = __shfl(keep[RL > 1 ? r % RR / NG : 0], 16 * (((4 * j + r) / RR) & 3));
+#pragma unroll
+      for (int c = 0; c < CB; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[c][r] *= f[r];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) off[r] *= f[r];
+    }
+    float p[8][RL];
+#pragma unroll
+    for (int rl = 0; rl < RL; ++rl) {
+      const float ms = mc[rl] == -INFINITY ? 0.f : mc[rl];
+#pragma unroll
+      for (int t = 0; t < 8; ++t) p[t][rl] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][rl], a.scale_log2, -ms));
+    }
+    if (partial) {                                                           // keys not seen: no weight
+#pragma unroll
+      for (int t = 0; t < 8; ++t)
+#pragma unroll
+        for (int rl = 0; rl < RL; ++rl) p[t][rl] = key0 + t < row_vis[rl] ? p[t][rl] : 0.f;
+    }
+#pragma unroll
+    for (int rl = 0; rl < RL; ++rl)
+#pragma unroll
+      for (int t = 0; t < 8; t += 2) l[rl] += p[t][rl] + p[t + 1][rl];
+    // probabilities times scales, octet n of pair j RR + r
+#pragma unroll
+    for (int r = 0; r < RR; ++r) {
+      const int rl = RL > 1 ? r / NG : 0;
+      float x[8];
+#pragma unroll
+      for (int t = 0; t < 8; ++t) x[t] = p[t][rl] * bf16_at(vs[r], t);
+      if (partial) {                                                         // whose scale may be anything
+#pragma unroll
+        for (int t = 0; t < 8; ++t) x[t] = key0 + t < row_vis[rl] ? x[t] : 0.f;
+      }
+      bf16x8 piece[NP];
+      split_bf16<NP>(x, piece);
+#pragma unroll
+      for (int i = 0; i < NP; ++i) sh.p[wave][i][j * RR + r][n] = piece[i];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    // output: row n of A is pair n (rows past the pairs repeat them and are not used), octets 4 tile + j
+#pragma unroll
+    for (int vp = 0; vp < VP; ++vp) {
+#pragma unroll
+      for (int i = 0; i < VT; ++i) {
+        bf16x8 pf[NP];
+#pragma unroll
+        for (int q = 0; q < NP; ++q) pf[q] = sh.p[wave][q][n & (D::PAIRS - 1)][4 * (vp * VT + i) + j];
+        if constexpr (OFFT != 0.f) {
+#pragma unroll
+          for (int q = 0; q < NP; ++q) off = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf[q], ones.v, off, 0, 0, 0);
+        }
+#pragma unroll
+        for (int c = 0; c < CB; ++c) {
+          const bf16x8 vf = unpack_codes<BITS>(&vw[i][c * L::WORD / 4], nb);
+#pragma unroll
+          for (int q = 0; q < NP; ++q) acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf[q], vf, acc[c], 0, 0, 0);
+        }
+      }
+      if (vp + 1 < VP) load_v(turn, vp + 1);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");                    // the next turn's probabilities overwrite these
+    __builtin_amdgcn_wave_barrier();
+  }
+
+#pragma unroll
+  for (int rl = 0; rl < RL; ++rl) {
+    const float sum = sum16(l[rl]);
+    if (n == 0 && j * RR % NG == 0) { sh.m[wave][j * RR / NG + rl] = mc[rl]; sh.l[wave][j * RR / NG + rl] = sum; }
+  }
+#pragma unroll
+  for (int c = 0; c < CB; ++c)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int p = 4 * j + r;
+      if (p < D::PAIRS && p % NG == c / 2) sh.o[wave][p / NG][16 * c + n] = acc[c][r] - off[r];
+    }
+  __syncthreads();
+  write_rows<T, DH, D::ROWS>(a, sh, b, h, 0, split);
+}
+
+// ---- many rows -------------------------------------------------------------------------------------------------------------------
+// steps of a turn, so that the codes in flight fit the registers beside the accumulators; waves per SIMD: one where two would spill
+template <int BITS, int DH> constexpr int kv_steps() { return DH * BITS <= 512 ? 4 : 2; }
+template <int BITS, int DH> constexpr int kv_waves() { return DH == 256 || (DH == 128 && BITS == 4) ? 1 : 2; }
+
+template <typename T, int BITS, int DH>
+__global__ __launch_bounds__(64 * KW, (kv_waves<BITS, DH>())) void kv_attn_kernel(KvAttnArgs a) {
+  using L = KvTile<BITS, DH>;
+  constexpr int NG = L::NG, TS = kv_steps<BITS, DH>(), NO = TS / 2, CB = DH / 16, ROWS = 16;
+  constexpr int NQ = sizeof(T) == 4 ? 3 : 1, NP = sizeof(T) == 4 ? 3 : 2;   // bf16 pieces of queries / probabilities
+  constexpr float OFFT = kv_offset<BITS>();
+  constexpr bool LDS_Q = NG * NQ > 8;                                        // the pieces of long fp32 rows live in LDS
+  constexpr int KWORDS = NG * L::WORD / 4, VWORDS = CB * L::WORD / 4;
+  struct Shared {
+    float o[KW][ROWS][DH];
+    float m[KW][ROWS], l[KW][ROWS];
+    bf16x8 q[LDS_Q ? NG : 1][NQ][LDS_Q ? 64 : 1];
+  };
+  __shared__ Shared sh;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, j = lane >> 4;
   const int b = blockIdx.z, h = blockIdx.y;
@@ -165,15 +504,11 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<T, BITS, DH, PACKED>())) void kv
   constexpr int SUB = 8 / TS;                                                // steps of a turn
 
   // this lane's column: its row
-  const int rho = row0 + (PACKED ? n / NG : n), my_g = PACKED ? n % NG : 0;
+  const int rho = row0 + n;
   const bool real = rho < R;
-  int t_row = 0, g_row = rho;                                                // rho = t_row G + g_row
-  if (a.kv.T > 1) {
-    t_row = (int)((uint32_t)rho / (uint32_t)a.G);
-    g_row = rho - t_row * a.G;
-  }
+  const int t_row = (int)((uint32_t)rho / (uint32_t)a.G), g_row = rho - t_row * a.G;
 
-  uint32_t kw[TS][KWORDS], ks[GL][TS * 2], vw[NO][VWORDS], vs[GL][TS * 2];
+  uint32_t kw[TS][KWORDS], ks[NG][TS * 2], vw[NO][VWORDS], vs[NG][TS * 2];
   int t_begin = 0;
   auto key_base = [&](int step, int tile_in_turn) __attribute__((always_inline)) -> const uint8_t* {
     const int tile = (t_begin + wave + KW * (step / SUB)) * 4 + tile_in_turn;
@@ -186,7 +521,7 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<T, BITS, DH, PACKED>())) void kv
     for (int t = 0; t < TS; ++t) load_words<KWORDS>(kt + (4 * (s * TS + t) + (n & 3)) * L::KROW + j * NG * L::WORD, kw[t]);
     const uint8_t* st = key_base(step, j) + L::KS + s * TS * 8;
 #pragma unroll
-    for (int g = 0; g < GL; ++g) load_words<TS * 2>(st + (PACKED ? my_g : g) * KV_TILE * 2, ks[g]);
+    for (int g = 0; g < NG; ++g) load_words<TS * 2>(st + g * KV_TILE * 2, ks[g]);
   };
   auto load_v = [&](int step) __attribute__((always_inline)) {
     const int s = step % SUB;
@@ -194,22 +529,22 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<T, BITS, DH, PACKED>())) void kv
 #pragma unroll
     for (int o = 0; o < NO; ++o) load_words<VWORDS>(vt + L::V + ((s * NO + o) * 16 + n) * CB * L::WORD, vw[o]);
 #pragma unroll
-    for (int g = 0; g < GL; ++g) load_words<TS * 2>(vt + L::VS + s * TS * 8 + (PACKED ? my_g : g) * KV_TILE * 2, vs[g]);
+    for (int g = 0; g < NG; ++g) load_words<TS * 2>(vt + L::VS + s * TS * 8 + g * KV_TILE * 2, vs[g]);
   };
   // with the whole key range in this workgroup the first turn's place is known before the sequence's length is
   if (a.splits == 1) load_k(0);
 
   // queries: B operand of step g = channels 32 g + 8 j + 0..7 of column n's row
-  bf16x8 qf[NQF][NQ];
-  float q0[GL];                                                              // what the offset of the codes adds to a score
+  bf16x8 qf[LDS_Q ? 1 : NG][NQ];
+  float q0[NG];                                                              // what the offset of the codes adds to a score
   {
     const T* q = (const T*)a.q + b * a.q_sb + (int64_t)(h * a.G + g_row) * a.q_sh + (int64_t)t_row * a.q_st + 8 * j;
 #pragma unroll
-    for (int g = 0; g < (PACKED ? 1 : NG); ++g) {
+    for (int g = 0; g < NG; ++g) {
       float x[8], sum = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float v = real ? to_f32(q[32 * (PACKED ? my_g : g) + e]) : 0.f;
+        const float v = real ? to_f32(q[32 * g + e]) : 0.f;
         x[e] = a.negate ? -v : v;
         sum += x[e];
       }
@@ -217,59 +552,34 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<T, BITS, DH, PACKED>())) void kv
       split_bf16<NQ>(x, piece);
 #pragma unroll
       for (int i = 0; i < NQ; ++i) {
-        if constexpr (LDS_Q) sh_q[g][i][lane] = piece[i];                    // the four waves write the same values
+        if constexpr (LDS_Q) sh.q[g][i][lane] = piece[i];                    // the four waves write the same values
         else qf[g][i] = piece[i];
       }
-      sum += __shfl_xor(sum, 16);
-      sum += __shfl_xor(sum, 32);
-      q0[g] = -OFFT * sum;
-    }
-    if constexpr (PACKED && !OWN_Q) {
-#pragma unroll
-      for (int i = 0; i < NQ; ++i) {
-        const Frag own = {.v = qf[0][i]};
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          Frag f;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) f.u[w] = g == my_g ? own.u[w] : 0u;
-          qf[g][i] = f.v;
-        }
-      }
+      q0[g] = -OFFT * sum_j2(sum_j1(sum));
     }
   }
   if constexpr (LDS_Q) __syncthreads();
-  auto query = [&](int g, int i, int own_g) __attribute__((always_inline)) -> bf16x8 {
-    if constexpr (LDS_Q) return sh_q[g][i][lane];
-    if constexpr (!OWN_Q) return qf[g][i];
-    const Frag own = {.v = qf[0][i]};
-    Frag f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) f.u[w] = g == own_g ? own.u[w] : 0u;
-    return f.v;
-  };
 
   // what the rows of this tile see: all of them at least n_min keys, none more than n_max
   int n_min;
   const int n_max = tile_keys(a, b, row0, n_min);
   const int vis = real ? min(a.kv.visible(b, t_row), a.max_keys) : 0x7FFFFFFF;
 
-  f32x4 acc[CB], off = {0.f, 0.f, 0.f, 0.f};                                 // PACKED: one offset sum; else one per group
-  f32x4 offg[PACKED ? 1 : NG];
+  f32x4 acc[CB], offg[NG];
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int c = 0; c < CB; ++c) acc[c] = off;
+  for (int c = 0; c < CB; ++c) acc[c] = zero;
 #pragma unroll
-  for (int g = 0; g < (PACKED ? 1 : NG); ++g) offg[g] = off;
+  for (int g = 0; g < NG; ++g) offg[g] = zero;
   float mc = -INFINITY, l = 0.f;                                             // maximum in log2 units, this lane's share of the sum
   Frag ones;
 #pragma unroll
   for (int i = 0; i < 8; ++i) ones.v[i] = (bf16_t)OFFT;
-
   const Nibbles nb;
+
   const int turns = (n_max + KV_TURN - 1) / KV_TURN;
-  const int each = (int)((uint32_t)turns / (uint32_t)a.splits), more = turns - each * a.splits;        // the first `more` splits take one more
-  t_begin = split * each + min(split, more);
-  const int t_end = t_begin + each + (split < more ? 1 : 0);
+  int t_end;
+  split_turns(a, split, turns, t_begin, t_end);
   const int my_turns = t_end - t_begin > wave ? (t_end - t_begin - wave + KW - 1) / KW : 0;
   const int steps = my_turns * SUB;
   if (a.splits > 1 && steps > 0) load_k(0);
@@ -277,51 +587,26 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<T, BITS, DH, PACKED>())) void kv
     load_v(step);
     // scores
     f32x4 sc[TS];
-    int own_g = my_g;
-    if constexpr (OWN_Q) asm volatile("" : "+v"(own_g));      // the selects stay in the loop: ahead of it they would take NG times the registers
 #pragma unroll
-    for (int t = 0; t < TS; ++t) sc[t] = PACKED ? f32x4{q0[0], q0[0], q0[0], q0[0]} : f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < TS; ++t) sc[t] = zero;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       bf16x8 qg[NQ];
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) qg[i] = query(g, i, own_g);
+      for (int i = 0; i < NQ; ++i) {
+        if constexpr (LDS_Q) qg[i] = sh.q[g][i][lane];
+        else qg[i] = qf[g][i];
+      }
 #pragma unroll
       for (int t = 0; t < TS; ++t) {
         const bf16x8 kf = unpack_codes<BITS>(&kw[t][g * L::WORD / 4], nb);
-        if constexpr (PACKED) {
+        f32x4 d = {q0[g], q0[g], q0[g], q0[g]};
 #pragma unroll
-          for (int i = 0; i < NQ; ++i) sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qg[i], sc[t], 0, 0, 0);
-        } else {
-          f32x4 d = {q0[g], q0[g], q0[g], q0[g]};
+        for (int i = 0; i < NQ; ++i) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qg[i], d, 0, 0, 0);
 #pragma unroll
-          for (int i = 0; i < NQ; ++i) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qg[i], d, 0, 0, 0);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float k_scale = r & 1 ? bf16_hi(ks[g][2 * t + r / 2]) : bf16_lo(ks[g][2 * t + r / 2]);
-            sc[t][r] = __builtin_fmaf(d[r], k_scale, sc[t][r]);
-          }
-        }
+        for (int r = 0; r < 4; ++r) sc[t][r] = __builtin_fmaf(d[r], bf16_at(ks[g], 4 * t + r), sc[t][r]);
       }
     }
-    if constexpr (PACKED) {
-#pragma unroll
-      for (int t = 0; t < TS; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float k_scale = r & 1 ? bf16_hi(ks[0][2 * t + r / 2]) : bf16_lo(ks[0][2 * t + r / 2]);
-          sc[t][r] = group_sum<NG>(sc[t][r] * k_scale);
-        }
-    }
-    // (the sums stay in this block: moved behind the branch below, an add and the lane exchange that feeds it are two instructions)
-#pragma unroll
-    for (int t = 0; t < TS; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float v = sc[t][r];
-        asm volatile("" : "+v"(v));
-        sc[t][r] = v;
-      }
     if (step + 1 < steps) load_k(step + 1);
     // keys of this lane: key0 + 4 t + r
     const int turn0 = (t_begin + wave + KW * (step / SUB)) * KV_TURN;
@@ -354,7 +639,7 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<T, BITS, DH, PACKED>())) void kv
 #pragma unroll
         for (int r = 0; r < 4; ++r) acc[c][r] *= f[r];
 #pragma unroll
-      for (int g = 0; g < (PACKED ? 1 : NG); ++g)
+      for (int g = 0; g < NG; ++g)
 #pragma unroll
         for (int r = 0; r < 4; ++r) offg[g][r] *= f[r];
     }
@@ -373,7 +658,7 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<T, BITS, DH, PACKED>())) void kv
           p[t][r] = seen ? p[t][r] : 0.f;
           if (!seen) {
 #pragma unroll
-            for (int g = 0; g < GL; ++g) vs[g][2 * t + r / 2] &= r & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+            for (int g = 0; g < NG; ++g) vs[g][2 * t + r / 2] &= r & 1 ? 0x0000FFFFu : 0xFFFF0000u;
           }
         }
     }
@@ -382,66 +667,36 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<T, BITS, DH, PACKED>())) void kv
     // output
 #pragma unroll
     for (int o = 0; o < NO; ++o) {
-      bf16x8 pf[GL][NP];
+      bf16x8 pf[NG][NP];
 #pragma unroll
-      for (int g = 0; g < GL; ++g) {
+      for (int g = 0; g < NG; ++g) {
         float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t w = vs[g][4 * o + e / 2];
-          x[e] = p[2 * o + e / 4][e % 4] * (e & 1 ? bf16_hi(w) : bf16_lo(w));
-        }
+        for (int e = 0; e < 8; ++e) x[e] = p[2 * o + e / 4][e % 4] * bf16_at(vs[g], 8 * o + e);
         split_bf16<NP>(x, pf[g]);
+        if constexpr (OFFT != 0.f) {
 #pragma unroll
-        for (int i = 0; i < NP && OFFT != 0.f; ++i) offg[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf[g][i], ones.v, offg[g], 0, 0, 0);
+          for (int i = 0; i < NP; ++i) offg[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf[g][i], ones.v, offg[g], 0, 0, 0);
+        }
       }
 #pragma unroll
       for (int c = 0; c < CB; ++c) {
         const bf16x8 vf = unpack_codes<BITS>(&vw[o][c * L::WORD / 4], nb);
 #pragma unroll
-        for (int i = 0; i < NP; ++i) acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf[PACKED ? 0 : c / 2][i], vf, acc[c], 0, 0, 0);
+        for (int i = 0; i < NP; ++i) acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf[c / 2][i], vf, acc[c], 0, 0, 0);
       }
     }
   }
 
   // this wave's state -> LDS (accumulator row 4 j + r, channel 16 c + n)
-  l += __shfl_xor(l, 16);
-  l += __shfl_xor(l, 32);
-  if (j == 0 && my_g == 0) { sh_m[wave][rho - row0] = mc; sh_l[wave][rho - row0] = l; }
+  l = sum_j2(sum_j1(l));
+  if (j == 0) { sh.m[wave][n] = mc; sh.l[wave][n] = l; }
 #pragma unroll
   for (int c = 0; c < CB; ++c)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int ar = 4 * j + r;
-      if (PACKED && ar % NG != c / 2) continue;
-      sh_o[wave][PACKED ? ar / NG : ar][16 * c + n] = acc[c][r] - offg[PACKED ? 0 : c / 2][r];
-    }
+    for (int r = 0; r < 4; ++r) sh.o[wave][4 * j + r][16 * c + n] = acc[c][r] - offg[c / 2][r];
   __syncthreads();
-  for (int i = tid; i < ROWS * DH; i += 64 * KW) {
-    const int row = i / DH, ch = i % DH, rr = row0 + row;
-    if (rr >= R) break;
-    float M = sh_m[0][row];
-#pragma unroll
-    for (int w = 1; w < KW; ++w) M = fmaxf(M, sh_m[w][row]);
-    const float Ms = M == -INFINITY ? 0.f : M;
-    float S = 0.f, o = 0.f;
-#pragma unroll
-    for (int w = 0; w < KW; ++w) {
-      const float f = __builtin_amdgcn_exp2f(sh_m[w][row] - Ms);
-      S += f * sh_l[w][row];
-      o += f * sh_o[w][row][ch];
-    }
-    const int t = rr / a.G, hq = h * a.G + rr % a.G;
-    if (a.splits == 1) {
-      const bool any = a.kv.visible(b, t) > 0;
-      ((T*)a.out)[b * a.o_sb + hq * a.o_sh + t * a.o_st + ch] = from_f32<T>(any ? o / S : 0.f);
-      if (a.lse && ch == 0) a.lse[((int64_t)b * a.kv.H * a.G + hq) * a.kv.T + t] = any ? (M + __log2f(S)) * 0.6931471805599453f : -INFINITY;
-    } else {
-      float* part = a.part + ((((int64_t)b * a.kv.H + h) * R + rr) * a.splits + split) * (DH + 2);
-      part[ch] = o;
-      if (ch == 0) { part[DH] = M; part[DH + 1] = S; }
-    }
-  }
+  write_rows<T, DH, ROWS>(a, sh, b, h, row0, split);
 }
 
 // Joins the splits of a row: one wave per row, the states of eight splits under way together.
@@ -491,19 +746,18 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(KvAttnArgs a, uint32_
   if (a.lse && lane == 0) a.lse[((int64_t)b * a.kv.H * a.G + hq) * a.kv.T + t] = any ? (M + __log2f(S)) * 0.6931471805599453f : -INFINITY;
 }
 
-// How many workgroups share a row tile's key range: enough to give every CU two (512), none with less than one turn for each wave.
-// (Even splits of every sequence: splits of a fixed number of turns, fewer for short sequences, leave CUs idle - 16 uneven sequences
-// of 8 heads, 8 bits, 67 against 79 us.)
+// Which kernel, and how many workgroups share a row tile's key range: enough to give every CU two (512), none with less than one turn for
+// each wave.  (Even splits of every sequence: splits of a fixed number of turns, fewer for short sequences, leave CUs idle - 16
+// uneven sequences of 8 heads, 8 bits, 67 against 79 us.)
 struct KvPlan {
-  bool packed;
+  int pairs;                                 // (row, channel group) pairs per cache head; more than 16: kv_attn_kernel
   int row_tiles, splits;
 };
 static KvPlan kv_attn_plan(const bg_kv_cache* c, int Hq, int T, int max_keys) {
   KvPlan p;
-  const int64_t R = (int64_t)T * (Hq / c->H);
-  const int ng = c->Dh / KV_GROUP;
-  p.packed = R <= 16 / ng;
-  p.row_tiles = (int)cdiv(R, p.packed ? 16 / ng : 16);
+  const int64_t R = (int64_t)T * (Hq / c->H), pairs = R * (c->Dh / KV_GROUP);
+  p.pairs = pairs > 16 ? 17 : (int)pairs;
+  p.row_tiles = pairs > 16 ? (int)cdiv(R, 16) : 1;
   const int64_t base = (int64_t)c->B * c->H * p.row_tiles;
   const int64_t most = cdiv(max_keys, KV_TURN * KW), want = cdiv(512, base);
   p.splits = (int)(want < most ? want : most);
@@ -522,9 +776,11 @@ extern "C" size_t bg_kv_cache_attn_workspace_bytes(const bg_kv_cache* cache, int
 
 template <typename T, int BITS, int DH>
 static void kv_attn_launch(const KvAttnArgs& a, const KvPlan& p, hipStream_t st) {
-  const dim3 grid((unsigned)(p.row_tiles * p.splits), (unsigned)a.kv.H, (unsigned)a.kv.B);
-  if (p.packed) hipLaunchKernelGGL((kv_attn_kernel<T, BITS, DH, true>), grid, dim3(64 * KW), 0, st, a);
-  else hipLaunchKernelGGL((kv_attn_kernel<T, BITS, DH, false>), grid, dim3(64 * KW), 0, st, a);
+  const dim3 grid((unsigned)(p.row_tiles * p.splits), (unsigned)a.kv.H, (unsigned)a.kv.B), block(64 * KW);
+  if (p.pairs > 16) hipLaunchKernelGGL((kv_attn_kernel<T, BITS, DH>), grid, block, 0, st, a);
+  else if (p.pairs > 8) hipLaunchKernelGGL((kv_decode_kernel<T, BITS, DH, 4>), grid, block, 0, st, a);
+  else if (DH == 256 || p.pairs > 4) hipLaunchKernelGGL((kv_decode_kernel<T, BITS, DH, 2>), grid, block, 0, st, a);
+  else if constexpr (DH < 256) hipLaunchKernelGGL((kv_decode_kernel<T, BITS, DH, 1>), grid, block, 0, st, a);
   if (p.splits > 1) {
     const uint32_t rows = (uint32_t)(a.kv.B * a.kv.H) * (uint32_t)(a.kv.T * a.G);
     hipLaunchKernelGGL((kv_attn_join_kernel<T, DH>), dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, st, a, rows);
@@ -558,7 +814,7 @@ extern "C" int bg_kv_cache_attn_fwd(const bg_kv_cache* cache, const void* data, 
   a.out = out; a.o_sb = o_sb; a.o_sh = o_sh; a.o_st = o_st;
   a.lse = lse; a.part = (float*)workspace;
   a.G = Hq / cache->H; a.max_keys = max_keys; a.splits = p.splits;
-  a.rows_per_tile = p.packed ? 16 / (cache->Dh / KV_GROUP) : 16;
+  a.rows_per_tile = p.pairs > 16 ? 16 : T * a.G;
   a.negate = scale < 0.f;
   a.scale_log2 = (float)((scale < 0.f ? -(double)scale : (double)scale) * 1.4426950408889634);
   hipStream_t st = (hipStream_t)stream;
