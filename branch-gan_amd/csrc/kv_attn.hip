@@ -184,8 +184,8 @@ __device__ __forceinline__ void split_turns(const KvAttnArgs& a, int split, int 
 template <typename T, int BITS, int DH, int RR> struct DecodeShape {
   static constexpr int NG = DH / KV_GROUP, ROWS = 4 * RR / NG, PAIRS = 4 * RR;
   static constexpr int RL = RR > NG ? RR / NG : 1;                           // rows a lane holds scores of
-  // a turn's codes in flight, K and V: whole (32 registers each at most), halves or quarters
-  static constexpr int KT = DH * BITS <= 512 ? 8 : DH * BITS <= 1024 ? 4 : 2, VT = KT / 2;
+  // a turn's codes in flight, K and V: whole (16 registers each at most), halves or quarters
+  static constexpr int KT = DH * BITS <= 256 ? 8 : DH * BITS <= 1024 ? 4 : 2, VT = KT / 2;
   // waves per SIMD: small heads are bound by vector work and latency as much as by memory
   static constexpr int WAVES = DH * BITS > 256 || RR == 4 ? 2 : DH * BITS == 256 && sizeof(T) == 4 ? 3 : 4;
 };
@@ -194,7 +194,7 @@ template <typename T, int BITS, int DH, int RR>
 __global__ __launch_bounds__(64 * KW, (DecodeShape<T, BITS, DH, RR>::WAVES)) void kv_decode_kernel(KvAttnArgs a) {
   using L = KvTile<BITS, DH>;
   using D = DecodeShape<T, BITS, DH, RR>;
-  constexpr int NG = L::NG, CB = DH / 16, RL = D::RL, KT = D::KT, VT = D::VT, KP = 8 / KT, VP = 4 / VT;
+  constexpr int NG = L::NG, CB = DH / 16, RL = D::RL, KT = D::KT, VT = D::VT, KP = 8 / KT;
   constexpr int NQ = sizeof(T) == 4 ? 3 : 1, NP = sizeof(T) == 4 ? 3 : 2;   // bf16 pieces of queries / probabilities
   constexpr float OFFT = kv_offset<BITS>();
   constexpr bool OWN_Q = NG * NQ > 4;               // keep a lane's one group only, and the zeros of the others as a select per use
@@ -237,10 +237,10 @@ __global__ __launch_bounds__(64 * KW, (DecodeShape<T, BITS, DH, RR>::WAVES)) voi
   const auto load_v = [&](int turn, int piece) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < VT; ++i) load_words<VWORDS>(tile_at(turn, piece * VT + i) + L::V + (j * 16 + n) * CB * L::WORD, vw[i]);
-    if (piece == 0) {
+  };
+  const auto load_v_scales = [&](int turn) __attribute__((always_inline)) {
 #pragma unroll
-      for (int r = 0; r < RR; ++r) load_words<4>(tile_at(turn, n >> 2) + L::VS + L::scale_at(8 * (n & 3), pair_g[r]), vs[r]);
-    }
+    for (int r = 0; r < RR; ++r) load_words<4>(tile_at(turn, n >> 2) + L::VS + L::scale_at(8 * (n & 3), pair_g[r]), vs[r]);
   };
   // with the whole key range in this workgroup the first turn's place is known before the sequence's length is
   if (a.splits == 1) load_k(wave, 0);
@@ -303,64 +303,59 @@ __global__ __launch_bounds__(64 * KW, (DecodeShape<T, BITS, DH, RR>::WAVES)) voi
   for (int i = 0; i < 8; ++i) ones.v[i] = (bf16_t)OFFT;
   const Nibbles nb;
 
-  for (int turn = t_begin + wave; turn < t_end; turn += KW) {
-    const bool more = turn + KW < t_end;
-    load_v(turn, 0);
-    // scores of this lane's rows against keys 8 n + t
-    float s[8][RL];
+  // scores of this lane's rows against keys 8 n + t, t of one piece
+  float s[8][RL];
+  const auto scores = [&](int kp) __attribute__((always_inline)) {
+    f32x4 d[KT];
 #pragma unroll
-    for (int kp = 0; kp < KP; ++kp) {
-      f32x4 d[KT];
+    for (int i = 0; i < KT; ++i) {
+      d[i] = zero;
 #pragma unroll
-      for (int i = 0; i < KT; ++i) {
-        d[i] = zero;
-#pragma unroll
-        for (int r = 0; r < RR; ++r) d[i][r] = q0[r];
-      }
-      int own_g = q_g;
-      if constexpr (OWN_Q) asm volatile("" : "+v"(own_g));    // the selects stay in the loop: ahead of it they would take NG times the registers
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        bf16x8 qg[NQ];
-#pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-          if constexpr (OWN_Q) {
-            const Frag own = {.v = qf[0][i]};
-            Frag f;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) f.u[w] = g == own_g ? own.u[w] : 0u;
-            qg[i] = f.v;
-          } else {
-            qg[i] = qf[g][i];
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < KT; ++i) {
-          const bf16x8 kf = unpack_codes<BITS>(&kw[i][g * L::WORD / 4], nb);
-#pragma unroll
-          for (int q = 0; q < NQ; ++q) d[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qg[q], kf, d[i], 0, 0, 0);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < KT; ++i) {
-        const int t = kp * KT + i;
-        float v[RR];
-#pragma unroll
-        for (int r = 0; r < RR; ++r) v[r] = d[i][r] * bf16_at(ks[r], t);
-#pragma unroll
-        for (int rl = 0; rl < RL; ++rl) {
-          float x = v[rl * NG < RR ? rl * NG : 0];
-#pragma unroll
-          for (int g = 1; g < (NG < RR ? NG : RR); ++g) x += v[rl * NG + g];
-          if constexpr (NG >= 2 * RR) x = sum_j1(x);
-          if constexpr (NG >= 4 * RR) x = sum_j2(x);
-          s[t][rl] = x;
-        }
-      }
-      if (kp + 1 < KP) load_k(turn, kp + 1);
+      for (int r = 0; r < RR; ++r) d[i][r] = q0[r];
     }
-    if (more) load_k(turn + KW, 0);
-
+    int own_g = q_g;
+    if constexpr (OWN_Q) asm volatile("" : "+v"(own_g));      // the selects stay in the loop: ahead of it they would take NG times the registers
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      bf16x8 qg[NQ];
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+        if constexpr (OWN_Q) {
+          const Frag own = {.v = qf[0][i]};
+          Frag f;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) f.u[w] = g == own_g ? own.u[w] : 0u;
+          qg[i] = f.v;
+        } else {
+          qg[i] = qf[g][i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < KT; ++i) {
+        const bf16x8 kf = unpack_codes<BITS>(&kw[i][g * L::WORD / 4], nb);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) d[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qg[q], kf, d[i], 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < KT; ++i) {
+      const int t = kp * KT + i;
+      float v[RR];
+#pragma unroll
+      for (int r = 0; r < RR; ++r) v[r] = d[i][r] * bf16_at(ks[r], t);
+#pragma unroll
+      for (int rl = 0; rl < RL; ++rl) {
+        float x = v[rl * NG < RR ? rl * NG : 0];
+#pragma unroll
+        for (int g = 1; g < (NG < RR ? NG : RR); ++g) x += v[rl * NG + g];
+        if constexpr (NG >= 2 * RR) x = sum_j1(x);
+        if constexpr (NG >= 4 * RR) x = sum_j2(x);
+        s[t][rl] = x;
+      }
+    }
+  };
+  // the turn's scores to probabilities times scales in LDS: octet n of pair j RR + r
+  const auto softmax = [&](int turn, bool first) __attribute__((always_inline)) {
     const int key0 = turn * KV_TURN + 8 * n;
     const bool partial = turn * KV_TURN + KV_TURN > n_min;                   // some row does not see all of this turn
     if (partial) {
@@ -370,7 +365,7 @@ __global__ __launch_bounds__(64 * KW, (DecodeShape<T, BITS, DH, RR>::WAVES)) voi
         for (int rl = 0; rl < RL; ++rl) s[t][rl] = key0 + t < row_vis[rl] ? s[t][rl] : -INFINITY;
     }
     float top[RL];
-    bool past = turn == t_begin + wave;
+    bool past = first;
 #pragma unroll
     for (int rl = 0; rl < RL; ++rl) {
       top[rl] = s[0][rl];
@@ -415,14 +410,15 @@ __global__ __launch_bounds__(64 * KW, (DecodeShape<T, BITS, DH, RR>::WAVES)) voi
     for (int rl = 0; rl < RL; ++rl)
 #pragma unroll
       for (int t = 0; t < 8; t += 2) l[rl] += p[t][rl] + p[t + 1][rl];
-    // probabilities times scales, octet n of pair j RR + r
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");                   // the previous turn's are read
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int r = 0; r < RR; ++r) {
       const int rl = RL > 1 ? r / NG : 0;
       float x[8];
 #pragma unroll
       for (int t = 0; t < 8; ++t) x[t] = p[t][rl] * bf16_at(vs[r], t);
-      if (partial) {                                                         // whose scale may be anything
+      if (partial) {                                                         // the scale of a key not seen may be anything
 #pragma unroll
         for (int t = 0; t < 8; ++t) x[t] = key0 + t < row_vis[rl] ? x[t] : 0.f;
       }
@@ -434,29 +430,68 @@ __global__ __launch_bounds__(64 * KW, (DecodeShape<T, BITS, DH, RR>::WAVES)) voi
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    // output: row n of A is pair n (rows past the pairs repeat them and are not used), octets 4 tile + j
+  };
+  // one piece of the output: row n of A is pair n (rows past the pairs repeat them and are not used), octets 4 tile + j
+  const auto output = [&](int vp) __attribute__((always_inline)) {
 #pragma unroll
-    for (int vp = 0; vp < VP; ++vp) {
+    for (int i = 0; i < VT; ++i) {
+      bf16x8 pf[NP];
 #pragma unroll
-      for (int i = 0; i < VT; ++i) {
-        bf16x8 pf[NP];
+      for (int q = 0; q < NP; ++q) pf[q] = sh.p[wave][q][n & (D::PAIRS - 1)][4 * (vp * VT + i) + j];
+      if constexpr (OFFT != 0.f) {
 #pragma unroll
-        for (int q = 0; q < NP; ++q) pf[q] = sh.p[wave][q][n & (D::PAIRS - 1)][4 * (vp * VT + i) + j];
-        if constexpr (OFFT != 0.f) {
-#pragma unroll
-          for (int q = 0; q < NP; ++q) off = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf[q], ones.v, off, 0, 0, 0);
-        }
-#pragma unroll
-        for (int c = 0; c < CB; ++c) {
-          const bf16x8 vf = unpack_codes<BITS>(&vw[i][c * L::WORD / 4], nb);
-#pragma unroll
-          for (int q = 0; q < NP; ++q) acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf[q], vf, acc[c], 0, 0, 0);
-        }
+        for (int q = 0; q < NP; ++q) off = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf[q], ones.v, off, 0, 0, 0);
       }
-      if (vp + 1 < VP) load_v(turn, vp + 1);
+#pragma unroll
+      for (int c = 0; c < CB; ++c) {
+        const bf16x8 vf = unpack_codes<BITS>(&vw[i][c * L::WORD / 4], nb);
+#pragma unroll
+        for (int q = 0; q < NP; ++q) acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf[q], vf, acc[c], 0, 0, 0);
+      }
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");                    // the next turn's probabilities overwrite these
-    __builtin_amdgcn_wave_barrier();
+  };
+
+  int turn = t_begin + wave;
+  if constexpr (KP == 1) {
+    for (; turn < t_end; turn += KW) {
+      load_v(turn, 0);
+      load_v_scales(turn);
+      scores(0);
+      if (turn + KW < t_end) load_k(turn + KW, 0);
+      softmax(turn, turn == t_begin + wave);
+      output(0);
+    }
+  } else {
+    // In pieces: the next turn's scores run between the pieces of this turn's output, so that each piece's loads have the other's
+    // arithmetic to hide behind (16 uneven sequences, heads of 256, 8 bits: 61 -> 50 us).
+    if (turn < t_end) {
+      load_v_scales(turn);
+      load_v(turn, 0);
+#pragma unroll
+      for (int x = 0; x < KP; ++x) {
+        scores(x);
+        if (x + 1 < KP) load_k(turn, x + 1);
+      }
+      if (turn + KW < t_end) load_k(turn + KW, 0);
+      softmax(turn, true);
+    }
+    for (; turn < t_end; turn += KW) {
+      const int next = turn + KW;
+      const bool more = next < t_end;
+      if (more) load_v_scales(next);
+#pragma unroll
+      for (int x = 0; x < KP; ++x) {
+        if (more) {
+          scores(x);
+          if (x + 1 < KP) load_k(next, x + 1);
+          else if (next + KW < t_end) load_k(next + KW, 0);
+        }
+        output(x);
+        if (x + 1 < KP) load_v(turn, x + 1);
+        else if (more) load_v(next, 0);
+      }
+      if (more) softmax(next, false);
+    }
   }
 
 #pragma unroll
