@@ -37,7 +37,8 @@ struct KvAttnArgs {
   int64_t o_sb, o_sh, o_st;
   float* lse;
   float* part;                              // [row][split][Dh + 2]: unnormalised output, maximum (log2), sum
-  int G, max_keys, splits, rows_per_tile, negate;
+  int G, max_keys, splits, rows_per_tile;
+  bool negate, q_vec;                       // negative scale; queries on the 16-byte grid
   float scale_log2;                         // |scale| log2(e)
 };
 
@@ -61,6 +62,28 @@ template <int N> __device__ __forceinline__ void load_words(const uint8_t* p, ui
     w[0] = v.x; w[1] = v.y;
   } else {
     w[0] = *(const uint32_t*)p;
+  }
+}
+
+// 8 neighbouring channels of a query; vec: on the 16-byte grid
+template <typename T> __device__ __forceinline__ void load_query(const T* q, bool vec, bool real, bool negate, float (&x)[8]) {
+  if (vec && real) {
+    if constexpr (sizeof(T) == 2) {
+      const bf16x8 v = *(const bf16x8*)q;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = (float)v[e];
+    } else {
+      const f32x4 u = *(const f32x4*)q, v = *(const f32x4*)(q + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { x[e] = u[e]; x[4 + e] = v[e]; }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = real ? to_f32(q[e]) : 0.f;
+  }
+  if (negate) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = -x[e];
   }
 }
 
@@ -251,12 +274,9 @@ __global__ __launch_bounds__(64 * KW, (DecodeShape<T, BITS, DH, RR>::WAVES)) voi
     const int t_row = a.kv.T > 1 ? (int)((uint32_t)q_row / (uint32_t)a.G) : 0, g_row = q_row - t_row * a.G;
     const T* q = (const T*)a.q + b * a.q_sb + (int64_t)(h * a.G + g_row) * a.q_sh + (int64_t)t_row * a.q_st + 32 * q_g + 8 * j;
     float x[8], sum = 0.f;
+    load_query(q, a.q_vec, q_real, a.negate, x);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float v = q_real ? to_f32(q[e]) : 0.f;
-      x[e] = a.negate ? -v : v;
-      sum += x[e];
-    }
+    for (int e = 0; e < 8; ++e) sum += x[e];
     bf16x8 piece[NQ];
     split_bf16<NQ>(x, piece);
 #pragma unroll
@@ -577,12 +597,9 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<BITS, DH>())) void kv_attn_kerne
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       float x[8], sum = 0.f;
+      load_query(q + 32 * g, a.q_vec, real, a.negate, x);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float v = real ? to_f32(q[32 * g + e]) : 0.f;
-        x[e] = a.negate ? -v : v;
-        sum += x[e];
-      }
+      for (int e = 0; e < 8; ++e) sum += x[e];
       bf16x8 piece[NQ];
       split_bf16<NQ>(x, piece);
 #pragma unroll
@@ -851,6 +868,8 @@ extern "C" int bg_kv_cache_attn_fwd(const bg_kv_cache* cache, const void* data, 
   a.G = Hq / cache->H; a.max_keys = max_keys; a.splits = p.splits;
   a.rows_per_tile = p.pairs > 16 ? 16 : T * a.G;
   a.negate = scale < 0.f;
+  const int64_t es = dtype == BG_F32 ? 4 : 2;
+  a.q_vec = (((uintptr_t)q | (uintptr_t)(q_sb * es) | (uintptr_t)(q_sh * es) | (uintptr_t)(q_st * es)) & 15) == 0;
   a.scale_log2 = (float)((scale < 0.f ? -(double)scale : (double)scale) * 1.4426950408889634);
   hipStream_t st = (hipStream_t)stream;
 #define BG_GO(BITS, DH)                                           \
