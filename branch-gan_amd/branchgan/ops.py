@@ -820,7 +820,7 @@ class KVCacheLayer:
         if data.dtype != torch.uint8 or data.dim() != 3 or data.stride(-1) != 1 or data.shape[-1] != -(-int(capacity) // KV_TILE) * tile:
             raise ValueError(f"cache data must be uint8 (batch, heads, {-(-int(capacity) // KV_TILE) * tile}) with a dense last dimension")
         self.data, self.bits, self.head_dim, self.capacity = data, int(bits), int(head_dim), int(capacity)
-        self.batch, self.heads, self.device = data.shape[0], data.shape[1], data.device
+        self.batch, self.heads, self.device, self.rows_shape = data.shape[0], data.shape[1], data.device, data.shape[:1]
         sh = C.KvCache()
         sh.bits, sh.B, sh.H, sh.Dh, sh.capacity = self.bits, self.batch, self.heads, self.head_dim, self.capacity
         sh.c_sb, sh.c_sh = data.stride(0), data.stride(1)
@@ -831,9 +831,10 @@ def _kv_rows(name, t, layer):
     """start / counts of the cache calls: int32 (B,) on the cache's device, or None.  -> a dense tensor, its address"""
     if t is None:
         return None, None
-    if t.dtype != torch.int32 or t.shape != (layer.batch,) or t.device != layer.device:
+    if t.dtype != torch.int32 or t.shape != layer.rows_shape or t.device != layer.device:
         raise ValueError(f"{name} must be int32 of shape ({layer.batch},) on {layer.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    t = t.contiguous()
+    if not t.is_contiguous():
+        t = t.contiguous()
     return t, t.data_ptr()
 
 
@@ -842,12 +843,17 @@ def _no_grad_wanted(what, *tensors):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
 
 
-def _on_device(device, call):
-    """call(raw current stream of the device), made on that device."""
-    if torch.cuda.current_device() == device.index:
-        return call(C.raw_stream(device.index))
-    with torch.cuda.device(device):
-        return call(C.raw_stream(device.index))
+def _launch(name, device, entry, *args):
+    """entry(*args, raw current stream of the device), made on that device; its error, if any, raised."""
+    index = device.index
+    with _timed(name):
+        if torch.cuda.current_device() == index:
+            code = entry(*args, C.raw_stream(index))
+        else:
+            with torch.cuda.device(device):
+                code = entry(*args, C.raw_stream(index))
+    if code:
+        C.check(code, name)
 
 
 def kv_cache_append(layer, k, v, start=None, counts=None):
@@ -866,10 +872,8 @@ def kv_cache_append(layer, k, v, start=None, counts=None):
     if k.numel() == 0:
         return
     k, v = _unit_last(k), _unit_last(v)
-    with _timed("kv_cache_append"):
-        C.check(_on_device(layer.device, lambda stream: C.lib().bg_kv_cache_append(
-            layer._struct, layer.data.data_ptr(), k.data_ptr(), v.data_ptr(), code, T, *k.stride()[:3], *v.stride()[:3], p_start, p_counts, stream)),
-            "bg_kv_cache_append")
+    _launch("bg_kv_cache_append", layer.device, C.lib().bg_kv_cache_append, layer._struct, layer.data.data_ptr(), k.data_ptr(), v.data_ptr(), code, T,
+            *k.stride()[:3], *v.stride()[:3], p_start, p_counts)
 
 
 def kv_cache_read(layer, n, start=None, counts=None, dtype=torch.bfloat16):
@@ -885,9 +889,8 @@ def kv_cache_read(layer, n, start=None, counts=None, dtype=torch.bfloat16):
     code = C.dtype_code(k)
     if k.numel() == 0:
         return k, v
-    with _timed("kv_cache_read"):
-        C.check(_on_device(layer.device, lambda stream: C.lib().bg_kv_cache_read(
-            layer._struct, layer.data.data_ptr(), k.data_ptr(), v.data_ptr(), code, n, *k.stride()[:3], p_start, p_counts, stream)), "bg_kv_cache_read")
+    _launch("bg_kv_cache_read", layer.device, C.lib().bg_kv_cache_read, layer._struct, layer.data.data_ptr(), k.data_ptr(), v.data_ptr(), code, n,
+            *k.stride()[:3], p_start, p_counts)
     return k, v
 
 
@@ -897,9 +900,9 @@ def kv_cache_attention(q, layer, start=None, counts=None, scale=None, max_keys=N
     see nothing (padding) are zeros.  max_keys: the most keys any sequence holds after the append, if the host knows it (default:
     the capacity); keys past it are not read.  -> (out like q [a (B, T, Hq, Dh)-contiguous view], lse fp32 (B, Hq, T))."""
     C.require_cuda(q, layer.data, start, counts)
-    B, H = layer.batch, layer.heads
-    if q.dim() != 4 or q.shape[0] != B or q.shape[3] != layer.head_dim or q.shape[1] == 0 or q.shape[1] % max(H, 1):
-        raise ValueError(f"q must be ({B}, a multiple of {H} heads, T, {layer.head_dim}), got {tuple(q.shape)}")
+    B, H, shape = layer.batch, layer.heads, q.shape
+    if len(shape) != 4 or shape[0] != B or shape[3] != layer.head_dim or shape[1] == 0 or shape[1] % max(H, 1):
+        raise ValueError(f"q must be ({B}, a multiple of {H} heads, T, {layer.head_dim}), got {tuple(shape)}")
     if q.device != layer.device:
         raise ValueError(f"q is on {q.device}, the cache on {layer.device}")
     _no_grad_wanted("kv_cache_attention", q)
@@ -907,9 +910,9 @@ def kv_cache_attention(q, layer, start=None, counts=None, scale=None, max_keys=N
     max_keys = layer.capacity if max_keys is None else int(max_keys)
     if not 0 < max_keys <= layer.capacity:
         raise ValueError(f"max_keys {max_keys} is not in 1 .. {layer.capacity} (the capacity)")
-    code, (_, Hq, T, Dh) = C.dtype_code(q), q.shape
-    out = torch.empty((B, T, Hq, Dh), dtype=q.dtype, device=q.device).transpose(1, 2)
-    lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device)
+    code, (_, Hq, T, Dh) = C.dtype_code(q), shape
+    out = q.new_empty((B, T, Hq, Dh)).transpose(1, 2)
+    lse = q.new_empty((B, Hq, T), dtype=torch.float32)
     if q.numel() == 0:
         return out, lse
     q = _unit_last(q)
@@ -920,21 +923,15 @@ def kv_cache_attention(q, layer, start=None, counts=None, scale=None, max_keys=N
     # and graphs replayed side by side must not share one
     ws_bytes = lib.bg_kv_cache_attn_workspace_bytes(layer._struct, Hq, T, max_keys)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-    with _timed("kv_cache_attention"):
-        C.check(_on_device(layer.device, lambda stream: lib.bg_kv_cache_attn_fwd(
-            layer._struct, layer.data.data_ptr(), q.data_ptr(), code, Hq, T, *q.stride()[:3], p_start, p_counts, max_keys, float(scale),
-            out.data_ptr(), *out.stride()[:3], lse.data_ptr(), ws.data_ptr() if ws_bytes else None, ws_bytes, stream)), "bg_kv_cache_attn_fwd")
+    _launch("bg_kv_cache_attn_fwd", layer.device, lib.bg_kv_cache_attn_fwd, layer._struct, layer.data.data_ptr(), q.data_ptr(), code, Hq, T,
+            *q.stride()[:3], p_start, p_counts, max_keys, float(scale), out.data_ptr(), *out.stride()[:3], lse.data_ptr(),
+            ws.data_ptr() if ws_bytes else None, ws_bytes)
     return out, lse
 
 
 # ---------------------------------------------------------------------------------------------------
 # Clipped policy loss with a KL term
 # ---------------------------------------------------------------------------------------------------
-def _policy_launch(name, device, call):
-    with _timed(name):
-        C.check(_on_device(device, call), name)
-
-
 class _PolicyLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, rows_f32, ref_logits, denominator, shape):
@@ -944,11 +941,8 @@ class _PolicyLoss(torch.autograd.Function):
         y = dense(_rows_2d(ref_logits)) if ref_logits is not None else None
         rows, dev = x.shape[0], x.device
         ids = ids.reshape(rows).to(torch.int64).contiguous()
-        flat = [None if t is None else _f32c(t.reshape(rows)) for t in rows_f32]
-        sh = C.PolicyShape()
-        sh.dtype, sh.rows, sh.V = C.dtype_code(x), rows, V
-        sh.x_stride, sh.ref_stride = max(x.stride(0), V), (max(y.stride(0), V) if y is not None else 0)
-        sh.temperature, sh.clip_low, sh.clip_high, sh.kl_coef = shape
+        flat = [None if t is None else _f32c(t) for t in rows_f32]
+        sh = C.PolicyShape(C.dtype_code(x), 0, rows, V, max(x.stride(0), V), max(y.stride(0), V) if y is not None else 0, *shape)
         loss, lead = torch.empty((), dtype=torch.float32, device=dev), logits.shape[:-1]
         logp, kl = torch.empty(lead, dtype=torch.float32, device=dev), torch.empty(lead, dtype=torch.float32, device=dev)
         stats = torch.empty(rows * C.POLICY_STATS + 1, dtype=torch.float32, device=dev)
@@ -956,9 +950,8 @@ class _PolicyLoss(torch.autograd.Function):
         dx = torch.empty((rows, V), dtype=x.dtype, device=dev) if ctx.needs_input_grad[0] else None
         has = C.c_i32(0)
         ptr = lambda t: None if t is None else t.data_ptr()
-        _policy_launch("bg_policy_loss_fwd", dev, lambda stream: C.lib().bg_policy_loss_fwd(
-            ctypes.byref(sh), x.data_ptr(), ptr(y), ids.data_ptr(), *[ptr(t) for t in flat], ptr(denominator), loss.data_ptr(), logp.data_ptr(),
-            kl.data_ptr(), stats.data_ptr(), ptr(dx), ctypes.byref(has), stream))
+        _launch("bg_policy_loss_fwd", dev, C.lib().bg_policy_loss_fwd, ctypes.byref(sh), x.data_ptr(), ptr(y), ids.data_ptr(), *[ptr(t) for t in flat],
+                ptr(denominator), loss.data_ptr(), logp.data_ptr(), kl.data_ptr(), stats.data_ptr(), ptr(dx), ctypes.byref(has))
         ctx.save_for_backward(x, ids, stats, y)
         ctx.dx, ctx.sh, ctx.in_shape = dx if has.value else None, sh, logits.shape
         ctx.mark_non_differentiable(logp, kl)
@@ -976,9 +969,8 @@ class _PolicyLoss(torch.autograd.Function):
         has = dx is not None
         if not has:
             dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        _policy_launch("bg_policy_loss_bwd", x.device, lambda stream: C.lib().bg_policy_loss_bwd(
-            ctypes.byref(ctx.sh), x.data_ptr(), None if y is None else y.data_ptr(), ids.data_ptr(), stats.data_ptr(), g.data_ptr(), dx.data_ptr(),
-            int(has), stream))
+        _launch("bg_policy_loss_bwd", x.device, C.lib().bg_policy_loss_bwd, ctypes.byref(ctx.sh), x.data_ptr(), None if y is None else y.data_ptr(),
+                ids.data_ptr(), stats.data_ptr(), g.data_ptr(), dx.data_ptr(), int(has))
         return dx.view(ctx.in_shape), None, None, None, None, None
 
 
@@ -1011,6 +1003,7 @@ def policy_loss(logits, ids, old_logp, advantages, weights=None, ref_logp=None, 
             denominator = _f32c(denominator.detach().reshape(1))
         else:
             denominator = torch.full((1,), float(denominator), dtype=torch.float32, device=logits.device)
-    rows_f32 = tuple(None if t is None else t.detach() for t in (old_logp, ref_logp, advantages, weights))
-    return _PolicyLoss.apply(logits, ids, rows_f32, None if ref_logits is None else ref_logits.detach(), denominator,
+    # (no gradient flows into these: a tuple is not seen by autograd, and ref_logits gets none back)
+    rows_f32 = (old_logp, ref_logp, advantages, weights)
+    return _PolicyLoss.apply(logits, ids, rows_f32, ref_logits, denominator,
                              (float(temperature), float(clip_low), float(clip_high), float(kl_coef)))
