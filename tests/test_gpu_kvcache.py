@@ -205,6 +205,73 @@ def test_attention_against_float64(case, bits, dtype):
     assert bool(((lse.cpu().double() - ref_lse).abs()[seen] <= (rel + 2.0 ** -23 * (ref_lse.abs() + 8))[seen]).all())
 
 
+FEW = [(1, 1), (2, 1), (1, 3), (3, 2), (8, 1), (1, 10), (16, 1), (4, 5)]     # query heads per cache head, new tokens
+
+
+@pytest.mark.parametrize("G,T", FEW)
+@pytest.mark.parametrize("Dh", [32, 64, 128, 256])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_few_rows_around_the_turns(G, T, Dh, bits, dtype):
+    """Every shape of few-row tile, with sequences that end on, before and after a wave's 128 keys and a workgroup's 512."""
+    from branchgan import ops
+    gen = torch.Generator().manual_seed(G * 100 + T * 10 + Dh + bits)
+    held = (1, 127, 128, 129, 512, 641)
+    B, H = len(held), 1
+    n = max(held) + T
+    k, v = make(gen, B, H, n, Dh, dtype)
+    layer = new_cache(B, H, n + 3, Dh, bits, fill=21)
+    ops.kv_cache_append(layer, k.cuda(), v.cuda())
+    q = torch.randn(B, G * H, T, Dh, generator=gen).to(dtype)
+    kh, vh = O.held_values(k, bits), O.held_values(v, bits)
+    start = tuple(x - 1 for x in held)
+    ref, ref_lse = O.attention(q, kh, vh, start)
+    tol, rel = bound(q, kh, vh, 1 / math.sqrt(Dh), dtype, ref)
+    out, lse = ops.kv_cache_attention(q.cuda(), layer, start=i32(*start))
+    assert within(out.cpu().double() - ref, tol) and within(lse.cpu().double() - ref_lse, rel + 2.0 ** -23 * (ref_lse.abs() + 8))
+    # one sequence at a time: other splits of the key range, the same numbers within the bound
+    for b in (0, 3, 5):
+        one = ops.KVCacheLayer(layer.data[b:b + 1], bits, Dh, n + 3)
+        o1, _ = ops.kv_cache_attention(q[b:b + 1].cuda(), one, start=i32(start[b]), max_keys=start[b] + T)
+        assert within(o1.cpu().double() - ref[b:b + 1], tol[b:b + 1])
+
+
+def test_scales_of_any_sign():
+    from branchgan import ops
+    gen = torch.Generator().manual_seed(23)
+    for G, T in ((1, 1), (2, 20)):
+        k, v = make(gen, 2, 2, 300, 64, torch.float32)
+        layer = new_cache(2, 2, 300, 64, 4)
+        ops.kv_cache_append(layer, k.cuda(), v.cuda())
+        q = torch.randn(2, 2 * G, T, 64, generator=gen)
+        kh, vh = O.held_values(k, 4), O.held_values(v, 4)
+        for scale in (-0.2, 0.0, 1.0):
+            ref, _ = O.attention(q, kh, vh, (150, 280), scale=scale)
+            tol, _ = bound(q, kh, vh, abs(scale), torch.float32, ref)
+            out, _ = ops.kv_cache_attention(q.cuda(), layer, start=i32(150, 280), scale=scale)
+            assert within(out.cpu().double() - ref, tol), scale
+
+
+def test_on_another_stream():
+    """Append, read and attend on a side stream, ordered by events with the tensors' own: the same bits as on theirs."""
+    from branchgan import ops
+    gen = torch.Generator().manual_seed(24)
+    k, v = [t.cuda() for t in make(gen, 2, 2, 1500, 64, torch.bfloat16)]
+    q = torch.randn(2, 2, 1, 64, generator=gen).bfloat16().cuda()
+    res = []
+    for side in (None, torch.cuda.Stream()):
+        layer = new_cache(2, 2, 1600, 64, 4)
+        if side is not None:
+            side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side or torch.cuda.current_stream()):
+            ops.kv_cache_append(layer, k, v)
+            res.append([*ops.kv_cache_attention(q, layer, start=i32(1499, 1203)), *ops.kv_cache_read(layer, 1500)])
+        if side is not None:
+            torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
 def test_keys_behind_the_last_one_do_not_matter():
     """Stale scales of NaN and infinity behind the visible keys (an earlier, longer sequence) change nothing."""
     from branchgan import ops

@@ -79,7 +79,8 @@ def check(d, g=1.0, **kw):
     ratio = torch.exp(logp - d["old_logp"].double())
     pg_tol = (d["advantages"].double() * ratio).abs() * 2 * dl
     total = (w.abs() * (pg_tol + abs(beta) * kl_tol))[w != 0].sum() / abs(n) if n else torch.zeros(())
-    assert abs(float(got_loss) - float(loss)) <= float(total) + 2.0 ** -23 * abs(float(loss)), (float(got_loss), float(loss))
+    loss = float(loss.detach())
+    assert abs(float(got_loss) - loss) <= float(total) + 2.0 ** -23 * abs(loss), (float(got_loss), loss)
     # gradient: slope (off by 2 dl of its parts) times (1[j = id] - p), p off by dl; KL part p (gap - kl); one rounding at the end
     p = torch.softmax(d["logits"].double() / T, -1)
     one = torch.zeros_like(p)
@@ -203,6 +204,40 @@ def test_backward_twice_and_without_grad():
     torch.testing.assert_close(g3.float(), 3 * g1.float(), rtol=2.0 ** -7, atol=1e-12)
     with torch.no_grad():
         assert torch.equal(ops.policy_loss(x, *args, ref_logp=d["ref_logp"].cuda(), kl_coef=0.1)[0], loss)
+
+
+@pytest.mark.parametrize("ref", [None, "logp", "logits"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_for_every_size_of_workgroup(dtype, ref):
+    """Vocabularies on both sides of every limit in the choice of kernel (whole vectors per thread and workgroup), and rows whose
+    16-byte grid differs between logits, reference and gradient."""
+    n = 4 if dtype == torch.float32 else 8
+    for V in (2 * n - 1, 2 * n, 2 * n + 1, 512 * n - n - 1, 512 * n, 2048 * n - 1, 2048 * n + 1, 6656 * n - n - 1, 6656 * n - 1, 6656 * n + 1):
+        check(off_the_clip(inputs(2, V, dtype, V, ref), 1.0, 0.2, 0.2), kl_coef=0.1)
+    if ref == "logits":
+        from branchgan import ops
+        d = off_the_clip(inputs(5, 1001, dtype, 3, ref), 1.0, 0.2, 0.2)
+        wide = torch.zeros(5, 1003, dtype=dtype, device="cuda")
+        wide[:, 1:1002] = d["logits"].cuda()
+        want, _, _, grad = run(d, kl_coef=0.1)
+        x = wide.requires_grad_(True)
+        loss, _, _ = ops.policy_loss(x[:, 1:1002], *[d[k].cuda() for k in ("ids", "old_logp", "advantages")], ref_logits=d["ref_logits"].cuda(), kl_coef=0.1)
+        loss.backward()
+        torch.testing.assert_close(loss.detach().cpu(), want, rtol=1e-6, atol=1e-7)
+        torch.testing.assert_close(x.grad[:, 1:1002], grad, rtol=2 * torch.finfo(dtype).eps, atol=1e-9)
+
+
+def test_many_rows_and_the_largest_vocabulary_are_one_answer():
+    """More rows than the workgroups sum weights for themselves; the loss equals the mean of the rows' own losses."""
+    from branchgan import ops
+    d = off_the_clip(inputs(1500, 300, torch.float32, 61, "logp"), 1.0, 0.2, 0.2)
+    d["weights"] = (torch.arange(1500) % 5 > 0).float()
+    check(d, kl_coef=0.1)
+    args = [d[k].cuda() for k in ("logits", "ids", "old_logp", "advantages")]
+    whole, _, _ = ops.policy_loss(*args, weights=d["weights"].cuda(), ref_logp=d["ref_logp"].cuda(), kl_coef=0.1)
+    parts = [float(ops.policy_loss(*[a[i:i + 300] for a in args], weights=d["weights"][i:i + 300].cuda(), ref_logp=d["ref_logp"][i:i + 300].cuda(),
+                                   kl_coef=0.1, denominator=1200)[0]) for i in range(0, 1500, 300)]
+    assert abs(float(whole) - sum(parts)) <= 6 * 2.0 ** -23 * sum(abs(p) for p in parts)
 
 
 def test_captured_step_replays():
