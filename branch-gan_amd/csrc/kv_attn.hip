@@ -2,8 +2,7 @@
 //
 // Mathematics.  With codes c and scales s per 32 channels g,
 //   q . k = sum_g s_kg (q_g . c_kg)         o_ch = sum_k (p_k s_vg) c_v,ch
-// so the codes themselves are the matrix operands: as bf16 they are exact (4 bits: as c + 24, whose part is taken out of the sums; 8
-// bits: signed), the scales join in fp32 - on the scores after the product, on the probabilities before it.  Nothing held is rounded again.  bf16
+// so the codes themselves are the matrix operands: as bf16 they are exact (see unpack_codes), the scales join in fp32 - on the scores after the product, on the probabilities before it.  Nothing held is rounded again.  bf16
 // queries are exact operands; fp32 queries go in as three bf16 pieces (24 bits), probabilities as two (16 bits, for bf16 outputs) or three.
 //
 // Layouts.  One wave takes 4 tiles (128 keys) per turn with v_mfma_f32_16x16x32_bf16 (rows of A x columns of B, 32 deep; lane = (n =
@@ -39,7 +38,7 @@ struct KvAttnArgs {
   float* part;                              // [row][split][Dh + 2]: unnormalised output, maximum (log2), sum
   int G, max_keys, splits, rows_per_tile;
   bool negate, q_vec;                       // negative scale; queries on the 16-byte grid
-  float scale_log2;                         // |scale| log2(e)
+  float scale_log2;                         // |scale| log2(e), times the unit of the codes
 };
 
 // Most (returned) and fewest keys that the rows of the tile at row0 see.
@@ -92,21 +91,35 @@ union Frag {
   bf16x8 v;
 };
 
-// 8 codes -> 8 bf16 numbers code + OFFT.  4 bits: the nibble as bits 3..6 of a bf16 in [16, 32) is 16 + stored code; 8 bits: converted
-// (a conversion that takes its byte from the word, and half a pack).
-template <int BITS> constexpr float kv_offset() { return BITS == 4 ? 24.f : 0.f; }
-// The two constants sit in a vector and a scalar register: as literals they would make the mask-or two instructions.
+// 8 codes -> 8 bf16 numbers (code + offset) / unit.
+// 4 bits, bf16 queries: the nibble as bits 3..6 of a bf16 in [16, 32) is 16 + stored code = code + 24 - a shift and a mask-or per pair.
+// (The two constants sit in a vector and a scalar register: as literals they would make the mask-or two instructions.)
+// 4 bits, fp32 queries: sums of c + 24 would cost 2 to 3 bits that fp32 results show (error 4e-6 against 4e-7), so the codes come
+// signed, by the instruction that reads a signed nibble as sixteenths - twice the instructions.
+// 8 bits: signed bytes, converted (a conversion that takes its byte from the word, and half a pack).
+template <typename T, int BITS> constexpr float kv_offset() { return BITS == 4 && sizeof(T) == 2 ? 24.f : 0.f; }
+template <typename T, int BITS> constexpr float kv_unit() { return BITS == 4 && sizeof(T) == 4 ? 16.f : 1.f; }
 struct Nibbles {
   uint32_t mask, base;
   __device__ __forceinline__ Nibbles() : mask(0x00780078u), base(0x41804180u) { asm volatile("" : "+v"(mask), "+s"(base)); }
 };
-template <int BITS> __device__ __forceinline__ bf16x8 unpack_codes(const uint32_t* w, const Nibbles& nb) {
+template <typename T, int BITS> __device__ __forceinline__ bf16x8 unpack_codes(const uint32_t* w, const Nibbles& nb) {
   Frag f;
-  if constexpr (BITS == 4) {
+  if constexpr (BITS == 4 && sizeof(T) == 2) {
     f.u[0] = ((w[0] << 3) & nb.mask) | nb.base;
     f.u[1] = ((w[0] >> 1) & nb.mask) | nb.base;
     f.u[2] = ((w[0] >> 5) & nb.mask) | nb.base;
     f.u[3] = ((w[0] >> 9) & nb.mask) | nb.base;
+  } else if constexpr (BITS == 4) {
+    const uint32_t lo = w[0] ^ 0x88888888u;                // code + 8 to two's complement
+    uint32_t hi = lo >> 4;
+    asm volatile("" : "+v"(hi));                           // (one shift for four nibbles: the conversion picks its byte)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t x = i & 1 ? hi : lo;
+      f.v[2 * i] = (bf16_t)__builtin_amdgcn_cvt_off_f32_i4((int)((x >> (8 * (i / 2))) & 255u));
+      f.v[2 * i + 1] = (bf16_t)__builtin_amdgcn_cvt_off_f32_i4((int)((x >> (8 * (i / 2) + 16)) & 255u));
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) f.v[i] = (bf16_t)(float)(int8_t)(w[i / 4] >> (8 * (i % 4)));
@@ -219,7 +232,7 @@ __global__ __launch_bounds__(64 * KW, (DecodeShape<T, BITS, DH, RR>::WAVES)) voi
   using D = DecodeShape<T, BITS, DH, RR>;
   constexpr int NG = L::NG, CB = DH / 16, RL = D::RL, KT = D::KT, VT = D::VT, KP = 8 / KT;
   constexpr int NQ = sizeof(T) == 4 ? 3 : 1, NP = sizeof(T) == 4 ? 3 : 2;   // bf16 pieces of queries / probabilities
-  constexpr float OFFT = kv_offset<BITS>();
+  constexpr float OFFT = kv_offset<T, BITS>();
   constexpr bool OWN_Q = NG * NQ > 4;               // keep a lane's one group only, and the zeros of the others as a select per use
   constexpr int KWORDS = NG * L::WORD / 4, VWORDS = CB * L::WORD / 4;
   struct Shared {
@@ -352,7 +365,7 @@ __global__ __launch_bounds__(64 * KW, (DecodeShape<T, BITS, DH, RR>::WAVES)) voi
       }
 #pragma unroll
       for (int i = 0; i < KT; ++i) {
-        const bf16x8 kf = unpack_codes<BITS>(&kw[i][g * L::WORD / 4], nb);
+        const bf16x8 kf = unpack_codes<T, BITS>(&kw[i][g * L::WORD / 4], nb);
 #pragma unroll
         for (int q = 0; q < NQ; ++q) d[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qg[q], kf, d[i], 0, 0, 0);
       }
@@ -464,7 +477,7 @@ __global__ __launch_bounds__(64 * KW, (DecodeShape<T, BITS, DH, RR>::WAVES)) voi
       }
 #pragma unroll
       for (int c = 0; c < CB; ++c) {
-        const bf16x8 vf = unpack_codes<BITS>(&vw[i][c * L::WORD / 4], nb);
+        const bf16x8 vf = unpack_codes<T, BITS>(&vw[i][c * L::WORD / 4], nb);
 #pragma unroll
         for (int q = 0; q < NP; ++q) acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf[q], vf, acc[c], 0, 0, 0);
       }
@@ -524,7 +537,7 @@ __global__ __launch_bounds__(64 * KW, (DecodeShape<T, BITS, DH, RR>::WAVES)) voi
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int p = 4 * j + r;
-      if (p < D::PAIRS && p % NG == c / 2) sh.o[wave][p / NG][16 * c + n] = acc[c][r] - off[r];
+      if (p < D::PAIRS && p % NG == c / 2) sh.o[wave][p / NG][16 * c + n] = (acc[c][r] - off[r]) * kv_unit<T, BITS>();
     }
   __syncthreads();
   write_rows<T, DH, D::ROWS>(a, sh, b, h, 0, split);
@@ -540,7 +553,7 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<BITS, DH>())) void kv_attn_kerne
   using L = KvTile<BITS, DH>;
   constexpr int NG = L::NG, TS = kv_steps<BITS, DH>(), NO = TS / 2, CB = DH / 16, ROWS = 16;
   constexpr int NQ = sizeof(T) == 4 ? 3 : 1, NP = sizeof(T) == 4 ? 3 : 2;   // bf16 pieces of queries / probabilities
-  constexpr float OFFT = kv_offset<BITS>();
+  constexpr float OFFT = kv_offset<T, BITS>();
   constexpr bool LDS_Q = NG * NQ > 8;                                        // the pieces of long fp32 rows live in LDS
   constexpr int KWORDS = NG * L::WORD / 4, VWORDS = CB * L::WORD / 4;
   struct Shared {
@@ -651,7 +664,7 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<BITS, DH>())) void kv_attn_kerne
       }
 #pragma unroll
       for (int t = 0; t < TS; ++t) {
-        const bf16x8 kf = unpack_codes<BITS>(&kw[t][g * L::WORD / 4], nb);
+        const bf16x8 kf = unpack_codes<T, BITS>(&kw[t][g * L::WORD / 4], nb);
         f32x4 d = {q0[g], q0[g], q0[g], q0[g]};
 #pragma unroll
         for (int i = 0; i < NQ; ++i) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qg[i], d, 0, 0, 0);
@@ -733,7 +746,7 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<BITS, DH>())) void kv_attn_kerne
       }
 #pragma unroll
       for (int c = 0; c < CB; ++c) {
-        const bf16x8 vf = unpack_codes<BITS>(&vw[o][c * L::WORD / 4], nb);
+        const bf16x8 vf = unpack_codes<T, BITS>(&vw[o][c * L::WORD / 4], nb);
 #pragma unroll
         for (int i = 0; i < NP; ++i) acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf[c / 2][i], vf, acc[c], 0, 0, 0);
       }
@@ -746,7 +759,7 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<BITS, DH>())) void kv_attn_kerne
 #pragma unroll
   for (int c = 0; c < CB; ++c)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) sh.o[wave][4 * j + r][16 * c + n] = acc[c][r] - offg[c / 2][r];
+    for (int r = 0; r < 4; ++r) sh.o[wave][4 * j + r][16 * c + n] = (acc[c][r] - offg[c / 2][r]) * kv_unit<T, BITS>();
   __syncthreads();
   write_rows<T, DH, ROWS>(a, sh, b, h, row0, split);
 }
@@ -870,7 +883,8 @@ extern "C" int bg_kv_cache_attn_fwd(const bg_kv_cache* cache, const void* data, 
   a.negate = scale < 0.f;
   const int64_t es = dtype == BG_F32 ? 4 : 2;
   a.q_vec = (((uintptr_t)q | (uintptr_t)(q_sb * es) | (uintptr_t)(q_sh * es) | (uintptr_t)(q_st * es)) & 15) == 0;
-  a.scale_log2 = (float)((scale < 0.f ? -(double)scale : (double)scale) * 1.4426950408889634);
+  const double unit = dtype == BG_F32 && cache->bits == 4 ? kv_unit<float, 4>() : 1.0;                 // of the scores
+  a.scale_log2 = (float)((scale < 0.f ? -(double)scale : (double)scale) * 1.4426950408889634 * unit);
   hipStream_t st = (hipStream_t)stream;
 #define BG_GO(BITS, DH)                                           \
   if (dtype == BG_F32) kv_attn_launch<float, BITS, DH>(a, p, st); \
