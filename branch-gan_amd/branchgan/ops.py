@@ -932,28 +932,35 @@ def kv_cache_attention(q, layer, start=None, counts=None, scale=None, max_keys=N
 # ---------------------------------------------------------------------------------------------------
 # Clipped policy loss with a KL term
 # ---------------------------------------------------------------------------------------------------
+def _logit_rows(t, V):
+    """(..., V) -> rows with a dense last dimension and a row stride of at least V (a copy for expanded or transposed ones)."""
+    if t.dim() != 2 or t.stride(1) != 1:
+        t = _rows_2d(t)
+    return t if t.stride(0) >= V or t.shape[0] == 1 else t.contiguous()
+
+
 class _PolicyLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, rows_f32, ref_logits, denominator, shape):
-        V = logits.shape[-1]
-        dense = lambda t: t if t.stride(0) >= V or t.shape[0] == 1 else t.contiguous()       # expanded rows
-        x = dense(_rows_2d(logits))
-        y = dense(_rows_2d(ref_logits)) if ref_logits is not None else None
-        rows, dev = x.shape[0], x.device
-        ids = ids.reshape(rows).to(torch.int64).contiguous()
-        flat = [None if t is None else _f32c(t) for t in rows_f32]
-        sh = C.PolicyShape(C.dtype_code(x), 0, rows, V, max(x.stride(0), V), max(y.stride(0), V) if y is not None else 0, *shape)
-        loss, lead = torch.empty((), dtype=torch.float32, device=dev), logits.shape[:-1]
-        logp, kl = torch.empty(lead, dtype=torch.float32, device=dev), torch.empty(lead, dtype=torch.float32, device=dev)
-        stats = torch.empty(rows * C.POLICY_STATS + 1, dtype=torch.float32, device=dev)
+        V, lead = logits.shape[-1], logits.shape[:-1]
+        x = _logit_rows(logits, V)
+        y = _logit_rows(ref_logits, V) if ref_logits is not None else None
+        rows = x.shape[0]
+        if ids.dtype != torch.int64 or not ids.is_contiguous():
+            ids = ids.to(torch.int64).contiguous()
+        flat = [None if t is None else _f32c(t) for t in rows_f32]           # kept until the launch
+        ctx.sh = sh = C.PolicyShape(C.dtype_code(x), 0, rows, V, max(x.stride(0), V), max(y.stride(0), V) if y is not None else 0, *shape)
+        f32 = torch.float32
+        loss, logp, kl = x.new_empty((), dtype=f32), x.new_empty(lead, dtype=f32), x.new_empty(lead, dtype=f32)
+        stats = x.new_empty(rows * C.POLICY_STATS + 1, dtype=f32)
         # the gradient for an incoming gradient of 1 comes out of the same reading of the logits; backward hands this buffer out
-        dx = torch.empty((rows, V), dtype=x.dtype, device=dev) if ctx.needs_input_grad[0] else None
+        dx = x.new_empty(logits.shape) if ctx.needs_input_grad[0] else None
         has = C.c_i32(0)
-        ptr = lambda t: None if t is None else t.data_ptr()
-        _launch("bg_policy_loss_fwd", dev, C.lib().bg_policy_loss_fwd, ctypes.byref(sh), x.data_ptr(), ptr(y), ids.data_ptr(), *[ptr(t) for t in flat],
-                ptr(denominator), loss.data_ptr(), logp.data_ptr(), kl.data_ptr(), stats.data_ptr(), ptr(dx), ctypes.byref(has))
+        _launch("bg_policy_loss_fwd", x.device, C.lib().bg_policy_loss_fwd, ctypes.byref(sh), x.data_ptr(), None if y is None else y.data_ptr(),
+                ids.data_ptr(), *[None if t is None else t.data_ptr() for t in flat], None if denominator is None else denominator.data_ptr(),
+                loss.data_ptr(), logp.data_ptr(), kl.data_ptr(), stats.data_ptr(), None if dx is None else dx.data_ptr(), ctypes.byref(has))
         ctx.save_for_backward(x, ids, stats, y)
-        ctx.dx, ctx.sh, ctx.in_shape = dx if has.value else None, sh, logits.shape
+        ctx.dx, ctx.in_shape = dx if has.value else None, logits.shape
         ctx.mark_non_differentiable(logp, kl)
         ctx.set_materialize_grads(False)              # no zeros for the outputs without a gradient
         return loss, logp, kl
@@ -968,10 +975,10 @@ class _PolicyLoss(torch.autograd.Function):
         dx, ctx.dx = ctx.dx, None                     # the buffer is handed out once: a second backward computes its own
         has = dx is not None
         if not has:
-            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            dx = x.new_empty(ctx.in_shape)
         _launch("bg_policy_loss_bwd", x.device, C.lib().bg_policy_loss_bwd, ctypes.byref(ctx.sh), x.data_ptr(), None if y is None else y.data_ptr(),
                 ids.data_ptr(), stats.data_ptr(), g.data_ptr(), dx.data_ptr(), int(has))
-        return dx.view(ctx.in_shape), None, None, None, None, None
+        return dx, None, None, None, None, None
 
 
 def policy_loss(logits, ids, old_logp, advantages, weights=None, ref_logp=None, ref_logits=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0,
@@ -982,12 +989,13 @@ def policy_loss(logits, ids, old_logp, advantages, weights=None, ref_logp=None, 
     sampled token, d = ref_logp - logp.  All log-probs are those of softmax(logits / temperature).  denominator: what the sum over tokens
     is divided by (a number, or a one-element tensor on the device - a token count over micro-batches or ranks); default the
     sum of the weights that count.  -> (loss fp32 scalar, logp (...), kl (...); the last two carry no gradient)."""
-    C.require_cuda(logits, ids, old_logp, advantages, weights, ref_logp, ref_logits)
+    C.require_cuda(logits)
     if logits.dim() < 2 or logits.numel() == 0:
         raise ValueError(f"policy_loss: logits must be (..., V) with at least one row, got {tuple(logits.shape)}")
+    lead, device = logits.shape[:-1], logits.device
     for name, t in (("ids", ids), ("old_logp", old_logp), ("advantages", advantages), ("weights", weights), ("ref_logp", ref_logp)):
-        if t is not None and (t.shape != logits.shape[:-1] or t.device != logits.device):
-            raise ValueError(f"policy_loss: {name} must be {tuple(logits.shape[:-1])} on {logits.device}, got {tuple(t.shape)} on {t.device}")
+        if t is not None and (t.shape != lead or t.device != device):
+            raise ValueError(f"policy_loss: {name} must be {tuple(lead)} on {device}, got {tuple(t.shape)} on {t.device}")
     if ids.is_floating_point() or ids.dtype == torch.bool:
         raise TypeError(f"policy_loss: ids must be integers, got {ids.dtype}")
     if ref_logits is not None and (ref_logits.shape != logits.shape or ref_logits.dtype != logits.dtype or ref_logits.device != logits.device):
