@@ -185,8 +185,8 @@ __device__ __forceinline__ void append_tiles(const KvArgs& a, const T* src0, int
   const int64_t hi64 = (int64_t)start + count;
   const int lo = start < 0 ? 0 : min(start, a.capacity), hi = (int)(hi64 < 0 ? 0 : (hi64 > a.capacity ? a.capacity : hi64));
   const int tile = lo / KV_TILE + (blk % blocks_per_head) * TPW + lt;
-  const int k0 = tile * KV_TILE;                               // (a capacity below 2^30 is required)
-  const bool any = k0 < hi && lo < hi;                         // tiles past the last token: nothing to do
+  const bool any = (int64_t)tile * KV_TILE < hi && lo < hi;    // tiles past the last token: nothing to do
+  const int k0 = any ? tile * KV_TILE : 0;
   const bool whole = k0 >= lo && k0 + KV_TILE <= hi;
   uint8_t* out = a.data + b * a.c_sb + h * a.c_sh + (int64_t)tile * L::BYTES;
   uint8_t* img = image + lt * PART;
@@ -342,8 +342,10 @@ int kv_check(const char* who, const bg_kv_cache* c, const void* data, int dtype,
              "%s: B=%d H=%d capacity=%d T=%lld", who, c->B, c->H, c->capacity, (long long)T);
   const int64_t tiles = cdiv(c->capacity, KV_TILE), bytes = tiles * (int64_t)bg_kv_cache_tile_bytes(c->bits, c->Dh);
   BG_REQUIRE(((uintptr_t)data & 15) == 0 && c->c_sb % 16 == 0 && c->c_sh % 16 == 0, "%s: the cache must lie on 16-byte boundaries", who);
-  BG_REQUIRE((c->H == 1 || c->c_sh >= bytes) && (c->B == 1 || c->c_sb >= bytes), "%s: cache strides %lld, %lld overlap (%lld bytes per head)", who,
-             (long long)c->c_sb, (long long)c->c_sh, (long long)bytes);
+  // no two (batch, head) share a byte: one of the two strides steps over all that the other reaches
+  const int64_t sb = c->B == 1 ? 0 : c->c_sb, sh = c->H == 1 ? 0 : c->c_sh;
+  BG_REQUIRE((c->H == 1 || sh >= bytes) && (c->B == 1 || sb >= bytes) && (c->H == 1 || c->B == 1 || sb - bytes >= (c->H - 1) * sh || sh - bytes >= (c->B - 1) * sb),
+             "%s: cache strides %lld, %lld overlap (%lld bytes per head)", who, (long long)c->c_sb, (long long)c->c_sh, (long long)bytes);
   return BG_OK;
 }
 

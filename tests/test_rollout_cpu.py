@@ -54,6 +54,24 @@ def test_cache_calls_refuse_before_any_launch():
     assert attn(cache_struct(), max_keys=0) == 1
 
 
+def test_caches_whose_heads_and_sequences_interleave_are_refused():
+    """Strides that keep neighbours apart and still let (1, 0) and (0, 1) share bytes; the two orders that do not are taken (as far
+    as the next check, here a missing output)."""
+    from branchgan import _capi
+    lib = _capi.lib()
+    p = ctypes.c_void_p(1 << 20)
+    bytes_ = -(-100 // 32) * lib.bg_kv_cache_tile_bytes(4, 64)
+    def read(c_sb, c_sh):
+        c = cache_struct(B=3, H=4, c_sb=c_sb, c_sh=c_sh)
+        rc = lib.bg_kv_cache_read(ctypes.byref(c), p, None, None, 1, 3, 0, 0, 64, None, None, None)
+        assert rc == 1
+        return lib.bg_last_error()
+    for sb, sh in ((bytes_, bytes_), (2 * bytes_, bytes_), (4 * bytes_ - 16, bytes_), (bytes_, 3 * bytes_ - 16), (5 * bytes_, 2 * bytes_)):
+        assert b"overlap" in read(sb, sh), (sb, sh)
+    for sb, sh in ((4 * bytes_, bytes_), (bytes_, 3 * bytes_), (7 * bytes_, 2 * bytes_), (4 * bytes_ + 64, bytes_)):
+        assert b"null k / v" in read(sb, sh), (sb, sh)
+
+
 def test_policy_calls_refuse_before_any_launch():
     from branchgan import _capi
     lib = _capi.lib()
