@@ -162,7 +162,8 @@ def clippedPolicyLoss(logits, ids, oldLogProbs, advantages, mask=None, refLogPro
     REINFORCE loss, ReinforceLoss.py:21-52, is on-policy): with ratio = exp(logp - oldLogProbs),
         max(-advantages * ratio, -advantages * clamp(ratio, 1 - clipRange[0], 1 + clipRange[1])) + klWeight * KL(policy | reference),
     summed over the tokens mask counts and divided by their number (or by denominator).  What to use for tokens that
-    `generate(..., return_logprobs=True)` sampled - behind a quantised cache, some optimizer steps ago, or both.  One reading of
-    the logits forward, one backward (bg_policy_loss_*).  -> (loss, logProbs, kl), the last two per token, without gradient."""
+    `generate(..., return_logprobs=True)` sampled - behind a quantised cache, some optimizer steps ago, or both.  Value and gradient
+    come from one reading of the logits (bg_policy_loss_*); a loss that is scaled before its backward costs another one, so scale
+    through denominator, mask or advantages.  -> (loss, logProbs, kl), the last two per token, without gradient."""
     return ops.policy_loss(logits, ids, oldLogProbs, advantages, weights=mask, ref_logp=refLogProbs, ref_logits=refLogits,
                            clip_low=clipRange[0], clip_high=clipRange[1], kl_coef=klWeight, temperature=temperature, denominator=denominator)

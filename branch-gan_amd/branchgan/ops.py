@@ -988,7 +988,9 @@ def policy_loss(logits, ids, old_logp, advantages, weights=None, ref_logp=None, 
     0 = does not count; ref_logits (like logits) -> the KL over the vocabulary, or ref_logp (...) -> exp(d) - d - 1 of the
     sampled token, d = ref_logp - logp.  All log-probs are those of softmax(logits / temperature).  denominator: what the sum over tokens
     is divided by (a number, or a one-element tensor on the device - a token count over micro-batches or ranks); default the
-    sum of the weights that count.  -> (loss fp32 scalar, logp (...), kl (...); the last two carry no gradient)."""
+    sum of the weights that count.  -> (loss fp32 scalar, logp (...), kl (...); the last two carry no gradient).
+    Captured into a HIP graph, forward and backward belong into the same capture, made while no eager autograd graph of the same
+    leaves is alive (autograd binds a leaf's gradient to the stream of its first use: graphs.GraphedTrainStep)."""
     C.require_cuda(logits)
     if logits.dim() < 2 or logits.numel() == 0:
         raise ValueError(f"policy_loss: logits must be (..., V) with at least one row, got {tuple(logits.shape)}")

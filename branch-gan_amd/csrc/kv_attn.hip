@@ -20,7 +20,12 @@
 //   the usual turn needs no exchange between lanes for it.
 // Work.  Four waves per workgroup take turns round robin; the key range is split over workgroups when there are too few of
 //   them to fill 256 CUs (kv_attn_plan), the partial states joined by a second kernel.
-// Bound by HBM: 0.5625 or 1.0625 bytes per cached value.
+// Bound.  One token: HBM, 0.5625 or 1.0625 bytes per cached value.  Measured: 8 sequences of 65537 keys, 8 heads of 128, four query heads
+//   each, 4 bits, 604 MB in 115 us (5.3 TB/s; the launches of the call included, the part that stays in the last-level cache too);
+//   64 uneven sequences of up to 2047 keys, 16 heads of 64, 87 MB in 21 us (4.2 TB/s); 16 of up to 4001, 8 heads of 256, 8 bits,
+//   float32 queries, 162 MB in 41 + 5 us (3.5 TB/s: the longest sequences finish alone).  Many rows: vector work - 128 keys x 16 rows
+//   of 64 channels are some 930 vector instructions of a wave (exponentials, scales, splitting P, unpacking) against 64 matrix
+//   ones; 67 tokens of 4 sequences of 16 heads against about 2000 keys in 19 + 4 us.
 #include "kv_cache.h"
 
 namespace bg {
@@ -812,8 +817,9 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(KvAttnArgs a, uint32_
 }
 
 // Which kernel, and how many workgroups share a row tile's key range: enough to give every CU two (512), none with less than one turn for
-// each wave.  (Even splits of every sequence: splits of a fixed number of turns, fewer for short sequences, leave CUs idle - 16
-// uneven sequences of 8 heads, 8 bits, 67 against 79 us.)
+// each wave.  512 is what is resident at once: 640, 768 and 1024 took 140, 127 and 121 us against 116 for 8 sequences of 65537 keys
+// (8 heads of 128, 4 bits), 58, 60 and 56 against 50 for 16 uneven ones of up to 4001 (8 heads of 256, 8 bits).  Every sequence
+// is split evenly: splits of a fixed number of turns, fewer for short sequences, leave CUs idle and were a sixth slower.
 struct KvPlan {
   int pairs;                                 // (row, channel group) pairs per cache head; more than 16: kv_attn_kernel
   int row_tiles, splits;

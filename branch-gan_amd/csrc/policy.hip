@@ -10,6 +10,8 @@
 // whole of value and gradient is logits in, dlogits out.  The gradient is the one for g_loss = 1; bg_policy_loss_bwd does it over
 // when the loss was scaled after all.  Rows too long for the registers take policy_rows_kernel (forward) and policy_grad_kernel
 // (backward), one more reading of the logits.
+// Measured, bf16 with the gradient: 2047 rows of 50257 in 93 us (4.4 TB/s), 8184 rows of 50304 with a reference in 612 us (4.0
+// TB/s; a copy reaches 4.8); the weights' sum and the total take 5 us each at 2047 rows, a backward call with nothing to do 4.
 #include "common.h"
 
 namespace bg {
@@ -461,8 +463,9 @@ static PolicyArgs policy_args(const bg_policy_shape* sh, const void* logits, con
   return a;
 }
 
-// Rows of at most NT * NV vectors.  Few threads for short rows; for the usual vocabularies
-// 512, so that two rows share a CU and one's loads cover the other's exponentials.
+// Rows of at most NT * NV vectors.  Few threads for short rows; for the usual vocabularies 512, so that two rows share a CU and one's
+// loads cover the other's exponentials (with a reference its two rows spill a part of themselves at 128 registers; 1024 x 7 vectors,
+// 768 x 9, 256 x 26 and fewer waves with more registers were all slower).
 template <typename T, bool REF> static bool policy_row_launch(const PolicyArgs& a, const float* denominator, T* dlogits, hipStream_t st) {
   const int64_t nvec = a.V / Vec<T>::N + 1;
   if (a.V < 2 * Vec<T>::N) return false;

@@ -491,7 +491,7 @@ int bg_graph_replace_memset_nodes(void* graph, int* n_replaced);
  * 2^127 reads as NaN.  A value takes 0.5625 (1.0625) bytes.
  *
  * The cache is one byte buffer: per (batch, head) ceil(capacity / 32) tiles of bg_kv_cache_tile_bytes(bits, Dh) bytes, c_sb /
- * c_sh BYTES apart (multiples of 16; the buffer itself on a 16-byte boundary).  The order of codes and scales inside a tile is
+ * c_sh BYTES apart (multiples of 16; the buffer itself on a 16-byte boundary; no two (batch, head) share a byte).  The order of codes and scales inside a tile is
  * the library's own: use bg_kv_cache_read to see values.  Dh: 32, 64, 128 or 256.
  *
  * start (int32 (B), NULL = 0 everywhere): tokens each sequence held before the call.  counts (int32 (B), NULL = T everywhere): how
@@ -538,8 +538,9 @@ int bg_kv_cache_attn_fwd(const bg_kv_cache* cache, const void* data, const void*
  * kl are 0, its gradient is 0.  A logit of -inf (or the type's lowest value) has probability 0 and adds nothing to the KL.
  * _fwd writes out_loss (1 float), out_logp / out_kl (rows) and stats (rows x BG_POLICY_STATS + 1 floats on
  * an 8-byte boundary: what _bwd needs);  _bwd writes dlogits ([rows][V], dtype of logits) = *g_loss * dloss / dlogits.
- * _fwd takes dlogits too (NULL: value only): rows that fit a workgroup's registers (V up to 106480 in bf16, 53240 in fp32) leave their
- * gradient for g_loss = 1 there on the same reading of the logits, and *has_gradient (host) is 1.  Handed on to _bwd with that
+ * _fwd takes dlogits too (NULL: value only): rows that fit a workgroup's registers (V up to 106495 in bf16, 53247 in fp32; all
+ * three of logits, ref_logits and dlogits alike on the 16-byte grid) leave their gradient for g_loss = 1 there on the same reading
+ * of the logits, and *has_gradient (host) is 1.  Handed on to _bwd with that
  * buffer it makes _bwd end at once when *g_loss is 1; any other value computes the gradient from the logits again.
  */
 #define BG_POLICY_STATS 8
