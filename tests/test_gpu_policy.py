@@ -294,6 +294,44 @@ def test_rollouts_over_a_quantised_cache_and_the_update_on_them():
     assert lm.embed_out.weight.grad is not None and bool(lm.embed_out.weight.grad.isfinite().all()) and bool(lm.embed_out.weight.grad.any())
 
 
+def test_prompt_positions_left_out_by_weight_or_by_slice():
+    """The logits of a whole sequence with weight 0 on its prompt, or their slice: the same rows, the same value and gradient; what the
+    rows left out hold does not matter."""
+    from branchgan import losses
+    g = torch.Generator().manual_seed(71)
+    B, S, P, V = 3, 9, 4, 1003
+    logits, ref = [torch.randn((B, S, V), generator=g).to(torch.bfloat16).cuda() for _ in range(2)]
+    ids = torch.randint(0, V, (B, S), generator=g).cuda()
+    old, adv = [(torch.randn((B, S - P), generator=g) - c).cuda() for c in (7.0, 0.0)]
+    behind = lambda t: torch.nn.functional.pad(t, (P, 0))
+    x = logits.clone().requires_grad_(True)
+    want = losses.clippedPolicyLoss(x[:, P:], ids[:, P:], old, adv, refLogits=ref[:, P:], klWeight=0.1)
+    want[0].backward()
+    broken = [t.clone() for t in (logits, ref)]
+    for t in broken:
+        t[:, :P] = float("nan")
+    y = broken[0].requires_grad_(True)
+    got = losses.clippedPolicyLoss(y, ids, behind(old), behind(adv), mask=behind(torch.ones_like(old)), refLogits=broken[1], klWeight=0.1)
+    got[0].backward()
+    # Not bit for bit: V is odd, so a row lies elsewhere on the 16-byte grid in the copy that the slice becomes, and its elements fall to
+    # other threads.  A thread adds at most 17 terms in fp32 (two vectors of 8 and a single one), so each of the three sums s, s', t is off
+    # by at most 17 u of its terms' magnitudes, u = 2^-24, in either call; everything behind them is fp64 or the same operation.
+    #   log s: 17 u.   logp: that, and its rounding (|logp| < 16).   kl = t / s - (log s - log s'): with |difference of two logits| <= D
+    #   in every term, 17 u D from t, 17 u D from s, 34 u from the logs, rounding u |kl|.
+    u, D = 2.0 ** -24, float((logits - ref).float().abs().max() + (logits.float().amax(-1) - ref.float().amax(-1)).abs().max())
+    e_logp, e_kl = 2 * (17 + 16) * u, 2 * (34 * D + 34 + 2) * u
+    assert float((got[1][:, P:] - want[1]).abs().max()) <= e_logp and float((got[2][:, P:] - want[2]).abs().max()) <= e_kl
+    # a row's term A ratio moves by ratio (e_logp + 4 u) (expf, the product, the ratio's argument rounded to fp32: |argument| < 8)
+    A_r = (adv.abs() * (want[1] - old).exp()).max()
+    assert abs(float((got[0] - want[0]).detach())) <= float(A_r) * (e_logp + 12 * u) + 0.1 * e_kl + abs(float(want[0].detach())) * u
+    # a logit's gradient is p / N (slope and 0.1 (difference - off)), then bf16: neighbours at most (2^-7 of the value), and where the parts cancel,
+    # p / N times what slope, off (both e_kl and e_logp at most, as above) and p (relative 17 u, 3 more operations) moved
+    p_max = float(torch.softmax(logits.float(), -1).max())
+    moved = p_max / (B * (S - P)) * (float(A_r) * (e_logp + 32 * u) + 0.1 * (e_kl + D * 40 * u))
+    torch.testing.assert_close(y.grad.float(), x.grad.float(), rtol=2.0 ** -7, atol=moved)
+    assert not y.grad[:, :P].any()
+
+
 def test_refusals():
     from branchgan import ops
     d = inputs(4, 50, torch.float32, 53, "logits")
