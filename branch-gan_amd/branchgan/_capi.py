@@ -55,7 +55,8 @@ class KvCache(ctypes.Structure):
 
 class PolicyShape(ctypes.Structure):
     _fields_ = [("dtype", c_i32), ("reserved", c_i32), ("rows", c_i64), ("V", c_i64), ("x_stride", c_i64), ("ref_stride", c_i64),
-                ("temperature", c_f64), ("clip_low", c_f64), ("clip_high", c_f64), ("kl_coef", c_f64)]
+                ("temperature", c_f64), ("clip_low", c_f64), ("clip_high", c_f64), ("kl_coef", c_f64),
+                ("inner", c_i64), ("x_outer", c_i64), ("ref_outer", c_i64), ("d_outer", c_i64)]
 
 
 class ReduceDesc(ctypes.Structure):

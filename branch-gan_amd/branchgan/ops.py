@@ -933,34 +933,58 @@ def kv_cache_attention(q, layer, start=None, counts=None, scale=None, max_keys=N
 # Clipped policy loss with a KL term
 # ---------------------------------------------------------------------------------------------------
 def _logit_rows(t, V):
-    """(..., V) -> rows with a dense last dimension and a row stride of at least V (a copy for expanded or transposed ones)."""
+    """(..., V) -> t or a copy of it whose rows the kernels can walk, rows per group, row stride, group stride.  (B, T, V) with a
+    dense last dimension - also a slice along T, or (T, B, V) transposed - needs no copy."""
+    if t.dim() == 3:
+        if t.stride(2) != 1 or (t.stride(1) < V and t.shape[1] > 1):
+            t = t.contiguous()
+        return t, t.shape[1], max(t.stride(1), V), t.stride(0)
     if t.dim() != 2 or t.stride(1) != 1:
         t = _rows_2d(t)
-    return t if t.stride(0) >= V or t.shape[0] == 1 else t.contiguous()
+    if t.stride(0) < V and t.shape[0] > 1:
+        t = t.contiguous()
+    return t, t.shape[0], max(t.stride(0), V), 0
+
+
+def _gradient_rows(x, shape, inner, stride, outer, V):
+    """Uninitialised gradient of that shape and its group stride: rows V apart, on the 16-byte grid as x's are where they can be (the
+    kernel that holds a row in registers reads and writes it by the same whole vectors)."""
+    n = 16 // x.element_size()
+    off, pad = x.data_ptr() % 16 // x.element_size(), 0
+    if len(shape) == 3 and shape[0] > 1:
+        pad = (outer - inner * V) % n
+    if (off == 0 and pad == 0) or (stride - V) % n:
+        return x.new_empty(shape), inner * V
+    if pad == 0:
+        return x.new_empty(off + shape.numel())[off:].view(shape), inner * V
+    d_outer = inner * V + pad
+    return x.new_empty(off + shape[0] * d_outer).as_strided(shape, (d_outer, V, 1), off), d_outer
 
 
 class _PolicyLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, rows_f32, ref_logits, denominator, shape):
         V, lead = logits.shape[-1], logits.shape[:-1]
-        x = _logit_rows(logits, V)
-        y = _logit_rows(ref_logits, V) if ref_logits is not None else None
-        rows = x.shape[0]
+        x, inner, x_stride, x_outer = _logit_rows(logits, V)
+        y, _, y_stride, y_outer = _logit_rows(ref_logits, V) if ref_logits is not None else (None, 0, 0, 0)
+        rows = logits.numel() // V
         if ids.dtype != torch.int64 or not ids.is_contiguous():
             ids = ids.to(torch.int64).contiguous()
         flat = [None if t is None else _f32c(t) for t in rows_f32]           # kept until the launch
-        ctx.sh = sh = C.PolicyShape(C.dtype_code(x), 0, rows, V, max(x.stride(0), V), max(y.stride(0), V) if y is not None else 0, *shape)
+        # the gradient for an incoming gradient of 1 comes out of the same reading of the logits; backward hands this buffer out
+        ctx.rows = logits.shape, inner, x_stride, x_outer, V
+        dx, d_outer = _gradient_rows(x, *ctx.rows) if ctx.needs_input_grad[0] else (None, inner * V)
+        ctx.sh = sh = C.PolicyShape(C.dtype_code(x), 0, rows, V, x_stride, y_stride, *shape, inner, x_outer, y_outer, d_outer)
         f32 = torch.float32
         loss, logp, kl = x.new_empty((), dtype=f32), x.new_empty(lead, dtype=f32), x.new_empty(lead, dtype=f32)
         stats = x.new_empty(rows * C.POLICY_STATS + 1, dtype=f32)
-        # the gradient for an incoming gradient of 1 comes out of the same reading of the logits; backward hands this buffer out
-        dx = x.new_empty(logits.shape) if ctx.needs_input_grad[0] else None
         has = C.c_i32(0)
         _launch("bg_policy_loss_fwd", x.device, C.lib().bg_policy_loss_fwd, ctypes.byref(sh), x.data_ptr(), None if y is None else y.data_ptr(),
                 ids.data_ptr(), *[None if t is None else t.data_ptr() for t in flat], None if denominator is None else denominator.data_ptr(),
                 loss.data_ptr(), logp.data_ptr(), kl.data_ptr(), stats.data_ptr(), None if dx is None else dx.data_ptr(), ctypes.byref(has))
         ctx.save_for_backward(x, ids, stats, y)
-        ctx.dx, ctx.in_shape = dx if has.value else None, logits.shape
+        ctx.strides = x.stride(), None if y is None else y.stride()
+        ctx.dx = dx if has.value else None
         ctx.mark_non_differentiable(logp, kl)
         ctx.set_materialize_grads(False)              # no zeros for the outputs without a gradient
         return loss, logp, kl
@@ -971,19 +995,25 @@ class _PolicyLoss(torch.autograd.Function):
         if g_loss is None:
             return (None,) * 6
         x, ids, stats, y = ctx.saved_tensors
+        V, sh = ctx.rows[-1], ctx.sh
+        if x.stride() != ctx.strides[0] or (y is not None and y.stride() != ctx.strides[1]):      # saved-tensor hooks may return another layout
+            x, _, sh.x_stride, sh.x_outer = _logit_rows(x, V)
+            if y is not None:
+                y, _, sh.ref_stride, sh.ref_outer = _logit_rows(y, V)
         g = g_loss if g_loss.dtype == torch.float32 else g_loss.float()
         dx, ctx.dx = ctx.dx, None                     # the buffer is handed out once: a second backward computes its own
         has = dx is not None
         if not has:
-            dx = x.new_empty(ctx.in_shape)
-        _launch("bg_policy_loss_bwd", x.device, C.lib().bg_policy_loss_bwd, ctypes.byref(ctx.sh), x.data_ptr(), None if y is None else y.data_ptr(),
+            dx = _gradient_rows(x, *ctx.rows)[0]
+        _launch("bg_policy_loss_bwd", x.device, C.lib().bg_policy_loss_bwd, ctypes.byref(sh), x.data_ptr(), None if y is None else y.data_ptr(),
                 ids.data_ptr(), stats.data_ptr(), g.data_ptr(), dx.data_ptr(), int(has))
         return dx, None, None, None, None, None
 
 
 def policy_loss(logits, ids, old_logp, advantages, weights=None, ref_logp=None, ref_logits=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0,
                 temperature=1.0, denominator=None):
-    """Clipped policy loss with a KL term (bg_policy_loss_*), differentiable in logits (..., V) fp32 / bf16.  ids (...) int64: the
+    """Clipped policy loss with a KL term (bg_policy_loss_*), differentiable in logits (..., V) fp32 / bf16 (a slice of (B, T, V) along T,
+    e.g. logits[:, :-1], is read where it lies).  ids (...) int64: the
     sampled tokens; old_logp (...): their log-probs when they were sampled; advantages (...); weights (...) or None: per token,
     0 = does not count; ref_logits (like logits) -> the KL over the vocabulary, or ref_logp (...) -> exp(d) - d - 1 of the
     sampled token, d = ref_logp - logp.  All log-probs are those of softmax(logits / temperature).  denominator: what the sum over tokens

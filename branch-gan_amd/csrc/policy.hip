@@ -38,13 +38,20 @@ struct PolicyArgs {
   const float* ref_logp;
   const float* adv;
   const float* weights;
-  int64_t rows, V, x_stride, ref_stride;
+  int64_t rows, V, x_stride, ref_stride, x_outer, ref_outer, d_outer;
+  uint32_t inner;            // rows per group
   double inv_t, clip_low, clip_high, kl_coef;
   float c_hi, c_lo, inv_t32;
   float* out_logp;
   float* out_kl;
   float* stats;              // per row: m, 1 / s, w dloss_row/dlogp, w kl_coef, log s - log s' + kl, m', w loss_row (a double);  then 1 / N
 };
+
+// where a row starts: rows of a group lie one stride apart, groups one outer stride
+__device__ __forceinline__ int64_t row_at(const PolicyArgs& a, int64_t row, int64_t stride, int64_t outer) {
+  const uint32_t group = (uint32_t)row / a.inner;
+  return group * outer + ((uint32_t)row - group * a.inner) * stride;
+}
 
 // 2^(d c), d <= 0.  c_hi < c, so that c_lo > 0 and d = -inf gives 0, not a NaN.
 __device__ __forceinline__ float policy_exp(float d, float c_hi, float c_lo) {
@@ -229,9 +236,9 @@ __global__ __launch_bounds__(NT, 4) void policy_row_kernel(PolicyArgs a, const f
   __shared__ float sh_inv_n;
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x;
-  const T* x = (const T*)a.logits + row * a.x_stride;
-  const T* y = REF ? (const T*)a.ref + row * a.ref_stride : nullptr;
-  T* dx = dlogits ? dlogits + row * a.V : nullptr;
+  const T* x = (const T*)a.logits + row_at(a, row, a.x_stride, a.x_outer);
+  const T* y = REF ? (const T*)a.ref + row_at(a, row, a.ref_stride, a.ref_outer) : nullptr;
+  T* dx = dlogits ? dlogits + row_at(a, row, a.V, a.d_outer) : nullptr;
   const int V = (int)a.V, mis = misalignment<T>(x);
   const float w = row_weight(a, row);
   if (w == 0.f) {
@@ -352,8 +359,8 @@ __global__ __launch_bounds__(PT) void policy_rows_kernel(PolicyArgs a) {
     skip_row(a, row);
     return;
   }
-  const T* x = (const T*)a.logits + row * a.x_stride;
-  const T* y = REF ? (const T*)a.ref + row * a.ref_stride : nullptr;
+  const T* x = (const T*)a.logits + row_at(a, row, a.x_stride, a.x_outer);
+  const T* y = REF ? (const T*)a.ref + row_at(a, row, a.ref_stride, a.ref_outer) : nullptr;
   const int mis = misalignment<T>(x);
   const bool y_on = !REF || misalignment<T>(y) == mis;
   const int64_t id = a.ids[row];
@@ -407,9 +414,9 @@ __global__ __launch_bounds__(PT) void policy_grad_kernel(PolicyArgs a, const flo
   if (unless_one && g == 1.f) return;
   const int tid = threadIdx.x;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    T* dx = dlogits + row * a.V;
-    const T* x = (const T*)a.logits + row * a.x_stride;
-    const T* y = REF ? (const T*)a.ref + row * a.ref_stride : nullptr;
+    T* dx = dlogits + row_at(a, row, a.V, a.d_outer);
+    const T* x = (const T*)a.logits + row_at(a, row, a.x_stride, a.x_outer);
+    const T* y = REF ? (const T*)a.ref + row_at(a, row, a.ref_stride, a.ref_outer) : nullptr;
     const int mis = misalignment<T>(x);
     const bool y_on = !REF || misalignment<T>(y) == mis, d_on = misalignment<T>(dx) == mis;
     const float* st = a.stats + row * BG_POLICY_STATS;
@@ -445,6 +452,11 @@ static int policy_check(const char* who, const bg_policy_shape* sh, const void* 
   BG_REQUIRE(sh->rows > 0 && sh->rows < (1ll << 31) && sh->V > 0 && sh->V < (1ll << 31) && sh->x_stride >= sh->V, "%s: rows=%lld V=%lld stride=%lld",
              who, (long long)sh->rows, (long long)sh->V, (long long)sh->x_stride);
   BG_REQUIRE(!ref || sh->ref_stride >= sh->V, "%s: reference stride %lld", who, (long long)sh->ref_stride);
+  BG_REQUIRE(sh->inner >= 0 && (sh->inner == 0 || sh->rows % sh->inner == 0), "%s: groups of %lld of %lld rows", who, (long long)sh->inner,
+             (long long)sh->rows);
+  if (sh->inner > 0 && sh->inner < sh->rows)
+    BG_REQUIRE(sh->x_outer >= 0 && (!ref || sh->ref_outer >= 0) && sh->d_outer >= sh->inner * sh->V, "%s: group strides %lld, %lld, %lld", who,
+               (long long)sh->x_outer, (long long)sh->ref_outer, (long long)sh->d_outer);
   BG_REQUIRE(sh->temperature > 0.0 && sh->temperature < 1e6 && sh->temperature > 1e-6, "%s: temperature %g", who, sh->temperature);
   BG_REQUIRE(sh->clip_low >= 0.0 && sh->clip_high >= 0.0, "%s: clip range %g, %g", who, sh->clip_low, sh->clip_high);
   return BG_OK;
@@ -454,6 +466,8 @@ static PolicyArgs policy_args(const bg_policy_shape* sh, const void* logits, con
   PolicyArgs a = {};
   a.logits = logits; a.ref = ref; a.ids = ids; a.stats = stats;
   a.rows = sh->rows; a.V = sh->V; a.x_stride = sh->x_stride; a.ref_stride = sh->ref_stride;
+  a.inner = (uint32_t)(sh->inner ? sh->inner : sh->rows);
+  if (a.inner < a.rows) { a.x_outer = sh->x_outer; a.ref_outer = sh->ref_outer; a.d_outer = sh->d_outer; }
   a.inv_t = 1.0 / sh->temperature;
   a.clip_low = sh->clip_low; a.clip_high = sh->clip_high; a.kl_coef = sh->kl_coef;
   const double c = 1.4426950408889634 / sh->temperature;
@@ -470,11 +484,12 @@ template <typename T, bool REF> static bool policy_row_launch(const PolicyArgs& 
   const int64_t nvec = a.V / Vec<T>::N + 1;
   if (a.V < 2 * Vec<T>::N) return false;
   // reference or gradient rows that lie elsewhere on the 16-byte grid than the logits': the streaming kernels
-  const auto same_grid = [&](const void* p, int64_t stride) {
-    return (((uintptr_t)a.logits ^ (uintptr_t)p) & 15) == 0 && (a.x_stride - stride) * (int64_t)sizeof(T) % 16 == 0;
+  const auto same_grid = [&](const void* p, int64_t stride, int64_t outer) {
+    return (((uintptr_t)a.logits ^ (uintptr_t)p) & 15) == 0 && (a.x_stride - stride) * (int64_t)sizeof(T) % 16 == 0 &&
+           (a.x_outer - outer) * (int64_t)sizeof(T) % 16 == 0;
   };
-  if (REF && !same_grid(a.ref, a.ref_stride)) return false;
-  if (dlogits && !same_grid(dlogits, a.V)) return false;
+  if (REF && !same_grid(a.ref, a.ref_stride, a.ref_outer)) return false;
+  if (dlogits && !same_grid(dlogits, a.V, a.d_outer)) return false;
   const dim3 grid((unsigned)a.rows);
   if (nvec <= 256 * 2) hipLaunchKernelGGL((policy_row_kernel<T, REF, 256, 2>), grid, dim3(256), 0, st, a, denominator, dlogits);
   else if (nvec <= 256 * 8) hipLaunchKernelGGL((policy_row_kernel<T, REF, 256, 8>), grid, dim3(256), 0, st, a, denominator, dlogits);

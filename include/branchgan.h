@@ -534,10 +534,12 @@ int bg_kv_cache_attn_fwd(const bg_kv_cache* cache, const void* data, const void*
  *        = exp(d) - d - 1, d = ref_logp[r] - logp                             when ref_logp is given, 0 with neither,
  *   loss = sum_r w_r (pg + kl_coef kl) / N,  N = *denominator, or sum_r w_r over the rows that count when it is NULL
  *          (N = 0: loss and gradient are 0).
+ * Rows lie in groups of `inner` (0: one group): row r of logits at (r / inner) x_outer + (r % inner) x_stride elements, ref_logits alike;
+ * dlogits at (r / inner) d_outer + (r % inner) V, d_outer >= inner V.  The outer strides of a single group are not looked at.
  * weights (fp32, NULL = 1): a row with weight 0 or an id outside [0, V) does not count - its logits are not read, its logp and
  * kl are 0, its gradient is 0.  A logit of -inf (or the type's lowest value) has probability 0 and adds nothing to the KL.
  * _fwd writes out_loss (1 float), out_logp / out_kl (rows) and stats (rows x BG_POLICY_STATS + 1 floats on
- * an 8-byte boundary: what _bwd needs);  _bwd writes dlogits ([rows][V], dtype of logits) = *g_loss * dloss / dlogits.
+ * an 8-byte boundary: what _bwd needs);  _bwd writes dlogits (dtype of logits) = *g_loss * dloss / dlogits.
  * _fwd takes dlogits too (NULL: value only): rows that fit a workgroup's registers (V up to 106495 in bf16, 53247 in fp32; all
  * three of logits, ref_logits and dlogits alike on the 16-byte grid) leave their gradient for g_loss = 1 there on the same reading
  * of the logits, and *has_gradient (host) is 1.  Handed on to _bwd with that
@@ -548,6 +550,7 @@ typedef struct {
   int dtype, reserved;
   int64_t rows, V, x_stride, ref_stride;
   double temperature, clip_low, clip_high, kl_coef;
+  int64_t inner, x_outer, ref_outer, d_outer;
 } bg_policy_shape;
 int bg_policy_loss_fwd(const bg_policy_shape* sh, const void* logits, const void* ref_logits, const int64_t* ids, const float* old_logp,
                        const float* ref_logp, const float* advantages, const float* weights, const float* denominator,

@@ -3,6 +3,7 @@
 Tolerances, derived.  An exponential is off by |z| 2^-23 (the roundings of its argument z = (logit - max) / T, of which only |z| < 30
 matters: below it p < 1e-13) + 2^-21 (the instruction); the sum of V of them, V / 256 in a row and a tree of ten, by (V / 256 + 16)
 2^-24.  So  del = 34 * 2^-23 + (V / 256 + 16) 2^-24  bounds the relative error of every p and the absolute error of logp (which is then rounded: 2^-24 |logp|)."""
+import contextlib
 import math
 
 import pytest
@@ -40,10 +41,12 @@ def off_the_clip(d, temperature, low, high):
     return d
 
 
-def run(d, g=1.0, **kw):
+def run(d, g=1.0, place=None, **kw):
     from branchgan import losses
     names = dict(weights="mask", ref_logp="refLogProbs", ref_logits="refLogits")
     dev = {k: v.cuda() for k, v in d.items()}
+    if place is not None:
+        return run_placed(dev, g, place, names, kw)
     x = dev.pop("logits").requires_grad_(True)
     ids, old, adv = dev.pop("ids"), dev.pop("old_logp"), dev.pop("advantages")
     loss, logp, kl = losses.clippedPolicyLoss(x, ids, old, adv, **{names[k]: v for k, v in dev.items()}, clipRange=(kw.get("clip_low", 0.2), kw.get("clip_high", 0.2)),
@@ -52,11 +55,41 @@ def run(d, g=1.0, **kw):
     return loss.detach().cpu(), logp.cpu(), kl.cpu(), x.grad
 
 
+def run_placed(dev, g, place, names, kw):
+    """place(rows, V) -> (shape of a larger tensor, view(that tensor) holding the rows as (..., V), whether the reference lies alike)."""
+    from branchgan import losses
+    rows, V = dev["logits"].shape
+    shape, view, alike = place(rows, V)
+    def lay(t):
+        full = torch.full(shape, float("nan"), dtype=t.dtype, device="cuda")
+        view(full).copy_(t.view(view(full).shape))
+        return full
+    leaf = lay(dev.pop("logits")).requires_grad_(True)
+    x = view(leaf)
+    if "ref_logits" in dev:
+        dev["ref_logits"] = view(lay(dev["ref_logits"])) if alike else dev["ref_logits"].view(x.shape)
+    dev = {k: t if k == "ref_logits" else t.view(x.shape[:-1]) for k, t in dev.items()}
+    ids, old, adv = dev.pop("ids"), dev.pop("old_logp"), dev.pop("advantages")
+    loss, logp, kl = losses.clippedPolicyLoss(x, ids, old, adv, **{names[k]: v for k, v in dev.items()}, klWeight=kw.get("kl_coef", 0.0),
+                                              temperature=kw.get("temperature", 1.0))
+    if x.dim() < 4:
+        assert loss.grad_fn.saved_tensors[0].data_ptr() == x.data_ptr()             # read where it lies
+    first, = torch.autograd.grad(loss, leaf, retain_graph=True)
+    (loss * g).backward()
+    grad = view(leaf.grad).reshape(rows, V)
+    if g == 1.0:                                                                    # the gradient of the forward's reading, and the one computed again
+        torch.testing.assert_close(first, leaf.grad, rtol=2 * torch.finfo(x.dtype).eps if x.dtype == torch.bfloat16 else 1e-4, atol=1e-7)
+    outside = leaf.grad.clone()
+    view(outside).zero_()
+    assert not outside.any()
+    return loss.detach().cpu(), logp.reshape(-1).cpu(), kl.reshape(-1).cpu(), grad
+
+
 def check(d, g=1.0, **kw):
     T, beta = kw.get("temperature", 1.0), kw.get("kl_coef", 0.0)
     x = d["logits"].double().requires_grad_(True)
     ref = {k: v for k, v in d.items() if k != "logits"}
-    loss, logp, kl = O.policy_loss(x, **ref, **kw)
+    loss, logp, kl = O.policy_loss(x, **ref, **{k: v for k, v in kw.items() if k != "place"})
     (loss * g).backward()
     got_loss, got_logp, got_kl, grad = run(d, g, **kw)
     rows, V = d["logits"].shape
@@ -188,6 +221,48 @@ def test_strides_leading_dimensions_and_integer_types():
     rep = x[:1].repeat(12, 1).requires_grad_(True)
     ops.policy_loss(rep, *args((12,)))[0].backward()
     torch.testing.assert_close(one.grad[0], rep.grad.sum(0), rtol=1e-5, atol=1e-8)
+
+
+PLACES = {
+    "shifted": lambda R, V: ((3, R // 3 + 1, V), lambda t: t[:, :-1], True),                  # logits[:, :-1]
+    "middle": lambda R, V: ((3, R // 3 + 5, V), lambda t: t[:, 2:-3], True),
+    "middle_ref_dense": lambda R, V: ((3, R // 3 + 5, V), lambda t: t[:, 2:-3], False),
+    "transposed": lambda R, V: ((R // 3, 3, V), lambda t: t.transpose(0, 1), True),
+    "one_token": lambda R, V: ((R, 4, V), lambda t: t[:, 1:2], True),
+    "one_sequence": lambda R, V: ((2, R + 3, V), lambda t: t[1:, 1:-2], True),
+    "rows": lambda R, V: ((R + 4, V), lambda t: t[3:-1], True),
+    "wide": lambda R, V: ((3, R // 3 + 1, V + 9), lambda t: t[:, 1:, 4:-5], True),
+    "four_dimensions": lambda R, V: ((3, R // 6, 3, V), lambda t: t[:, :, 1:], True),
+}
+
+
+@pytest.mark.parametrize("place", PLACES)
+@pytest.mark.parametrize("V,dtype", [(1031, torch.bfloat16), (2048, torch.bfloat16), (1031, torch.float32), (20001, torch.bfloat16), (13, torch.float32)])
+@pytest.mark.parametrize("ref,g", [("logits", 1.0), ("logp", 1.0), ("logits", 0.7)])
+def test_rows_where_they_lie(place, V, dtype, ref, g):
+    """Slices and transpositions of (B, T, V), against float64; what lies around the rows is NaN and gets no gradient."""
+    d = off_the_clip(inputs(12, V, dtype, 83, ref), 0.8, 0.2, 0.2)
+    check(d, g, place=PLACES[place], kl_coef=0.1, temperature=0.8)
+
+
+@pytest.mark.parametrize("g", [1.0, 0.5])
+def test_saved_tensors_that_come_back_in_another_layout(g):
+    """Hooks that keep a copy of the saved logits (off-loading to the host does) return them dense, whatever they were."""
+    from branchgan import ops
+    d = inputs(12, 1031, torch.bfloat16, 85, "logits")
+    full, ref = [torch.zeros(3, 9, 1031, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    full[:, 2:6], ref[:, 2:6] = d["logits"].view(3, 4, 1031).cuda(), d["ref_logits"].view(3, 4, 1031).cuda()
+    rest = [d[k].view(3, 4).cuda() for k in ("ids", "old_logp", "advantages")]
+    grads = []
+    for hooked in (False, True):
+        x = full.clone().requires_grad_(True)
+        hooks = torch.autograd.graph.saved_tensors_hooks(lambda t: t.contiguous().clone(), lambda t: t) if hooked else contextlib.nullcontext()
+        with hooks:
+            loss = ops.policy_loss(x[:, 2:6], *rest, ref_logits=ref[:, 2:6], kl_coef=0.1)[0]
+        torch.autograd.grad(loss, x, retain_graph=True)                             # the second backward reads the logits again
+        (loss * g).backward()
+        grads.append(x.grad)
+    assert torch.equal(*grads)
 
 
 def test_backward_twice_and_without_grad():

@@ -134,3 +134,21 @@ def test_policy_oracle_gradient_against_differences():
     ref = torch.randn(rows, V, dtype=torch.float64, generator=g)
     for kw in (dict(), dict(ref_logits=ref), dict(ref_logp=old - 0.2)):
         assert torch.autograd.gradcheck(lambda t: OP.policy_loss(t, ids, old, adv, kl_coef=0.3, temperature=0.8, **kw)[0], (x,))
+
+
+def test_policy_row_groups_refuse_before_any_launch():
+    from branchgan import _capi
+    lib = _capi.lib()
+    p = ctypes.c_void_p(1 << 20)
+    def fwd(ref=None, **kw):
+        sh = _capi.PolicyShape(1, 0, 12, 100, 100, 100 if ref else 0, 1.0, 0.2, 0.2, 0.1, 4, 500, 500 if ref else 0, 400)
+        for k, v in kw.items():
+            setattr(sh, k, v)
+        # a missing output is what a shape that is accepted stumbles over
+        rc = lib.bg_policy_loss_fwd(ctypes.byref(sh), p, ref, p, p, None, p, None, None, None, p, p, p, None, None, None)
+        assert rc == 1
+        return lib.bg_last_error()
+    for kw in (dict(inner=5), dict(inner=-1), dict(x_outer=-1), dict(ref=p, ref_outer=-1), dict(d_outer=399)):
+        assert b"group" in fwd(**kw), (kw, lib.bg_last_error())
+    for kw in (dict(), dict(inner=0, d_outer=0, x_outer=-1), dict(inner=12, d_outer=0, x_outer=-1), dict(x_outer=0), dict(ref=p)):
+        assert b"null argument" in fwd(**kw), (kw, lib.bg_last_error())
