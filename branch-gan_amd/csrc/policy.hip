@@ -108,9 +108,15 @@ struct RowResult {          // what the gradient of a row needs
 
 __device__ __forceinline__ float inverse(double n) { return n == 0.0 ? 0.f : (float)(1.0 / n); }
 
+// a row's weight, 0 if its id is outside the vocabulary.  The weight is requested beside the id, not after it.
+__device__ __forceinline__ float row_weight(const PolicyArgs& a, int64_t row, int64_t& id) {
+  id = a.ids[row];
+  const float w = *(a.weights ? a.weights + row : (const float*)(a.ids + row));
+  return id >= 0 && id < a.V ? (a.weights ? w : 1.f) : 0.f;
+}
 __device__ __forceinline__ float row_weight(const PolicyArgs& a, int64_t row) {
-  const int64_t id = a.ids[row];
-  return id >= 0 && id < a.V ? (a.weights ? a.weights[row] : 1.f) : 0.f;
+  int64_t id;
+  return row_weight(a, row, id);
 }
 
 // log of a sum to ~1e-11, in few registers (the row sits in them meanwhile): s = 2^e f with f in [0.7, 1.42), log f = 2 atanh(z),
@@ -127,12 +133,27 @@ __device__ __forceinline__ double log_sum(double s) {
   return fma((double)e, 0.6931471805599453, 2.0 * fma(z * z2, q, z));
 }
 
-// One thread: the row's statistics to its log-prob, KL, loss term and gradient factors.
+struct RowInput {           // a row's numbers, requested ahead of the row itself: finish_row is one thread's work that the rest waits for
+  float w, old_logp, adv, ref_logp;
+  int64_t id;
+};
+
+__device__ __forceinline__ RowInput row_input(const PolicyArgs& a, int64_t row) {
+  RowInput in;
+  in.old_logp = a.old_logp[row];
+  in.adv = a.adv[row];
+  in.ref_logp = *(a.ref_logp ? a.ref_logp + row : a.old_logp + row);
+  in.w = row_weight(a, row, in.id);
+  return in;
+}
+
+// One thread: the row's statistics to its log-prob, KL, loss term and gradient factors.  ls, lsy: logs of the sums s and of the reference's.
 template <bool REF>
-__device__ RowResult finish_row(const PolicyArgs& a, int64_t row, float w, float m, double s, float my, double sy, double t, float x_id) {
-  const double ls = log_sum(s);
+__device__ RowResult finish_row(const PolicyArgs& a, int64_t row, const RowInput& in, float m, double s, double ls, float my, double lsy, double t,
+                                float x_id) {
+  const float w = in.w;
   const double logp = ((double)x_id - m) * a.inv_t - ls;
-  const float ratio = expf((float)(logp - a.old_logp[row])), A = a.adv[row];
+  const float ratio = expf((float)(logp - in.old_logp)), A = in.adv;
   const float lo = (float)(1.0 - a.clip_low), hi = (float)(1.0 + a.clip_high);
   const float plain = -A * ratio, clipped = -A * fminf(fmaxf(ratio, lo), hi);
   const float pg = plain != plain ? plain : fmaxf(plain, clipped);
@@ -143,10 +164,10 @@ __device__ RowResult finish_row(const PolicyArgs& a, int64_t row, float w, float
   double gap = 0.0;
   float kl = 0.f;
   if constexpr (REF) {
-    gap = ls - log_sum(sy);
+    gap = ls - lsy;
     kl = (float)(t / s * a.inv_t - gap);
   } else if (a.ref_logp) {
-    const float d = (float)((double)a.ref_logp[row] - logp);
+    const float d = (float)((double)in.ref_logp - logp);
     float e1;                                                        // exp(d) - 1
     if (__builtin_fabsf(d) < 0.5f) {                                 // exp(d) - 1 - d by its series: d^11 / 11! < 2^-24 of it
       float q = 1.f / 10.f;
@@ -192,6 +213,7 @@ __device__ __forceinline__ float grad_of(float p, float diff, float slope, float
 __global__ __launch_bounds__(1024) void policy_norm_kernel(PolicyArgs a) {
   __shared__ double red[16];
   double n = 0.0;
+#pragma unroll 4
   for (int64_t r = threadIdx.x; r < a.rows; r += 1024) n += row_weight(a, r);
   n = wave_sum(n);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = n;
@@ -205,6 +227,7 @@ __global__ __launch_bounds__(1024) void policy_norm_kernel(PolicyArgs a) {
 __global__ __launch_bounds__(1024) void policy_total_kernel(PolicyArgs a, const float* denominator, float* out_loss) {
   __shared__ double red[2][16];
   double sum = 0.0, n = 0.0;
+#pragma unroll 4
   for (int64_t r = threadIdx.x; r < a.rows; r += 1024) {
     sum += *(const double*)(a.stats + r * BG_POLICY_STATS + 6);
     if (!denominator) n += row_weight(a, r);
@@ -234,14 +257,15 @@ __global__ __launch_bounds__(NT, 4) void policy_row_kernel(PolicyArgs a, const f
   __shared__ double red[NW][4];
   __shared__ RowResult sh_row;
   __shared__ float sh_inv_n;
-  const int64_t row = blockIdx.x;
+  const uint32_t group = blockIdx.y, at = blockIdx.x;                  // (a division to get them costs a row 2 us: 8184 rows of 50304 with a reference 626 -> 662 us)
+  const int64_t row = (int64_t)group * a.inner + at;
   const int tid = threadIdx.x;
-  const T* x = (const T*)a.logits + row_at(a, row, a.x_stride, a.x_outer);
-  const T* y = REF ? (const T*)a.ref + row_at(a, row, a.ref_stride, a.ref_outer) : nullptr;
-  T* dx = dlogits ? dlogits + row_at(a, row, a.V, a.d_outer) : nullptr;
+  const T* x = (const T*)a.logits + (at * a.x_stride + group * a.x_outer);
+  const T* y = REF ? (const T*)a.ref + (at * a.ref_stride + group * a.ref_outer) : nullptr;
+  T* dx = dlogits ? dlogits + (at * a.V + group * a.d_outer) : nullptr;
   const int V = (int)a.V, mis = misalignment<T>(x);
-  const float w = row_weight(a, row);
-  if (w == 0.f) {
+  RowInput in = row_input(a, row);
+  if (in.w == 0.f) {
     skip_row(a, row);
     const float zero[N] = {};
     if (dlogits)
@@ -260,10 +284,14 @@ __global__ __launch_bounds__(NT, 4) void policy_row_kernel(PolicyArgs a, const f
     if constexpr (REF) vy[k] = *(const V_t*)(y + (i * N - mis));
   }
   const float ex = has_extra ? to_f32(x[extra]) : -INFINITY, ey = REF && has_extra ? to_f32(y[extra]) : -INFINITY;
-  const int id = (int)a.ids[row];
+  const int id = (int)in.id;
   const float x_id = to_f32(x[id]);
+  constexpr bool SUM_N = NT == 256;                                    // see NORM_ROWS
+  float n32 = denominator || (SUM_N && a.rows <= NORM_ROWS) ? 0.f : a.stats[a.rows * BG_POLICY_STATS];
+  if (denominator) n32 = denominator[0];
+  asm volatile("" ::"s"(in.old_logp), "s"(in.adv), "s"(in.ref_logp), "s"(n32));          // requested here, not where one thread needs them
   double n64 = 0.0;
-  if (NT == 256 && a.rows <= NORM_ROWS && !denominator)
+  if (SUM_N && a.rows <= NORM_ROWS && !denominator)
     for (int64_t r = tid; r < a.rows; r += NT) n64 += row_weight(a, r);
   V_t none;
 #pragma unroll
@@ -305,15 +333,18 @@ __global__ __launch_bounds__(NT, 4) void policy_row_kernel(PolicyArgs a, const f
     for (int j = 0; j < N; ++j) add((float)vx[k][j], REF ? (float)vy[REF ? k : 0][j] : 0.f);
   }
   const double s64 = wave_sum((double)s), t64 = REF ? wave_sum((double)t) : 0.0, sy64 = REF ? wave_sum((double)sy) : 0.0;
-  if constexpr (NT == 256) n64 = wave_sum(n64);
+  if constexpr (SUM_N) n64 = wave_sum(n64);
   if ((tid & 63) == 0) { red[tid >> 6][0] = s64; red[tid >> 6][1] = t64; red[tid >> 6][2] = sy64; red[tid >> 6][3] = n64; }
   __syncthreads();
-  if (tid == 0) {
+  if (tid < 64) {
     double S = 0.0, Tt = 0.0, Sy = 0.0, Nw = 0.0;
     for (int i = 0; i < NW; ++i) { S += red[i][0]; Tt += red[i][1]; Sy += red[i][2]; Nw += red[i][3]; }
-    sh_inv_n = denominator ? inverse(denominator[0])
-               : NT == 256 && a.rows <= NORM_ROWS ? inverse(Nw) : a.stats[a.rows * BG_POLICY_STATS];
-    sh_row = finish_row<REF>(a, row, w, ms, S, mys, Sy, Tt, x_id);
+    const double lg = log_sum(REF && tid == 1 ? Sy : S);
+    const double ls = __shfl(lg, 0), lsy = REF ? __shfl(lg, 1) : 0.0;
+    if (tid == 0) {
+      sh_inv_n = denominator ? inverse(n32) : SUM_N && a.rows <= NORM_ROWS ? inverse(Nw) : n32;
+      sh_row = finish_row<REF>(a, row, in, ms, S, ls, mys, lsy, Tt, x_id);
+    }
   }
   if (!dlogits) return;
   __syncthreads();
@@ -354,8 +385,8 @@ __global__ __launch_bounds__(PT) void policy_rows_kernel(PolicyArgs a) {
   __shared__ double red[NW][3];
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x;
-  const float w = row_weight(a, row);
-  if (w == 0.f) {
+  const RowInput in = row_input(a, row);
+  if (in.w == 0.f) {
     skip_row(a, row);
     return;
   }
@@ -363,7 +394,6 @@ __global__ __launch_bounds__(PT) void policy_rows_kernel(PolicyArgs a) {
   const T* y = REF ? (const T*)a.ref + row_at(a, row, a.ref_stride, a.ref_outer) : nullptr;
   const int mis = misalignment<T>(x);
   const bool y_on = !REF || misalignment<T>(y) == mis;
-  const int64_t id = a.ids[row];
   float m = -INFINITY, my = -INFINITY;
   for (int64_t e0 = (int64_t)tid * N - mis; e0 < a.V; e0 += PT * N) {
     const typename Vec<T>::type vx = row_vector<T>(x, e0, a.V, true);
@@ -402,7 +432,7 @@ __global__ __launch_bounds__(PT) void policy_rows_kernel(PolicyArgs a) {
   if (tid == 0) {
     double S = 0.0, Tt = 0.0, Sy = 0.0;
     for (int i = 0; i < NW; ++i) { S += red[i][0]; Tt += red[i][1]; Sy += red[i][2]; }
-    finish_row<REF>(a, row, w, ms, S, mys, Sy, Tt, to_f32(x[id]));
+    finish_row<REF>(a, row, in, ms, S, log_sum(S), mys, REF ? log_sum(Sy) : 0.0, Tt, to_f32(x[in.id]));
   }
 }
 
@@ -490,7 +520,9 @@ template <typename T, bool REF> static bool policy_row_launch(const PolicyArgs& 
   };
   if (REF && !same_grid(a.ref, a.ref_stride, a.ref_outer)) return false;
   if (dlogits && !same_grid(dlogits, a.V, a.d_outer)) return false;
-  const dim3 grid((unsigned)a.rows);
+  const int64_t groups = a.rows / a.inner;
+  if (groups > 65535) return false;
+  const dim3 grid(a.inner, (unsigned)groups);
   if (nvec <= 256 * 2) hipLaunchKernelGGL((policy_row_kernel<T, REF, 256, 2>), grid, dim3(256), 0, st, a, denominator, dlogits);
   else if (nvec <= 256 * 8) hipLaunchKernelGGL((policy_row_kernel<T, REF, 256, 8>), grid, dim3(256), 0, st, a, denominator, dlogits);
   else if (nvec <= 512 * 13) hipLaunchKernelGGL((policy_row_kernel<T, REF, 512, 13>), grid, dim3(512), 0, st, a, denominator, dlogits);
