@@ -935,8 +935,11 @@ def kv_cache_attention(q, layer, start=None, counts=None, scale=None, max_keys=N
 def _logit_rows(t, V):
     """(..., V) -> t or a copy of it whose rows the kernels can walk, rows per group, row stride, group stride.  (B, T, V) with a
     dense last dimension - also a slice along T, or (T, B, V) transposed - needs no copy."""
-    if t.dim() == 3:
-        if t.stride(2) != 1 or (t.stride(1) < V and t.shape[1] > 1):
+    st = t.stride()
+    if len(st) == 2 and st[1] == 1 and st[0] >= V:
+        return t, t.shape[0], st[0], 0
+    if len(st) == 3:
+        if st[2] != 1 or (st[1] < V and t.shape[1] > 1):
             t = t.contiguous()
         return t, t.shape[1], max(t.stride(1), V), t.stride(0)
     if t.dim() != 2 or t.stride(1) != 1:
@@ -949,10 +952,9 @@ def _logit_rows(t, V):
 def _gradient_rows(x, shape, inner, stride, outer, V):
     """Uninitialised gradient of that shape and its group stride: rows V apart, on the 16-byte grid as x's are where they can be (the
     kernel that holds a row in registers reads and writes it by the same whole vectors)."""
-    n = 16 // x.element_size()
-    off, pad = x.data_ptr() % 16 // x.element_size(), 0
-    if len(shape) == 3 and shape[0] > 1:
-        pad = (outer - inner * V) % n
+    e = x.element_size()
+    n, off = 16 // e, (x.data_ptr() & 15) // e
+    pad = 0 if outer == 0 or outer == inner * V else (outer - inner * V) % n        # (not a matter of addresses: backward's must be the same)
     if (off == 0 and pad == 0) or (stride - V) % n:
         return x.new_empty(shape), inner * V
     if pad == 0:
