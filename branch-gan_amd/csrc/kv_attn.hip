@@ -869,7 +869,7 @@ extern "C" int bg_kv_cache_attn_fwd(const bg_kv_cache* cache, const void* data, 
   BG_REQUIRE((int64_t)T * Hq < (1ll << 30), "bg_kv_cache_attn_fwd: T=%d Hq=%d", T, Hq);
   const KvPlan p = kv_attn_plan(cache, Hq, T, max_keys);
   const int64_t rows = (int64_t)cache->B * Hq * T;
-  BG_REQUIRE(cache->B <= 65535 && cache->H <= 65535 && (int64_t)p.row_tiles * p.splits < (1ll << 31) && rows < (1ll << 31),
+  BG_REQUIRE(cache->B <= 65535 && cache->H <= 65535 && (int64_t)p.row_tiles * p.splits < (1ll << 24) && rows < (1ll << 31),
              "bg_kv_cache_attn_fwd: B=%d H=%d, %lld rows", cache->B, cache->H, (long long)rows);
   const size_t need = bg_kv_cache_attn_workspace_bytes(cache, Hq, T, max_keys);
   if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 3))) {

@@ -385,7 +385,7 @@ extern "C" int bg_kv_cache_append(const bg_kv_cache* cache, void* data, const vo
   const int64_t heads = (int64_t)cache->B * cache->H;
   if (T == 1) {
     const int64_t blocks = cdiv(2 * heads * cache->Dh, 256);
-    BG_REQUIRE(blocks < (1ll << 31), "bg_kv_cache_append: %lld blocks", (long long)blocks);
+    BG_REQUIRE(blocks < (1ll << 24), "bg_kv_cache_append: %lld blocks", (long long)blocks);        // a launch has fewer than 2^32 threads
 #define BG_GO(BITS, DH)                                                                                                              \
   if (dtype == BG_F32)                                                                                                               \
     hipLaunchKernelGGL((kv_append_token_kernel<float, BITS, DH>), dim3((unsigned)blocks), dim3(256), 0, st, a, (const float*)k,      \
@@ -400,7 +400,7 @@ extern "C" int bg_kv_cache_append(const bg_kv_cache* cache, void* data, const vo
   }
   const int64_t tiles = cdiv((int64_t)T + KV_TILE - 1, KV_TILE);            // T tokens at any offset touch at most this many
   const int64_t per_head = cdiv(tiles, 256 / cache->Dh), blocks = 2 * per_head * heads;     // keys, values
-  BG_REQUIRE(blocks < (1ll << 31), "bg_kv_cache_append: %lld blocks", (long long)blocks);
+  BG_REQUIRE(blocks < (1ll << 25), "bg_kv_cache_append: %lld blocks", (long long)blocks);
 #define BG_GO2(TT, BITS, DH, VEC)                                                                                                   \
   hipLaunchKernelGGL((kv_append_tiles_kernel<TT, BITS, DH, VEC>), dim3((unsigned)blocks), dim3(128), 0, st, a, (const TT*)k,        \
                      (const TT*)v, k_sb, k_sh, k_st, v_sb, v_sh, v_st, (int)per_head)
@@ -424,7 +424,7 @@ extern "C" int bg_kv_cache_read(const bg_kv_cache* cache, const void* data, void
   const bool vec = aligned16(k, o_sb, o_sh, o_st, e) && aligned16(v, 0, 0, 0, e);
   const int64_t tiles = cdiv((int64_t)T + KV_TILE - 1, KV_TILE);
   const int64_t per_head = cdiv(tiles, 256 / cache->Dh), blocks = 2 * per_head * cache->B * cache->H;
-  BG_REQUIRE(blocks < (1ll << 31), "bg_kv_cache_read: %lld blocks", (long long)blocks);
+  BG_REQUIRE(blocks < (1ll << 25), "bg_kv_cache_read: %lld blocks", (long long)blocks);
 #define BG_GO2(TT, BITS, DH, VEC)                                                                                                 \
   hipLaunchKernelGGL((kv_read_kernel<TT, BITS, DH, VEC>), dim3((unsigned)blocks), dim3(128), 0, st, a, (TT*)k, (TT*)v, o_sb,      \
                      o_sh, o_st, (int)per_head)

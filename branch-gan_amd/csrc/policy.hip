@@ -17,6 +17,7 @@
 namespace bg {
 
 constexpr int PT = 256;      // threads per row of the streaming kernels
+constexpr int64_t MAX_ROWS = 1 << 22;      // a launch has fewer than 2^32 threads, a row up to 1024
 
 template <typename T> struct Vec;
 template <> struct Vec<float> {
@@ -479,7 +480,7 @@ using namespace bg;
 static int policy_check(const char* who, const bg_policy_shape* sh, const void* logits, const void* ref, const int64_t* ids, const float* stats) {
   BG_REQUIRE(sh && logits && ids && stats && ((uintptr_t)stats & 7) == 0, "%s: null argument or stats off the 8-byte grid", who);
   BG_REQUIRE(sh->dtype == BG_F32 || sh->dtype == BG_BF16, "%s: dtype %d", who, sh->dtype);
-  BG_REQUIRE(sh->rows > 0 && sh->rows < (1ll << 31) && sh->V > 0 && sh->V < (1ll << 31) && sh->x_stride >= sh->V, "%s: rows=%lld V=%lld stride=%lld",
+  BG_REQUIRE(sh->rows > 0 && sh->rows < MAX_ROWS && sh->V > 0 && sh->V < (1ll << 31) && sh->x_stride >= sh->V, "%s: rows=%lld V=%lld stride=%lld",
              who, (long long)sh->rows, (long long)sh->V, (long long)sh->x_stride);
   BG_REQUIRE(!ref || sh->ref_stride >= sh->V, "%s: reference stride %lld", who, (long long)sh->ref_stride);
   BG_REQUIRE(sh->inner >= 0 && (sh->inner == 0 || sh->rows % sh->inner == 0), "%s: groups of %lld of %lld rows", who, (long long)sh->inner,

@@ -534,7 +534,7 @@ int bg_kv_cache_attn_fwd(const bg_kv_cache* cache, const void* data, const void*
  *        = exp(d) - d - 1, d = ref_logp[r] - logp                             when ref_logp is given, 0 with neither,
  *   loss = sum_r w_r (pg + kl_coef kl) / N,  N = *denominator, or sum_r w_r over the rows that count when it is NULL
  *          (N = 0: loss and gradient are 0).
- * Rows lie in groups of `inner` (0: one group): row r of logits at (r / inner) x_outer + (r % inner) x_stride elements, ref_logits alike;
+ * rows: fewer than 2^22.  Rows lie in groups of `inner` (0: one group): row r of logits at (r / inner) x_outer + (r % inner) x_stride elements, ref_logits alike;
  * dlogits at (r / inner) d_outer + (r % inner) V, d_outer >= inner V.  The outer strides of a single group are not looked at.
  * weights (fp32, NULL = 1): a row with weight 0 or an id outside [0, V) does not count - its logits are not read, its logp and
  * kl are 0, its gradient is 0.  A logit of -inf (or the type's lowest value) has probability 0 and adds nothing to the KL.

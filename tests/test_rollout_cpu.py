@@ -152,3 +152,19 @@ def test_policy_row_groups_refuse_before_any_launch():
         assert b"group" in fwd(**kw), (kw, lib.bg_last_error())
     for kw in (dict(), dict(inner=0, d_outer=0, x_outer=-1), dict(inner=12, d_outer=0, x_outer=-1), dict(x_outer=0), dict(ref=p)):
         assert b"null argument" in fwd(**kw), (kw, lib.bg_last_error())
+
+
+def test_calls_of_more_threads_than_a_launch_has_are_refused():
+    from branchgan import _capi
+    lib = _capi.lib()
+    p = ctypes.c_void_p(1 << 20)
+    sh = _capi.PolicyShape(1, 0, 1 << 22, 16, 16, 0, 1.0, 0.2, 0.2, 0.1, 0, 0, 0, 0)
+    assert lib.bg_policy_loss_fwd(ctypes.byref(sh), p, None, p, p, None, p, None, None, p, p, p, p, None, None, None) == 1 and b"rows" in lib.bg_last_error()
+    tile = lib.bg_kv_cache_tile_bytes(4, 32)
+    wide = cache_struct(B=60000, H=60000, Dh=32, capacity=1, c_sh=tile, c_sb=60000 * tile)
+    for T in (1, 2):
+        assert lib.bg_kv_cache_append(ctypes.byref(wide), p, p, p, 1, T, 0, 0, 32, 0, 0, 32, None, None, None) == 1 and b"blocks" in lib.bg_last_error()
+        assert lib.bg_kv_cache_read(ctypes.byref(wide), p, p, p, 1, T, 0, 0, 32, None, None, None) == 1 and b"blocks" in lib.bg_last_error()
+    c = cache_struct(H=1, capacity=1)
+    assert lib.bg_kv_cache_attn_fwd(ctypes.byref(c), p, p, 1, 1, (1 << 28) + 1, 0, 0, 64, None, None, 1, 1.0, p, 0, 0, 64, None, None, 0, None) == 1
+    assert b"rows" in lib.bg_last_error()
