@@ -3,7 +3,9 @@
 // Mathematics.  With codes c and scales s per 32 channels g,
 //   q . k = sum_g s_kg (q_g . c_kg)         o_ch = sum_k (p_k s_vg) c_v,ch
 // so the codes themselves are the matrix operands: as bf16 they are exact (see unpack_codes), the scales join in fp32 - on the scores after the product, on the probabilities before it.  Nothing held is rounded again.  bf16
-// queries are exact operands; fp32 queries go in as three bf16 pieces (24 bits), probabilities as two (16 bits, for bf16 outputs) or three.
+// queries are exact operands; fp32 queries go in as three bf16 pieces (24 bits), probabilities as two (16 bits) for bf16 outputs - at most
+// 2^-17 of a probability, 1 / 256 of half a step of the output, where three would cost 7 % (8 sequences of 65537 keys 117 -> 125
+// us) - or as three.
 //
 // Layouts.  One wave takes 4 tiles (128 keys) per turn with v_mfma_f32_16x16x32_bf16 (rows of A x columns of B, 32 deep; lane = (n =
 // lane % 16, j = lane / 16) holds 8 elements of A's row n and of B's column n, and results (rows 4 j + r, column n)).
@@ -15,7 +17,8 @@
 //     n = key 8 n + t of the turn: lane (n, j) gets RR = 1, 2 or 4 pairs' scores for 8 keys, a quarter of the vector work of the layout
 //     above where RR is 1 (one query head per cache head up to heads of 128).  Sums over a row's pairs by lane swaps.  The
 //     probabilities go through LDS once (16 bytes per pair and octet of keys) to become A operands.
-//   In both the codes go from memory to operands with one shift and one mask-or per pair.
+//   In both 4-bit codes go from memory to operands of bf16 queries with one shift and one mask-or per pair; signed codes (4 bits with
+//   fp32 queries, 8 bits) take a conversion each.
 // Softmax.  The running maximum of a row moves only when a score passes it by 2^8 (probabilities stay below 256), so that
 //   the usual turn needs no exchange between lanes for it.
 // Work.  Four waves per workgroup take turns round robin; the key range is split over workgroups when there are too few of
@@ -99,6 +102,10 @@ union Frag {
 // 8 codes -> 8 bf16 numbers (code + offset) / unit.
 // 4 bits, bf16 queries: the nibble as bits 3..6 of a bf16 in [16, 32) is 16 + stored code = code + 24 - a shift and a mask-or per pair.
 // (The two constants sit in a vector and a scalar register: as literals they would make the mask-or two instructions.)
+// What the offset adds to an output is taken off turn by turn (step by step where there are many rows): sums that kept it grow with
+// the number of keys while the output, an average, shrinks - over 65536 random keys 18 % of the bf16 outputs then were not the rounded
+// ones, now 0.8 %.  16 subtractions a turn at heads of 64 (64 sequences 22.9 us either way, 67 tokens 21.5 -> 21.8); signed codes
+// for bf16 queries would cost 26.3 and 23.5.
 // 4 bits, fp32 queries: sums of c + 24 would cost 2 to 3 bits that fp32 results show (error 4e-6 against 4e-7), so the codes come
 // signed, by the instruction that reads a signed nibble as sixteenths - twice the instructions.
 // 8 bits: signed bytes, converted (a conversion that takes its byte from the word, and half a pack).
@@ -330,7 +337,7 @@ __global__ __launch_bounds__(64 * KW, (DecodeShape<T, BITS, DH, RR>::WAVES)) voi
   if (a.splits > 1 && t_begin + wave < t_end) load_k(t_begin + wave, 0);
 
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  f32x4 acc[CB], off = zero;
+  f32x4 acc[CB], off = zero;                                                 // off: what the codes' offset added in this turn
 #pragma unroll
   for (int c = 0; c < CB; ++c) acc[c] = zero;
   float mc[RL], l[RL];                                                       // maximum in log2 units, this lane's share of the sum
@@ -428,8 +435,6 @@ __global__ __launch_bounds__(64 * KW, (DecodeShape<T, BITS, DH, RR>::WAVES)) voi
       for (int c = 0; c < CB; ++c)
 #pragma unroll
         for (int r = 0; r < 4; ++r) acc[c][r] *= f[r];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) off[r] *= f[r];
     }
     float p[8][RL];
 #pragma unroll
@@ -469,8 +474,10 @@ __global__ __launch_bounds__(64 * KW, (DecodeShape<T, BITS, DH, RR>::WAVES)) voi
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   };
-  // one piece of the output: row n of A is pair n (rows past the pairs repeat them and are not used), octets 4 tile + j
+  // one piece of the output: row n of A is pair n (rows past the pairs repeat them and are not used), octets 4 tile + j.  The offset
+  // leaves with its turn: see unpack_codes.
   const auto output = [&](int vp) __attribute__((always_inline)) {
+    if (OFFT != 0.f && vp == 0) off = zero;
 #pragma unroll
     for (int i = 0; i < VT; ++i) {
       bf16x8 pf[NP];
@@ -486,6 +493,12 @@ __global__ __launch_bounds__(64 * KW, (DecodeShape<T, BITS, DH, RR>::WAVES)) voi
 #pragma unroll
         for (int q = 0; q < NP; ++q) acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf[q], vf, acc[c], 0, 0, 0);
       }
+    }
+    if (OFFT != 0.f && vp == KP - 1) {
+#pragma unroll
+      for (int c = 0; c < CB; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[c][r] -= off[r];
     }
   };
 
@@ -542,7 +555,7 @@ __global__ __launch_bounds__(64 * KW, (DecodeShape<T, BITS, DH, RR>::WAVES)) voi
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int p = 4 * j + r;
-      if (p < D::PAIRS && p % NG == c / 2) sh.o[wave][p / NG][16 * c + n] = (acc[c][r] - off[r]) * kv_unit<T, BITS>();
+      if (p < D::PAIRS && p % NG == c / 2) sh.o[wave][p / NG][16 * c + n] = acc[c][r] * kv_unit<T, BITS>();
     }
   __syncthreads();
   write_rows<T, DH, D::ROWS>(a, sh, b, h, 0, split);
@@ -635,12 +648,10 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<BITS, DH>())) void kv_attn_kerne
   const int n_max = tile_keys(a, b, row0, n_min);
   const int vis = real ? min(a.kv.visible(b, t_row), a.max_keys) : 0x7FFFFFFF;
 
-  f32x4 acc[CB], offg[NG];
+  f32x4 acc[CB];
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int c = 0; c < CB; ++c) acc[c] = zero;
-#pragma unroll
-  for (int g = 0; g < NG; ++g) offg[g] = zero;
   float mc = -INFINITY, l = 0.f;                                             // maximum in log2 units, this lane's share of the sum
   Frag ones;
 #pragma unroll
@@ -708,10 +719,6 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<BITS, DH>())) void kv_attn_kerne
       for (int c = 0; c < CB; ++c)
 #pragma unroll
         for (int r = 0; r < 4; ++r) acc[c][r] *= f[r];
-#pragma unroll
-      for (int g = 0; g < NG; ++g)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) offg[g][r] *= f[r];
     }
     const float ms = mc == -INFINITY ? 0.f : mc;
     float p[TS][4];
@@ -735,6 +742,9 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<BITS, DH>())) void kv_attn_kerne
 #pragma unroll
     for (int t = 0; t < TS; ++t) l += (p[t][0] + p[t][1]) + (p[t][2] + p[t][3]);
     // output
+    f32x4 offg[NG];                                                          // what the codes' offset adds in this step
+#pragma unroll
+    for (int g = 0; g < NG; ++g) offg[g] = zero;
 #pragma unroll
     for (int o = 0; o < NO; ++o) {
       bf16x8 pf[NG][NP];
@@ -756,6 +766,12 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<BITS, DH>())) void kv_attn_kerne
         for (int i = 0; i < NP; ++i) acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf[c / 2][i], vf, acc[c], 0, 0, 0);
       }
     }
+    if constexpr (OFFT != 0.f) {
+#pragma unroll
+      for (int c = 0; c < CB; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[c][r] -= offg[c / 2][r];
+    }
   }
 
   // this wave's state -> LDS (accumulator row 4 j + r, channel 16 c + n)
@@ -764,7 +780,7 @@ __global__ __launch_bounds__(64 * KW, (kv_waves<BITS, DH>())) void kv_attn_kerne
 #pragma unroll
   for (int c = 0; c < CB; ++c)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) sh.o[wave][4 * j + r][16 * c + n] = (acc[c][r] - offg[c / 2][r]) * kv_unit<T, BITS>();
+    for (int r = 0; r < 4; ++r) sh.o[wave][4 * j + r][16 * c + n] = acc[c][r] * kv_unit<T, BITS>();
   __syncthreads();
   write_rows<T, DH, ROWS>(a, sh, b, h, row0, split);
 }

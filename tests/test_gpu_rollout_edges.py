@@ -1,0 +1,41 @@
+"""The quantised cache, the attention over it and the clipped policy loss where sums, scales and masks reach their ends; against float64."""
+import math
+
+import pytest
+import torch
+
+from oracle import kvcache as OK
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("Dh,B,H,G,T", [(32, 32, 16, 1, 1), (64, 32, 16, 1, 1), (128, 16, 16, 2, 1), (32, 16, 16, 16, 2), (128, 16, 16, 4, 8), (32, 1, 2, 1, 3)])
+def test_sums_over_many_keys_do_not_lose_digits(Dh, B, H, G, T):
+    """4 bits, bf16 queries, 65536 keys, key ranges with and without splits.  Keys of zero give every key the probability 1, scales of
+    values are 8-bit numbers in [1, 2), and the values of a turn of 128 keys add up to at most 2 (its halves cancel).  Whatever the
+    sums are kept in, a multiple of 2^-7 below 2^17 is exact in fp32: the values of one turn with codes offset by up to 24 reach 128 * 31 *
+    2 < 2^13, all turns together without an offset 512 * 2 = 2^10 - so the output is the exact sum over the exact count, divided (2^-22) and
+    rounded to bf16 (half a step).  Sums that carry an offset from turn to turn reach 65536 / 4 * 31 * 1.5 > 2^19 and do not pass."""
+    from branchgan import kvcache, ops
+    gen = torch.Generator().manual_seed(Dh + G)
+    n = 65536
+    s = (1 + torch.randint(0, 128, (n // 128, 1, 64, Dh // 32), generator=gen) / 128).double().expand(-1, 2, -1, -1).reshape(n, Dh // 32)
+    c = torch.randint(-6, 7, (n // 128, 64, Dh), generator=gen).double()
+    c[..., ::32] = 7.0                                                       # the largest magnitude of its 32 channels: fixes the scale
+    c = torch.stack((c, -c), 1)
+    c[:, 1, 0, 1:31] += 1                                                    # a turn leaves one s behind, in most channels
+    c = c.view(n, Dh)
+    v = c * s.repeat_interleave(32, 1)
+    assert torch.equal(v, v.float().double()) and torch.equal(v, OK.held_values(v.float(), 4))
+    turns = v.view(-1, 128, Dh)
+    assert turns.sum(1).abs().max() < 2 and turns.cumsum(1).abs().max() < 2.0 ** 13
+    layer = kvcache.QuantizedKVCache(1, B, H, n, Dh).layer(0)
+    ops.kv_cache_append(layer, torch.zeros(1, 1, n, Dh, device="cuda").expand(B, H, n, Dh), v.float().cuda().view(1, 1, n, Dh).expand(B, H, n, Dh))
+    q = torch.randn(B, H * G, T, Dh, generator=gen).bfloat16().cuda()
+    start = torch.full((B,), n - T, dtype=torch.int32, device="cuda")
+    out, lse = ops.kv_cache_attention(q, layer, start=start)
+    seen = torch.arange(n - T, n) + 1
+    want = (v.cumsum(0)[seen - 1] / seen[:, None]).cuda()
+    err = (out.double() - want).abs()
+    assert bool((err <= (2.0 ** -8 + 2.0 ** -22) * want.abs()).all()), float((err - 2.0 ** -8 * want.abs()).max() / want.abs().max())
+    assert float((lse.double() - torch.log(seen.double()).cuda()).abs().max()) < 2.0 ** -19
