@@ -39,3 +39,27 @@ def test_sums_over_many_keys_do_not_lose_digits(Dh, B, H, G, T):
     err = (out.double() - want).abs()
     assert bool((err <= (2.0 ** -8 + 2.0 ** -22) * want.abs()).all()), float((err - 2.0 ** -8 * want.abs()).max() / want.abs().max())
     assert float((lse.double() - torch.log(seen.double()).cuda()).abs().max()) < 2.0 ** -19
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("T", [1, 2])
+def test_scales_next_to_a_tie(bits, T):
+    """fp32 maxima on, one step below and one above L t, t halfway between two bf16 numbers: the scale is the quotient's, rounded to fp32
+    and from there to bf16 - worked out here in whole numbers, and read off the held value of the maximum itself, L s."""
+    from branchgan import kvcache, ops
+    top = 7 if bits == 4 else 127
+    t = torch.arange(257, 512, 2).double() / 256                             # the 128 ties of [1, 2)
+    a = torch.cat([torch.nextafter((top * t).float(), torch.tensor(to)) for to in (0.0, math.inf)] + [(top * t).float()])
+    a = torch.cat([a * 2.0 ** e for e in (-100, 0, 3, 90)])
+    quotient = (a.double() / top).float()                                    # 53 bits hold enough of a quotient of 24 by 7 to round it again
+    u = quotient.view(torch.int32).long()
+    scale = (((u + 0x7FFF + ((u >> 16) & 1)) >> 16) << 16).int().view(torch.float32)
+    x = torch.zeros(len(a), 1, T, 64)
+    x[:, 0, :, 3], x[:, 0, :, 40] = a[:, None], -a[:, None]
+    x[:, 0, :, 50] = 0.37 * a[:, None]
+    layer = kvcache.QuantizedKVCache(1, len(a), 1, T, 64, bits=bits).layer(0)
+    ops.kv_cache_append(layer, x.cuda(), x.flip(-1).contiguous().cuda())
+    k, v = [r.cpu() for r in ops.kv_cache_read(layer, T, dtype=torch.float32)]
+    for t in range(T):
+        assert torch.equal(k[:, 0, t, 3], top * scale) and torch.equal(k[:, 0, t, 40], -top * scale)
+    assert torch.equal(k.double(), OK.held_values(x, bits)) and torch.equal(v.double(), OK.held_values(x.flip(-1), bits))
