@@ -999,6 +999,7 @@ class _PolicyLoss(torch.autograd.Function):
         x, ids, stats, y = ctx.saved_tensors
         V, sh = ctx.rows[-1], ctx.sh
         if x.stride() != ctx.strides[0] or (y is not None and y.stride() != ctx.strides[1]):      # saved-tensor hooks may return another layout
+            sh = C.PolicyShape.from_buffer_copy(sh)                                               # (this time; the next backward may get the saved one)
             x, _, sh.x_stride, sh.x_outer = _logit_rows(x, V)
             if y is not None:
                 y, _, sh.ref_stride, sh.ref_outer = _logit_rows(y, V)

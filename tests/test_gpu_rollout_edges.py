@@ -63,3 +63,24 @@ def test_scales_next_to_a_tie(bits, T):
     for t in range(T):
         assert torch.equal(k[:, 0, t, 3], top * scale) and torch.equal(k[:, 0, t, 40], -top * scale)
     assert torch.equal(k.double(), OK.held_values(x, bits)) and torch.equal(v.double(), OK.held_values(x.flip(-1), bits))
+
+
+def test_saved_tensors_that_come_back_in_a_layout_of_their_own_each_time():
+    """Hooks that answer dense, as saved, dense again: the same gradient from every backward."""
+    from branchgan import ops
+    gen = torch.Generator().manual_seed(85)
+    B, T, V = 3, 4, 1031
+    full, ref = [torch.randn(B, 9, V, generator=gen).bfloat16().cuda() for _ in range(2)]
+    rows = [torch.randint(0, V, (B, T), generator=gen).cuda(), torch.randn(B, T, generator=gen).cuda() - 7, torch.randn(B, T, generator=gen).cuda()]
+    x, dense = full.requires_grad_(True), [False]
+    unpack = lambda t: t.contiguous().clone() if dense[0] and t.dim() == 3 else t
+    def loss():
+        return ops.policy_loss(x[:, 2:6], *rows, ref_logits=ref[:, 2:6], kl_coef=0.1)[0]
+    plain = loss()
+    torch.autograd.grad(plain, x, retain_graph=True)
+    want, = torch.autograd.grad(plain, x)                                    # a second backward reads the logits again, as the ones below do
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        hooked = loss()
+    torch.autograd.grad(hooked, x, retain_graph=True)
+    for dense[0] in (True, False, True):
+        assert torch.equal(torch.autograd.grad(hooked, x, retain_graph=True)[0], want)
