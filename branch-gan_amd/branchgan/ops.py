@@ -1019,7 +1019,8 @@ def policy_loss(logits, ids, old_logp, advantages, weights=None, ref_logp=None, 
     e.g. logits[:, :-1], is read where it lies).  ids (...) int64: the
     sampled tokens; old_logp (...): their log-probs when they were sampled; advantages (...); weights (...) or None: per token,
     0 = does not count; ref_logits (like logits) -> the KL over the vocabulary, or ref_logp (...) -> exp(d) - d - 1 of the
-    sampled token, d = ref_logp - logp.  All log-probs are those of softmax(logits / temperature).  denominator: what the sum over tokens
+    sampled token, d = ref_logp - logp; with neither kl is 0 and kl_coef without effect, with kl_coef 0 kl is reported only (whatever it is, also
+    infinite, loss and gradient do not contain it).  All log-probs are those of softmax(logits / temperature).  denominator: what the sum over tokens
     is divided by (a number, or a one-element tensor on the device - a token count over micro-batches or ranks); default the
     sum of the weights that count.  -> (loss fp32 scalar, logp (...), kl (...); the last two carry no gradient).
     Captured into a HIP graph, forward and backward belong into the same capture, made while no eager autograd graph of the same

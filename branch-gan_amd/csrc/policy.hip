@@ -180,7 +180,7 @@ __device__ RowResult finish_row(const PolicyArgs& a, int64_t row, const RowInput
       e1 = expf(d) - 1.f;                                           // |d| >= 1/2: no digits to lose
       kl = e1 - d;
     }
-    slope -= (float)a.kl_coef * e1;
+    if (a.kl_coef != 0.0) slope -= (float)a.kl_coef * e1;             // a KL that is reported only may be infinite
   }
   r.slope = w * slope;
   r.w_kl = (float)(w * a.kl_coef);
@@ -190,7 +190,7 @@ __device__ RowResult finish_row(const PolicyArgs& a, int64_t row, const RowInput
   a.out_kl[row] = kl;
   float* st = a.stats + row * BG_POLICY_STATS;
   st[0] = r.m; st[1] = r.inv_s; st[2] = r.slope; st[3] = r.w_kl; st[4] = r.off; st[5] = r.my;
-  *(double*)(st + 6) = (double)w * (pg + a.kl_coef * kl);
+  *(double*)(st + 6) = (double)w * (a.kl_coef != 0.0 ? pg + a.kl_coef * kl : pg);
   return r;
 }
 
@@ -204,8 +204,8 @@ template <bool REF>
 __device__ __forceinline__ float grad_of(float p, float diff, float slope, float w_kl, float off, float inv_t) {
   float d = -slope * p;
   if constexpr (REF) {
-    const float k = w_kl * p * __builtin_fmaf(diff, inv_t, -off);
-    d += p != 0.f ? k : 0.f;                                         // a masked entry: its difference may be infinite
+    const float pk = w_kl * p, k = pk * __builtin_fmaf(diff, inv_t, -off);
+    d += pk != 0.f ? k : 0.f;                                        // a masked entry, or a KL that is reported only: the difference may be infinite
   }
   return d;
 }

@@ -532,6 +532,7 @@ int bg_kv_cache_attn_fwd(const bg_kv_cache* cache, const void* data, const void*
  *   pg   = max(-A ratio, -A clamp(ratio, 1 - clip_low, 1 + clip_high)),
  *   kl   = sum_j p_j (log p_j - log q_j), q = softmax(ref_logits / T)         when ref_logits is given,
  *        = exp(d) - d - 1, d = ref_logp[r] - logp                             when ref_logp is given, 0 with neither,
+ *          (kl_coef = 0: out_kl reports it, loss and gradient do not contain it, also where it is infinite or NaN),
  *   loss = sum_r w_r (pg + kl_coef kl) / N,  N = *denominator, or sum_r w_r over the rows that count when it is NULL
  *          (N = 0: loss and gradient are 0).
  * rows: fewer than 2^22.  Rows lie in groups of `inner` (0: one group): row r of logits at (r / inner) x_outer + (r % inner) x_stride elements, ref_logits alike;

@@ -84,3 +84,41 @@ def test_saved_tensors_that_come_back_in_a_layout_of_their_own_each_time():
     torch.autograd.grad(hooked, x, retain_graph=True)
     for dense[0] in (True, False, True):
         assert torch.equal(torch.autograd.grad(hooked, x, retain_graph=True)[0], want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [40, 5003, 120001])
+@pytest.mark.parametrize("g", [1.0, 0.5])
+@pytest.mark.parametrize("ref", ["masked", "nan", "logp"])
+def test_a_kl_that_is_reported_only_stays_out_of_the_update(dtype, V, g, ref):
+    """kl_coef 0 with a reference that masks an entry the policy gives weight (an infinite KL), a broken one, or a reference log-prob far
+    above the policy's: loss and gradient are those without a reference, to rounding."""
+    from branchgan import ops
+    gen = torch.Generator().manual_seed(V)
+    rows = 5
+    x = torch.randn(rows, V, generator=gen).to(dtype)
+    ids = torch.randint(2, V, (rows,), generator=gen)
+    logp = torch.log_softmax(x.double(), -1).gather(1, ids[:, None])[:, 0]
+    old, adv = (logp + torch.tensor([0.1, -0.1, 0.05, 0.5, -0.5])).float(), torch.tensor([1.0, -2.0, 0.5, 1.0, 1.0])
+    kw = dict(ref_logp=torch.full((rows,), 150.0, device="cuda"))
+    if ref != "logp":
+        y = x.clone()
+        y[:4, 1] = -math.inf if ref == "masked" else math.nan
+        y[4, 0] = -math.inf if ref == "masked" else math.nan
+        kw = dict(ref_logits=y.cuda())
+    xd = x.double().requires_grad_(True)
+    ratio = torch.exp(torch.log_softmax(xd, -1).gather(1, ids[:, None])[:, 0] - old.double())
+    want = torch.maximum(-adv.double() * ratio, -adv.double() * ratio.clamp(0.8, 1.2)).mean()
+    (want * g).backward()
+    leaf = x.cuda().requires_grad_(True)
+    loss, got_logp, kl = ops.policy_loss(leaf, ids.cuda(), old.cuda(), adv.cuda(), **kw)
+    (loss * g).backward()
+    assert bool((kl.isnan() if ref == "nan" else kl == math.inf).all())
+    # a p and a log-prob are off by dl at most (34 roundings of an argument below 30, V / 256 + 16 of a sum), a row's term by |A| ratio times
+    # twice that, its gradient by four times, then the rounding of the result
+    dl = 34 * 2.0 ** -23 + (V / 256 + 16) * 2.0 ** -24
+    size = (adv.abs() * ratio.detach())
+    assert abs(float(loss.detach()) - float(want.detach())) <= float(size.mean()) * 2 * dl + 2.0 ** -23 * abs(float(want.detach()))
+    one = torch.zeros(rows, V, dtype=torch.float64).scatter_(1, ids[:, None], 1.0)
+    tol = 4 * dl * size[:, None] / rows * (one + torch.softmax(xd.detach(), -1)) + torch.finfo(dtype).eps / 2 * (1 + 1e-5) * xd.grad.abs() + 1e-38
+    assert bool(((leaf.grad.cpu().double() - xd.grad).abs() <= tol).all())
