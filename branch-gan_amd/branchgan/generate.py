@@ -43,7 +43,8 @@ def generate(model, input_ids, max_new_tokens=128, do_sample=False, temperature=
     several return sequences are not offered.  `generator`: a torch.Generator on the device for reproducible sampling.
     `cache_bits` 4 or 8: decode over a quantised cache (models without dropout only).  `return_logprobs=True`: -> (ids, log-probs of the
     new tokens (B, max_new_tokens) fp32 under the policy that chose them - softmax(logits / temperature) when sampling,
-    softmax(logits) when greedy -, 0 where a finished sequence was filled up): the `oldLogProbs` of losses.clippedPolicyLoss."""
+    softmax(logits) when greedy -, 0 where a finished sequence was filled up): the `oldLogProbs` of losses.clippedPolicyLoss, whose
+    mask is liveTokens of the new ids (a log-prob of 0 does not tell: a token of probability 1 has it too)."""
     if num_beams != 1 or num_return_sequences != 1:
         raise NotImplementedError("generate: num_beams = num_return_sequences = 1 only")
     if do_sample and temperature <= 0:
@@ -117,6 +118,15 @@ def generate(model, input_ids, max_new_tokens=128, do_sample=False, temperature=
         score(step.logits[:, -1], tok)
     seq = torch.cat([ids] + new, dim=1)
     return (seq, torch.cat(logps, dim=1)[:, :max_new_tokens]) if return_logprobs else seq
+
+
+def liveTokens(newIDs, eos_token_id):
+    """(B, n) generated ids, without their prompt -> (B, n) bool: True up to a sequence's first `eos_token_id` and there, False for what
+    `generate` filled it up with behind (also where that is the same id); all True with None."""
+    if eos_token_id is None:
+        return torch.ones_like(newIDs, dtype=torch.bool)
+    ends = newIDs == eos_token_id
+    return ends.long().cumsum(1) - ends.long() == 0
 
 
 def generateTexts(generator, data, settings, device, tokenizer=None, generationLength=128, startIndex=None, maxNumSamples=None,

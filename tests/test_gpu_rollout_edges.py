@@ -122,3 +122,35 @@ def test_a_kl_that_is_reported_only_stays_out_of_the_update(dtype, V, g, ref):
     one = torch.zeros(rows, V, dtype=torch.float64).scatter_(1, ids[:, None], 1.0)
     tol = 4 * dl * size[:, None] / rows * (one + torch.softmax(xd.detach(), -1)) + torch.finfo(dtype).eps / 2 * (1 + 1e-5) * xd.grad.abs() + 1e-38
     assert bool(((leaf.grad.cpu().double() - xd.grad).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("pad_is_eos", [False, True])
+def test_what_fills_up_a_finished_sequence_does_not_train(pad_is_eos):
+    """Rollouts with an end of sequence, masked by liveTokens: the padding behind it has no gradient and no part in the loss's mean."""
+    from branchgan import configs, generate, losses, models
+    torch.manual_seed(9)
+    lm = models.make_lm(configs.LMConfig("gpt_neox", 19, 64, 2, 2, 64)).cuda()
+    B, P, new, eos = 8, 5, 30, 3
+    prompt = torch.randint(0, 19, (B, P), device="cuda")
+    seq, old = generate.generate(lm, prompt, max_new_tokens=new, do_sample=True, cache_bits=4, return_logprobs=True, eos_token_id=eos,
+                                 pad_token_id=eos if pad_is_eos else 0, generator=torch.Generator(device="cuda").manual_seed(2))
+    live = generate.liveTokens(seq[:, P:], eos)
+    ends = [row.index(eos) + 1 if eos in row else new for row in seq[:, P:].tolist()]
+    assert live.sum(1).tolist() == ends and min(ends) < new and not old[~live].any()
+    adv = torch.randn(B, new, generator=torch.Generator().manual_seed(3)).cuda()
+    logits = lm(input_ids=seq[:, :-1], returnLmLogits=True).logits
+    logits.retain_grad()
+    behind = lambda t: torch.nn.functional.pad(t, (P - 1, 0))
+    loss, logp, _ = losses.clippedPolicyLoss(logits, seq[:, 1:], behind(old), behind(adv), mask=behind(live.float()))
+    loss.backward()
+    grad = logits.grad[:, P - 1:]
+    assert not grad[~live].any() and not logits.grad[:, :P - 1].any() and not logp[:, P - 1:][~live].any() and bool((grad[live].abs().amax(-1) > 0).any())
+    x = logits.detach().cpu().double()[:, P - 1:][live.cpu()].requires_grad_(True)
+    tok = torch.log_softmax(x, -1).gather(1, seq[:, P:][live].cpu()[:, None])[:, 0]
+    r, a = torch.exp(tok - old[live].cpu().double()), adv[live].cpu().double()
+    want = torch.maximum(-a * r, -a * r.clamp(0.8, 1.2)).sum() / sum(ends)
+    want.backward()
+    # the vocabulary is small: a log-prob is off by 34 * 2^-23 + 17 * 2^-24 < 6e-6, a term by |A| r twice that, a gradient by four times
+    size = (a.abs() * r.detach()).max()
+    assert abs(float(loss.detach()) - float(want.detach())) <= float(size) * 1.2e-5
+    assert float((grad[live].cpu().double() - x.grad).abs().max()) <= float(size) / sum(ends) * 2 * 2.4e-5

@@ -5,6 +5,13 @@ import torch
 B, T, V = 3, 4, 1031
 
 
+def test_live_tokens():
+    from branchgan import generate
+    ids = torch.tensor([[5, 2, 0, 0, 0], [2, 2, 2, 2, 2], [1, 3, 4, 5, 6], [0, 0, 7, 2, 9], [1, 1, 1, 1, 2]])
+    want = torch.tensor([[1, 1, 0, 0, 0], [1, 0, 0, 0, 0], [1, 1, 1, 1, 1], [1, 1, 1, 1, 0], [1, 1, 1, 1, 1]]).bool()
+    assert torch.equal(generate.liveTokens(ids, 2), want) and generate.liveTokens(ids, None).all() and generate.liveTokens(ids[:, :0], 2).shape == (5, 0)
+
+
 def policy_calls(monkeypatch):
     """ops.policy_loss without its launches: the shape structs that the calls got, copied."""
     from branchgan import _capi, ops
