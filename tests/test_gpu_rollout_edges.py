@@ -154,3 +154,51 @@ def test_what_fills_up_a_finished_sequence_does_not_train(pad_is_eos):
     size = (a.abs() * r.detach()).max()
     assert abs(float(loss.detach()) - float(want.detach())) <= float(size) * 1.2e-5
     assert float((grad[live].cpu().double() - x.grad).abs().max()) <= float(size) / sum(ends) * 2 * 2.4e-5
+
+
+@pytest.mark.parametrize("shape,cut,g", [((2500, 40), slice(None), 0.5), ((5000, 1, 33), slice(None), 1.0), ((70000, 2, 17), slice(1, None), 1.0),
+                                         ((70000, 2, 17), slice(1, None), -0.25)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("with_ref", [False, True])
+def test_more_rows_and_groups_than_a_launch_takes(shape, cut, g, dtype, with_ref):
+    """A gradient computed again over more rows than its launch has workgroups, and more groups of rows than a grid's second dimension."""
+    from branchgan import ops
+    gen = torch.Generator().manual_seed(shape[0] + shape[-1])
+    V, view = shape[-1], lambda t: t[:, cut] if len(shape) == 3 else t
+    full = [torch.randn(shape, generator=gen).to(dtype) for _ in range(2)]
+    x, y = [view(t).reshape(-1, V).double() for t in full]
+    rows = x.shape[0]
+    lead = view(full[0]).shape[:-1]
+    ids = torch.randint(0, V, (rows,), generator=gen)
+    lx, ly = torch.log_softmax(x, -1), torch.log_softmax(y, -1)
+    logp = lx.gather(1, ids[:, None])[:, 0]
+    old, adv = (logp + 0.3 * torch.randn(rows, generator=gen)).float(), torch.randn(rows, generator=gen)
+    ratio = torch.exp(logp - old.double())
+    for end in (0.8, 1.2):                                                   # off the clip's ends, where the gradient jumps
+        old = torch.where((ratio - end).abs() < 1e-3, old + 0.01, old)
+    ratio, a, beta = torch.exp(logp - old.double()), adv.double(), 0.1 if with_ref else 0.0
+    w = (torch.arange(rows) % 5 > 0).double()
+    plain, clipped = -a * ratio, -a * ratio.clamp(0.8, 1.2)
+    slope, p, gap = torch.where(plain >= clipped, plain, 0.0), lx.exp(), lx - ly
+    kl = (p * gap).sum(-1) if with_ref else torch.zeros(rows, dtype=torch.float64)
+    want = (w * (torch.maximum(plain, clipped) + beta * kl)).sum() / w.sum()
+    one = torch.zeros_like(p).scatter_(1, ids[:, None], 1.0)
+    grad = g / w.sum() * w[:, None] * (slope[:, None] * (one - p) + beta * p * (gap - kl[:, None]))
+    leaf = full[0].cuda().requires_grad_(True)
+    dev = lambda t: t.cuda().view(lead)
+    loss, got_logp, got_kl = ops.policy_loss(view(leaf), dev(ids), dev(old), dev(adv), weights=dev(w.float()), kl_coef=beta,
+                                             ref_logits=view(full[1].cuda()) if with_ref else None)
+    (loss * g).backward()
+    # dl: a p, and a log-prob; the full KL 4 dl of its terms' magnitudes and 4 dl; a row's term 2 dl |A| ratio, its gradient 4 dl of its parts
+    dl = 34 * 2.0 ** -23 + (V / 256 + 16) * 2.0 ** -24
+    kl_tol = 4 * dl * (p * gap.abs()).sum(-1) + 4 * dl + 2.0 ** -23 * kl.abs()
+    near = lambda got, ref, tol: bool((((got.cpu().double().reshape(ref.shape) - ref).abs() <= tol) | (w == 0)).all())
+    assert near(got_logp, logp, dl + 2.0 ** -24 * logp.abs()) and near(got_kl, kl, kl_tol)
+    term_tol = 2 * dl * (a * ratio).abs() + beta * kl_tol
+    assert abs(float(loss.detach()) - float(want)) <= float((w * term_tol).sum() / w.sum()) + 2.0 ** -23 * abs(float(want))
+    tol = 4 * dl * (a * ratio).abs()[:, None] * (one + p) + beta * p * (4 * dl * (gap.abs() + kl.abs()[:, None]) + 4 * dl + kl_tol[:, None])
+    tol = tol * abs(g) / w.sum() * w[:, None] + torch.finfo(dtype).eps / 2 * (1 + 1e-5) * grad.abs() + 1e-38
+    got = leaf.grad.cpu().double()
+    assert bool(((view(got).reshape(-1, V) - grad).abs() <= tol).all())
+    view(got).zero_()
+    assert not got.any()
