@@ -202,3 +202,44 @@ def test_more_rows_and_groups_than_a_launch_takes(shape, cut, g, dtype, with_ref
     assert bool(((view(got).reshape(-1, V) - grad).abs() <= tol).all())
     view(got).zero_()
     assert not got.any()
+
+
+@pytest.mark.parametrize("family", ["gpt2", "gpt_neox"])
+@pytest.mark.parametrize("fused_path", [True, False])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_a_chunk_through_the_model_is_its_tokens_one_by_one(family, fused_path, bits, monkeypatch):
+    """models.CachePast with several new tokens, sequences of uneven length and padding: the logits of each token decoded alone, and nothing
+    written behind a sequence's last one."""
+    from branchgan import configs, fused, kvcache, models, ops
+    monkeypatch.setattr(fused, "ENABLED", fused_path)
+    torch.manual_seed(6)
+    lm = models.make_lm(configs.LMConfig(family, 211, 128, 2, 4, 128)).cuda()
+    B, T, cap, held, counts = 4, 7, 64, (40, 0, 33, 12), (7, 5, 0, 1)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    ids = torch.randint(0, 211, (B, T), device="cuda")
+    gen = torch.Generator().manual_seed(bits)
+    caches = [kvcache.QuantizedKVCache(2, B, 4, cap, 32, bits=bits) for _ in range(2)]
+    for l in range(2):
+        k, v = [torch.randn(B, 4, cap, 32, generator=gen).cuda() for _ in range(2)]
+        for c in caches:
+            ops.kv_cache_append(c.layer(l), k, v)
+    before = [ops.kv_cache_read(caches[0].layer(l), cap, dtype=torch.float32) for l in range(2)]
+    start = i32(held)
+    def forward(cache, tokens, at, n, most):
+        pos = at[:, None] + torch.arange(tokens.shape[1], device="cuda", dtype=torch.int32)
+        return lm(input_ids=tokens, position_ids=pos, textualPast=models.CachePast(cache, at, n, max_keys=most), returnLmLogits=True).logits.float()
+    with torch.no_grad():
+        whole = forward(caches[0], ids, start, i32(counts), max(held) + T)
+        for t in range(T):
+            n = i32([int(t < c) for c in counts])
+            one = forward(caches[1], ids[:, t:t + 1], start + t, n, cap)
+            # layer 0's keys are the same numbers up to fp32 rounding; a code of layer 1 may flip at its border, a step of 1 / 7 of a key's maximum
+            for b in range(B):
+                if t < counts[b]:
+                    torch.testing.assert_close(whole[b, t], one[b, 0], rtol=0, atol=0.02 * float(whole.abs().max()))
+    for l in range(2):
+        for was, now in zip(before[l], ops.kv_cache_read(caches[0].layer(l), cap, dtype=torch.float32)):
+            for b in range(B):
+                new = torch.zeros(cap, dtype=torch.bool)
+                new[held[b]:held[b] + counts[b]] = True
+                assert torch.equal(was[b][:, ~new], now[b][:, ~new]) and (counts[b] == 0 or not torch.equal(was[b][:, new], now[b][:, new]))
