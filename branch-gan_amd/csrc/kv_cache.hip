@@ -1,7 +1,11 @@
 // The quantised key / value cache: bg_kv_cache_append writes new tokens into it, bg_kv_cache_read gives back the values it holds.
 //
 // Per (token, head, 32 channels), a = the largest magnitude, L = 7 or 127:
-//   s = bf16(fp32(a / L)),  c = clamp(round-half-even(x / s), -L, L),  the value held is s * c (exact in fp32: 8 + 7 bits at most)
+//   s = bf16(a * fp32(1 / L)) (an fp32 product),  c = clamp(round-half-even(x / s), -L, L),  the value held is s * c (exact in fp32: 8 + 7
+// bits at most)
+// The product is what a tensor divided by a number is on this device (compared for all of [1, 2)), so elementary tensor code
+// gives the same cache bit for bit.  bf16(fp32(a / L)) is the other neighbour for 70 (4 bits) and 1 (8 bits) of the 2^23 fp32
+// mantissas, where a / L lies halfway between two bf16 numbers to the last bit of fp32 and either is as near; never for bf16 a.
 // s is 0 (the group reads as zeros) when it would be subnormal; a group with a NaN, an infinity or a magnitude above 2^127 gets
 // s = NaN and reads as NaN, so a broken activation shows instead of turning into a large finite number.
 // The code is that of the REAL quotient x / s, not of a rounded one: with r = 1 / s correctly rounded, q0 = x r, q = q0 + (x - q0 s) r
@@ -26,13 +30,9 @@ template <int CTRL> __device__ __forceinline__ uint32_t dpp_max(uint32_t x) {
 }
 
 // Scale bits of a group from the bits of its largest magnitude (ordered as integers: finite < inf < NaN); rs = 1 / s or 0.
-// The quotient a / L is a product with 1 / L and one corrective step, which makes it the rounded one (compared with the division for
-// every float up to 2^127, both L); for bf16 a the product alone gives the same bf16 s (compared for all of them).
-template <typename T, int TOP> __device__ __forceinline__ uint16_t group_scale(uint32_t amax_bits, float& s, float& rs) {
+template <int TOP> __device__ __forceinline__ uint16_t group_scale(uint32_t amax_bits, float& s, float& rs) {
   const float a = __uint_as_float(amax_bits);
-  float q = a * (1.0f / TOP);
-  if constexpr (sizeof(T) == 4) q = __builtin_fmaf(__builtin_fmaf(-q, (float)TOP, a), 1.0f / TOP, q);
-  uint32_t b = f32_to_bf16_bits(q);
+  uint32_t b = f32_to_bf16_bits(a * (1.0f / TOP));
   if (b < 0x0080u) b = 0;
   const bool broken = amax_bits > 0x7F000000u;
   s = broken ? 0.f : bf16_bits_to_f32(b);
@@ -81,7 +81,7 @@ __global__ __launch_bounds__(256) void kv_append_token_kernel(KvArgs a, const T*
   m = dpp_max<0x140>(m);
   m = max(m, (uint32_t)__shfl_xor((int)m, 16));
   float s, rs;
-  const uint16_t sb = group_scale<T, L::TOP>(m, s, rs);
+  const uint16_t sb = group_scale<L::TOP>(m, s, rs);
   const uint32_t code = rs == 0.f ? (uint32_t)L::OFF : code_bits<T, L::OFF>(x, s, rs) & (BITS == 4 ? 15u : 255u);
   uint8_t* tile = a.data + b * a.c_sb + h * a.c_sh + (int64_t)(pos / KV_TILE) * L::BYTES;
   const int key = pos % KV_TILE, g = c / KV_GROUP, kg = (c / 8) % 4;
@@ -224,7 +224,7 @@ __device__ __forceinline__ void append_tiles(const KvArgs& a, const T* src0, int
       m = dpp_max<0xB1>(m);                                    // the 4 lanes of a group are adjacent
       m = dpp_max<0x4E>(m);
       float s, rs;
-      const uint16_t scale = group_scale<T, L::TOP>(m, s, rs);
+      const uint16_t scale = group_scale<L::TOP>(m, s, rs);
       const int key = 8 * oct + e;
       if (in && kg == 0) *(uint16_t*)(img + CODE_BYTES + L::scale_at(key, g)) = scale;
       uint32_t kw[BITS / 4];

@@ -486,7 +486,7 @@ int bg_graph_replace_memset_nodes(void* graph, int* n_replaced);
  * Inference/GenerateTexts.py:19, whose cache holds the model's own dtype: none of this has a counterpart there).
  *
  * Every 32 channels of a token's key (value) of one head share a scale.  With a = the largest magnitude among them and L = 7
- * (4 bits) or 127 (8 bits):  s = bf16(fp32(a / L)),  c = clamp(round-half-even(x / s), -L, L),  held value = s * c.
+ * (4 bits) or 127 (8 bits):  s = bf16(a * fp32(1 / L)), an fp32 product (not always bf16(a / L) where that is a tie),  c = clamp(round-half-even(x / s), -L, L),  held value = s * c.
  * s is 0 - the group reads as zeros - when it would be below 2^-126; a group holding a NaN, an infinity or a magnitude above
  * 2^127 reads as NaN.  A value takes 0.5625 (1.0625) bytes.
  *

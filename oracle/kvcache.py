@@ -8,14 +8,14 @@ GROUP = 32
 
 
 def held_values(x, bits):
-    """x (..., Dh) -> the values the cache holds for it, float64.  Per 32 channels: s = bf16(fp32(max|x| / L)), c =
+    """x (..., Dh) -> the values the cache holds for it, float64.  Per 32 channels: s = bf16(max|x| * fp32(1 / L)), an fp32 product, c =
     clamp(round-half-even(x / s), -L, L); s below 2^-126 holds zeros; a NaN, an infinity or a magnitude above 2^127 makes the
     group NaN."""
     top = 7 if bits == 4 else 127
     g = x.double().unflatten(-1, (-1, GROUP))
     a = g.abs().amax(-1, keepdim=True)
     broken = ~(a <= 2.0 ** 127)
-    s = (torch.where(broken, torch.zeros_like(a), a) / top).float().bfloat16().double()
+    s = (torch.where(broken, torch.zeros_like(a), a).float() * torch.tensor(1 / top, dtype=torch.float32)).bfloat16().double()
     s = torch.where(s < 2.0 ** -126, torch.zeros_like(s), s)
     c = torch.round(torch.where(broken, torch.zeros_like(g), g) / torch.where(s == 0, torch.ones_like(s), s)).clamp(-top, top)
     return torch.where(broken, torch.full_like(g, math.nan), c * s).flatten(-2)

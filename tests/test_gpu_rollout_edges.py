@@ -41,30 +41,6 @@ def test_sums_over_many_keys_do_not_lose_digits(Dh, B, H, G, T):
     assert float((lse.double() - torch.log(seen.double()).cuda()).abs().max()) < 2.0 ** -19
 
 
-@pytest.mark.parametrize("bits", [4, 8])
-@pytest.mark.parametrize("T", [1, 2])
-def test_scales_next_to_a_tie(bits, T):
-    """fp32 maxima on, one step below and one above L t, t halfway between two bf16 numbers: the scale is the quotient's, rounded to fp32
-    and from there to bf16 - worked out here in whole numbers, and read off the held value of the maximum itself, L s."""
-    from branchgan import kvcache, ops
-    top = 7 if bits == 4 else 127
-    t = torch.arange(257, 512, 2).double() / 256                             # the 128 ties of [1, 2)
-    a = torch.cat([torch.nextafter((top * t).float(), torch.tensor(to)) for to in (0.0, math.inf)] + [(top * t).float()])
-    a = torch.cat([a * 2.0 ** e for e in (-100, 0, 3, 90)])
-    quotient = (a.double() / top).float()                                    # 53 bits hold enough of a quotient of 24 by 7 to round it again
-    u = quotient.view(torch.int32).long()
-    scale = (((u + 0x7FFF + ((u >> 16) & 1)) >> 16) << 16).int().view(torch.float32)
-    x = torch.zeros(len(a), 1, T, 64)
-    x[:, 0, :, 3], x[:, 0, :, 40] = a[:, None], -a[:, None]
-    x[:, 0, :, 50] = 0.37 * a[:, None]
-    layer = kvcache.QuantizedKVCache(1, len(a), 1, T, 64, bits=bits).layer(0)
-    ops.kv_cache_append(layer, x.cuda(), x.flip(-1).contiguous().cuda())
-    k, v = [r.cpu() for r in ops.kv_cache_read(layer, T, dtype=torch.float32)]
-    for t in range(T):
-        assert torch.equal(k[:, 0, t, 3], top * scale) and torch.equal(k[:, 0, t, 40], -top * scale)
-    assert torch.equal(k.double(), OK.held_values(x, bits)) and torch.equal(v.double(), OK.held_values(x.flip(-1), bits))
-
-
 def test_saved_tensors_that_come_back_in_a_layout_of_their_own_each_time():
     """Hooks that answer dense, as saved, dense again: the same gradient from every backward."""
     from branchgan import ops
@@ -243,3 +219,32 @@ def test_a_chunk_through_the_model_is_its_tokens_one_by_one(family, fused_path, 
                 new = torch.zeros(cap, dtype=torch.bool)
                 new[held[b]:held[b] + counts[b]] = True
                 assert torch.equal(was[b][:, ~new], now[b][:, ~new]) and (counts[b] == 0 or not torch.equal(was[b][:, new], now[b][:, new]))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("T", [1, 2])
+def test_scales_next_to_a_tie_are_the_documented_product(bits, T):
+    """fp32 maxima on, one step below and one above L t, t halfway between two bf16 numbers, where a product with 1 / L and a quotient by L can
+    round to different neighbours: the scale is bf16(a * fp32(1 / L)), worked out here in whole numbers, and what a tensor divided by the
+    number L gives on the same device.  It is read off the held value of the maximum itself, L s."""
+    from branchgan import kvcache, ops
+    top = 7 if bits == 4 else 127
+    t = torch.arange(257, 512, 2).double() / 256                             # the 128 ties of [1, 2)
+    a = torch.cat([torch.nextafter((top * t).float(), torch.tensor(to)) for to in (0.0, math.inf)] + [(top * t).float()])
+    a = torch.cat([a * 2.0 ** e for e in (-100, 0, 3, 90)])
+    def bf16_of(x):                                                          # fp32 -> bf16, half to even, on the bits
+        u = x.view(torch.int32).long()
+        return (((u + 0x7FFF + ((u >> 16) & 1)) >> 16) << 16).int().view(torch.float32)
+    reciprocal = torch.tensor(1 / top, dtype=torch.float32)
+    scale = bf16_of((a.double() * reciprocal.double()).float())             # 48 bits: exact in a double, rounded to fp32 once
+    assert not torch.equal(scale, bf16_of((a.double() / top).float()))       # the points tell the two apart
+    assert torch.equal(scale, bf16_of((a.cuda() / top).cpu()))
+    x = torch.zeros(len(a), 1, T, 64)
+    x[:, 0, :, 3], x[:, 0, :, 40] = a[:, None], -a[:, None]
+    x[:, 0, :, 50] = 0.37 * a[:, None]
+    layer = kvcache.QuantizedKVCache(1, len(a), 1, T, 64, bits=bits).layer(0)
+    ops.kv_cache_append(layer, x.cuda(), x.flip(-1).contiguous().cuda())
+    k, v = [r.cpu() for r in ops.kv_cache_read(layer, T, dtype=torch.float32)]
+    for t in range(T):
+        assert torch.equal(k[:, 0, t, 3], top * scale) and torch.equal(k[:, 0, t, 40], -top * scale)
+    assert torch.equal(k.double(), OK.held_values(x, bits)) and torch.equal(v.double(), OK.held_values(x.flip(-1), bits))
