@@ -6,6 +6,7 @@ torch supplies device memory and autograd bookkeeping only; there is no CPU or e
 import ctypes
 import itertools
 import math
+import warnings
 
 import torch
 
@@ -1019,10 +1020,11 @@ def policy_loss(logits, ids, old_logp, advantages, weights=None, ref_logp=None, 
     e.g. logits[:, :-1], is read where it lies).  ids (...) int64: the
     sampled tokens; old_logp (...): their log-probs when they were sampled; advantages (...); weights (...) or None: per token,
     0 = does not count; ref_logits (like logits) -> the KL over the vocabulary, or ref_logp (...) -> exp(d) - d - 1 of the
-    sampled token, d = ref_logp - logp; with neither kl is 0 and kl_coef without effect, with kl_coef 0 kl is reported only (whatever it is, also
+    sampled token, d = ref_logp - logp; with neither kl is 0 and kl_coef without effect (a warning says so), with kl_coef 0 kl is reported only (whatever it is, also
     infinite, loss and gradient do not contain it).  All log-probs are those of softmax(logits / temperature).  denominator: what the sum over tokens
     is divided by (a number, or a one-element tensor on the device - a token count over micro-batches or ranks); default the
-    sum of the weights that count.  -> (loss fp32 scalar, logp (...), kl (...); the last two carry no gradient).
+    sum of the weights that count.  -> (loss fp32 scalar, logp (...), kl (...); the last two carry no gradient,
+    and none flows into anything but logits).
     Captured into a HIP graph, forward and backward belong into the same capture, made while no eager autograd graph of the same
     leaves is alive (autograd binds a leaf's gradient to the stream of its first use: graphs.GraphedTrainStep)."""
     C.require_cuda(logits)
@@ -1038,6 +1040,8 @@ def policy_loss(logits, ids, old_logp, advantages, weights=None, ref_logp=None, 
         raise ValueError("policy_loss: ref_logits must be like logits in shape, dtype and device")
     if ref_logits is not None and ref_logp is not None:
         raise ValueError("policy_loss: ref_logits or ref_logp, not both")
+    if kl_coef != 0 and ref_logits is None and ref_logp is None:
+        warnings.warn("policy_loss: kl_coef without ref_logits or ref_logp: there is no KL term")
     if not temperature > 0 or not clip_low >= 0 or not clip_high >= 0:
         raise ValueError(f"policy_loss: temperature {temperature} must be positive, the clip range ({clip_low}, {clip_high}) not negative")
     if denominator is not None:

@@ -23,6 +23,18 @@ def policy_calls(monkeypatch):
     return calls
 
 
+def test_a_kl_weight_without_a_reference_is_told(monkeypatch, recwarn):
+    from branchgan import ops
+    policy_calls(monkeypatch)
+    x = [torch.zeros(4, V), torch.zeros(4, dtype=torch.long), torch.zeros(4), torch.zeros(4)]
+    ops.policy_loss(*x)
+    ops.policy_loss(*x, ref_logp=torch.zeros(4), kl_coef=0.1)
+    ops.policy_loss(*x, ref_logits=x[0], kl_coef=0.1)
+    assert not [w for w in recwarn if "KL" in str(w.message)]
+    with pytest.warns(UserWarning, match="no KL term"):
+        ops.policy_loss(*x, kl_coef=0.1)
+
+
 @pytest.mark.parametrize("with_ref", [False, True])
 def test_each_backward_walks_the_layout_that_the_hooks_returned(monkeypatch, with_ref):
     """Saved-tensor hooks that answer dense, as saved, dense again: every call's strides are those of the tensors it was given."""
