@@ -24,11 +24,12 @@
 // Work.  Four waves per workgroup take turns round robin; the key range is split over workgroups when there are too few of
 //   them to fill 256 CUs (kv_attn_plan), the partial states joined by a second kernel.
 // Bound.  One token: HBM, 0.5625 or 1.0625 bytes per cached value.  Measured: 8 sequences of 65537 keys, 8 heads of 128, four query heads
-//   each, 4 bits, 604 MB in 115 us (5.3 TB/s; the launches of the call included, the part that stays in the last-level cache too);
-//   64 uneven sequences of up to 2047 keys, 16 heads of 64, 87 MB in 21 us (4.2 TB/s); 16 of up to 4001, 8 heads of 256, 8 bits,
+//   each, 4 bits, 604 MB in 117 us (5.2 TB/s; the launches of the call included, the part that stays in the last-level cache too);
+//   64 uneven sequences of up to 2047 keys, 16 heads of 64, 87 MB in 22 us (4.0 TB/s); 16 of up to 4001, 8 heads of 256, 8 bits,
 //   float32 queries, 162 MB in 41 + 5 us (3.5 TB/s: the longest sequences finish alone).  Many rows: vector work - 128 keys x 16 rows
 //   of 64 channels are some 930 vector instructions of a wave (exponentials, scales, splitting P, unpacking) against 64 matrix
-//   ones; 67 tokens of 4 sequences of 16 heads against about 2000 keys in 19 + 4 us.
+//   ones; 67 tokens of 4 sequences of 16 heads against about 2000 keys in 20 + 4 us, of which that
+//   work is less than half: two turns a wave do not hide the prologue, the joins and every tile's own reading of the keys.
 #include "kv_cache.h"
 
 namespace bg {
@@ -104,8 +105,11 @@ union Frag {
 // (The two constants sit in a vector and a scalar register: as literals they would make the mask-or two instructions.)
 // What the offset adds to an output is taken off turn by turn (step by step where there are many rows): sums that kept it grow with
 // the number of keys while the output, an average, shrinks - over 65536 random keys 18 % of the bf16 outputs then were not the rounded
-// ones, now 0.8 %.  16 subtractions a turn at heads of 64 (64 sequences 22.9 us either way, 67 tokens 21.5 -> 21.8); signed codes
+// ones, now 0.8 %.  16 subtractions a turn at heads of 64 (64 sequences 21.8 -> 22.2 us, 67 tokens 21.7 -> 21.9); signed codes
 // for bf16 queries would cost 26.3 and 23.5.
+// To a score, a product of its own for every key, the offset adds rounding of some 24 sum|q| 2^-24 times the key's scale s: a
+// hundred-thousandth of what half a code step, s / 2 per channel, may be off in the cache already (2e-7 of a key's largest magnitude at
+// heads of 64 and queries of size 1).
 // 4 bits, fp32 queries: sums of c + 24 would cost 2 to 3 bits that fp32 results show (error 4e-6 against 4e-7), so the codes come
 // signed, by the instruction that reads a signed nibble as sixteenths - twice the instructions.
 // 8 bits: signed bytes, converted (a conversion that takes its byte from the word, and half a pack).
@@ -234,7 +238,8 @@ template <typename T, int BITS, int DH, int RR> struct DecodeShape {
   static constexpr int RL = RR > NG ? RR / NG : 1;                           // rows a lane holds scores of
   // a turn's codes in flight, K and V: whole (16 registers each at most), halves or quarters
   static constexpr int KT = DH * BITS <= 256 ? 8 : DH * BITS <= 1024 ? 4 : 2, VT = KT / 2;
-  // waves per SIMD: small heads are bound by vector work and latency as much as by memory
+  // waves per SIMD: small heads are bound by vector work and latency as much as by memory.  At RR = 2 that leaves <fp32, 4, 32>, <bf16,
+  // 4, 64> and <bf16, 8, 32> 3 to 8 registers short, at RR = 4 the heads of 256 4 to 8: spilled around the loop
   static constexpr int WAVES = DH * BITS > 256 || RR == 4 ? 2 : DH * BITS == 256 && sizeof(T) == 4 ? 3 : 4;
 };
 
@@ -562,7 +567,8 @@ __global__ __launch_bounds__(64 * KW, (DecodeShape<T, BITS, DH, RR>::WAVES)) voi
 }
 
 // ---- many rows -------------------------------------------------------------------------------------------------------------------
-// steps of a turn, so that the codes in flight fit the registers beside the accumulators; waves per SIMD: one where two would spill
+// steps of a turn, so that the codes in flight fit the registers beside the accumulators; waves per SIMD: one where two would spill far
+// more than the 3 registers that <bf16, 4, 256> and <fp32, 8, 256> still do
 template <int BITS, int DH> constexpr int kv_steps() { return DH * BITS <= 512 ? 4 : 2; }
 template <int BITS, int DH> constexpr int kv_waves() { return DH == 256 || (DH == 128 && BITS == 4) ? 1 : 2; }
 
@@ -832,8 +838,10 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(KvAttnArgs a, uint32_
   if (a.lse && lane == 0) a.lse[((int64_t)b * a.kv.H * a.G + hq) * a.kv.T + t] = any ? (M + __log2f(S)) * 0.6931471805599453f : -INFINITY;
 }
 
-// Which kernel, and how many workgroups share a row tile's key range: enough to give every CU two (512), none with less than one turn for
-// each wave.  512 is what is resident at once: 640, 768 and 1024 took 140, 127 and 121 us against 116 for 8 sequences of 65537 keys
+// Which kernel, and how many workgroups share a row tile's key range: at least two per CU (512), none with less than one turn for
+// each wave.  512 is what is resident at once for heads of 128 and 256 and few rows, by their registers (smaller heads: three or four per
+// CU; many rows at heads of 256, or of 128 in 4 bits: one); the rule rounds up, so it is met exactly only where the heads of the
+// batch divide 512 (24 sequences of 12 heads: 576).  More was slower where it was measured: 640, 768 and 1024 took 140, 127 and 121 us against 116 for 8 sequences of 65537 keys
 // (8 heads of 128, 4 bits), 58, 60 and 56 against 50 for 16 uneven ones of up to 4001 (8 heads of 256, 8 bits).  Every sequence
 // is split evenly: splits of a fixed number of turns, fewer for short sequences, leave CUs idle and were a sixth slower.
 struct KvPlan {

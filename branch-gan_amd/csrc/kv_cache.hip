@@ -14,7 +14,7 @@
 // L + 1/2.  Adding 1.5 * 2^23 + offset rounds q to an integer, half to even, in the float's low bits, where packing takes it from.
 //
 // Bound by HBM for prompts (bytes in + 0.56 or 1.06 bytes per value out): 16 sequences of up to 2017 tokens, 8 heads of 256, bf16 to
-// 4 bits, 289 MB: written in 77 us (3.8 TB/s), read back in 64 (4.5; a copy reaches 4.8).  By launch and latency for one token: 64
+// 4 bits, 289 MB: written in 76 us (3.8 TB/s), read back in 62 (4.7; a copy reaches 4.8).  By launch and latency for one token: 64
 // sequences of 16 heads of 64 in 3.4 us, read back in 3.8.
 #include "kv_cache.h"
 

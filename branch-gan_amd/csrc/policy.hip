@@ -10,8 +10,12 @@
 // whole of value and gradient is logits in, dlogits out.  The gradient is the one for g_loss = 1; bg_policy_loss_bwd does it over
 // when the loss was scaled after all.  Rows too long for the registers take policy_rows_kernel (forward) and policy_grad_kernel
 // (backward), one more reading of the logits.
-// Measured, bf16 with the gradient: 2047 rows of 50257 in 87 us (4.7 TB/s), 8184 rows of 50304 with a reference in 609 us (4.1
-// TB/s; a copy reaches 4.8); the weights' sum and the total take 5 us each at 2047 rows, a backward call with nothing to do 4.
+// Measured, bf16 with the gradient: 2047 rows of 50257 in 85 us (4.8 TB/s), 8184 rows of 50304 with a reference in 609 - 620 us
+// (4.0 TB/s; a copy reaches 4.8); the weights' sum and the total, one workgroup each, take 3 and 5 us at 2047 rows, 5 and 13 at 8184, a
+// backward call with nothing to do 4.  A loss that was scaled: 118 -> 174 us and 622 -> 1118 us a call.
+// A thread works through all NV vectors of its kernel, whatever V is: 2047 rows of 32000 take as long as of 50257.  With a reference
+// the kernels of 13 vectors spill 37 (512 threads) and 84 registers (1024: fp32 from V = 26624, bf16 from 53248): 2047 rows of 50257 in
+// fp32 421 us (257 at the copy's rate), of 65536 in bf16 368 us (168).
 #include "common.h"
 
 namespace bg {

@@ -515,7 +515,8 @@ int bg_kv_cache_read(const bg_kv_cache* cache, const void* data, void* k, void* 
 /* Attention of T new tokens over the cache (their own keys / values are in it already): q [B][Hq][T][Dh], Hq a multiple of the
  * cache's H (query head h reads cache head h / (Hq / H)); row (b, t) sees keys 0 .. start[b] + t.
  *   out = softmax(scale * q k^T) v over the values the codes stand for, fp32 sums;  lse (optional, fp32 [B][Hq][T]) = log-sum-exp.
- * A row that sees nothing (t >= counts[b], or start[b] + t < 0) is written as zeros, lse -inf.
+ * A row that sees nothing (t >= counts[b], or start[b] + t < 0) is written as zeros, lse -inf.  Sums are normalised at the end: values of
+ * more than 2^117 / (number of keys) in magnitude may come out as infinity or NaN.
  * max_keys (host): no sequence holds more keys than this after the call, 1 .. capacity - it sizes the split of the key range over
  * workgroups (keys past it are NOT read).  workspace: bg_kv_cache_attn_workspace_bytes bytes (0: may be NULL), contents irrelevant;
  * calls that overlap in time need workspaces of their own. */
